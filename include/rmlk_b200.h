@@ -485,6 +485,71 @@ RMLK_API int rmlk_b200_swiglu_pitched(rmlk_stream_t stream, int dtype, int64_t r
 RMLK_API int rmlk_b200_scale_mask_softmax(rmlk_stream_t stream, int dtype, const int64_t* lead3, int64_t cols,
                                  const int64_t* mask_strides3, float scale, const void* scores, const void* mask, void* out);
 
+/* ---- serving in 8 bits -------------------------------------------------------------------------------------------
+ * Products in 8-bit integers, a paged cache of 8-bit codes and the attention that reads it.  (No counterpart in the reference, whose
+ * ops are f16 / f32 over dense tensors.) */
+
+/* Rows of x (f32 or f16, ldx elements apart) as 8-bit integers with one scale each:
+ *   scales[m] = max(fl32(max_k |x[m,k]| / 127), 2^-126),  codes[m,k] = the integer nearest to x[m,k] / scales[m], ties to even.
+ * The codes are those of the real quotient (no rounding before the one to an integer), -127 .. 127.  A row that holds an infinity or a NaN gets
+ * the scale NaN and codes 0.  codes: int8, rows ldc apart.  Activations: one scale per token; weights [n, k]: one per channel. */
+RMLK_API int rmlk_b200_quantize_rows(rmlk_stream_t stream, int dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx, void* codes,
+                            int64_t ldc, float* scales);
+
+/* out[m,n] = (sum_k x[m,k] w[n,k]) * x_scales[m] * w_scales[n]: int8 operands (any codes, -128 too), both with k running along the rows,
+ * ldx / ldw bytes apart (multiples of 16, on 16-byte boundaries; what lies behind k in a row is not read as part of it); the sum is exact
+ * (int32: k <= 131071), converted to fp32 and scaled there.  out: f32 or f16, rows ldo elements apart, on 16-byte boundaries in its first row.
+ * `status`: device word that receives RMLK_ERR_TIMEOUT should a bounded wait of the tensor-core kernel expire, or NULL. */
+RMLK_API int rmlk_b200_matmul_i8(rmlk_stream_t stream, int out_dtype, int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx,
+                        const float* x_scales, const void* w, int64_t ldw, const float* w_scales, void* out, int64_t ldo, int* status);
+
+/* A cache of keys and values in pages of page_size tokens: k, v: int8 codes [pages, kv_heads, page_size, head_dim]; k_scales, v_scales:
+ * [pages, kv_heads] fp32, one for the block of a page and head: a value is its code times the scale.  page_size 16, 32, 64 or 128;
+ * head_dim 64 or 128; everything on 16-byte boundaries.
+ * Sequence b of a batch holds lens[b] tokens (int32, device); token t lies in slot t % page_size of page table[b * table_width + t / page_size]
+ * (int32, device).  Entries behind the last token's page are not read.  The new tokens of a call are the LAST ones of each sequence - lens counts them:
+ * rows starts[b] .. starts[b+1] of its tensors (int32 [batch + 1], device, rising from 0), or tokens / batch rows each where starts is NULL.
+ * A sequence of length 0 is one that the call passes over.  Rows behind starts[batch] are neither read nor written. */
+typedef struct rmlk_paged_cache {
+    int64_t pages, kv_heads, page_size, head_dim;
+    void* k;
+    void* v;
+    float* k_scales;
+    float* v_scales;
+} rmlk_paged_cache;
+
+/* Puts the keys and values of new tokens into the cache, the keys rotated on the way, and rotates their queries.
+ *   k, v: [tokens, kv_heads, head_dim] (f32 or f16), q: [tokens, q_heads, head_dim] or NULL; heads dense, rows *_stride elements apart.
+ *   rotation, as rmlk_b200_rope has it: r = x cos[p] + (-x[D/2:], x[:D/2]) sin[p] with rows p = the token's position of the tables cos, sin
+ *   [table_rows, head_dim] f32; products and sum exact to one rounding to fp32 (to the type of q for queries, written to q_out).  NULL: keys as
+ *   they are (and no q).
+ * Scale of a block: a power of two, 2^e >= 2^-126, the least with max |value| <= 127 2^e over the new tokens; where the block holds earlier tokens
+ * (slots before the first new one) at least its present scale, and where it grows their codes are divided by the ratio, rounded to nearest even.
+ * Codes are value / 2^e rounded to nearest even.  A block that receives an infinity or a NaN gets the scale NaN - what attends to it is NaN -
+ * until it is begun anew in its first slot.  Positions below 0 (lens[b] less than the new tokens) are passed over.
+ * A token whose page is not in [0, pages), which lies behind table_width pages or table_rows positions is not stored, its query is not
+ * written, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG.  No page may receive tokens of two sequences in one call. */
+RMLK_API int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rmlk_paged_cache* cache, int64_t tokens, int64_t batch,
+                           const int32_t* starts, const int32_t* lens, const int32_t* table, int64_t table_width, const void* k,
+                           int64_t k_stride, const void* v, int64_t v_stride, const float* cos, const float* sin, int64_t table_rows,
+                           int64_t q_heads, const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int* status);
+
+/* Attention of the new tokens over such a cache (their own keys and values in it already): row i of sequence b, at position
+ * p = lens[b] - new[b] + i, sees positions 0 .. p;
+ *   out[row, h] = softmax_t(scale q[row, h] . k[t, h / (q_heads / kv_heads)]) v[t, ..]
+ * q, out: [tokens, q_heads, head_dim] f32 or f16, heads dense, rows q_stride / out_stride elements apart; q_heads a multiple of
+ * kv_heads, up to 64 for each.  A row that sees nothing is 0; one that sees a token whose page is not in [0, pages) or lies behind table_width is
+ * NaN, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG (RMLK_ERR_TIMEOUT: a bounded wait expired).
+ * `workspace`: rmlk_b200_paged_attention_workspace_bytes() bytes on a 16-byte boundary, zero-filled before its first use; its counters are
+ * zero again after each call.  Calls that may overlap on the GPU take one each. */
+RMLK_API int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const rmlk_paged_cache* cache, int64_t tokens, int64_t batch,
+                              int64_t q_heads, const int32_t* starts, const int32_t* lens, const int32_t* table, int64_t table_width,
+                              const void* q, int64_t q_stride, float scale, void* out, int64_t out_stride, void* workspace,
+                              size_t workspace_bytes, int* status);
+/* ragged: 1 where starts will be given, 0 where not */
+RMLK_API size_t rmlk_b200_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                 int ragged);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,6 +30,13 @@ def lib() -> ctypes.CDLL:
         _lib.rmlk_b200_dtype_size.restype = ctypes.c_size_t
         _lib.rmlk_b200_matmul_workspace_bytes.restype = ctypes.c_size_t
         _lib.rmlk_b200_matmul_tp_workspace_bytes.restype = ctypes.c_size_t
+        p, i, n, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+        _lib.rmlk_b200_quantize_rows.argtypes = [p, i, n, n, p, n, p, n, p]
+        _lib.rmlk_b200_matmul_i8.argtypes = [p, i, n, n, n, p, n, p, p, n, p, p, n, p]
+        _lib.rmlk_b200_paged_append.argtypes = [p, i, p, n, n, p, p, p, n, p, n, p, n, p, p, n, n, p, n, p, n, p]
+        _lib.rmlk_b200_paged_attention.argtypes = [p, i, p, n, n, n, p, p, p, n, p, n, f, p, n, p, ctypes.c_size_t, p]
+        _lib.rmlk_b200_paged_attention_workspace_bytes.argtypes = [n, n, n, n, n, i]
+        _lib.rmlk_b200_paged_attention_workspace_bytes.restype = ctypes.c_size_t
     return _lib
 
 

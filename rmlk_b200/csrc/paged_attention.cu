@@ -1,0 +1,108 @@
+// Attention over a paged cache of 8-bit codes (paged.cuh): softmax(scale q k^T) v, k and v = code times the scale of their page and head.
+#include "paged.cuh"
+
+namespace rmlk {
+namespace paged {
+
+struct Attend {
+    const void* q;
+    void* out;
+    int64_t qs, os;  // row strides
+    int q_heads, group;
+    float scale;
+    int* status;
+};
+
+__device__ __forceinline__ float as_f32(float x) { return x; }
+__device__ __forceinline__ float as_f32(__half x) { return __half2float(x); }
+
+// One warp per (new token, query head), one key after the other.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) row_kernel(const Cache c, const Batch q, const Attend a) {
+    dep_sync();
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int64_t row = item / a.q_heads;
+    const int h = static_cast<int>(item - row * a.q_heads), lane = threadIdx.x & 31, kv = h / a.group;
+    if (row >= q.tokens) return;
+    int b;
+    int64_t first = 0, count = 0;
+    if (!q.starts) {
+        b = static_cast<int>(row / q.each);
+        q.rows(b, first, count);
+    } else {
+        for (b = 0; b < q.batch; b++) {
+            q.rows(b, first, count);
+            if (row >= first && row < first + count) break;
+        }
+        if (b == q.batch) return;
+    }
+    constexpr int N = D / 32;
+    float x[N], acc[N];
+    const T* src = static_cast<const T*>(a.q) + row * a.qs + static_cast<int64_t>(h) * D;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        x[i] = as_f32(src[lane + 32 * i]);
+        acc[i] = 0.f;
+    }
+    const int64_t see = q.lens[b] - count + row - first + 1;
+    float top = -INFINITY, sum = 0.f;
+    bool bad = false;
+    for (int64_t t = 0; t < see; t++) {
+        const int64_t at = t >> c.page_log;
+        const int page = at < q.width ? q.table[b * q.width + at] : -1;
+        if (page < 0 || page >= c.pages) {
+            bad = true;
+            break;
+        }
+        const int64_t block = static_cast<int64_t>(page) * c.kv_heads + kv, off = (block * c.page + (t & (c.page - 1))) * D;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) s = fmaf(x[i], static_cast<float>(c.k[off + lane + 32 * i]), s);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        s *= c.ks[block] * a.scale;
+        const float most = s > top || s != s ? s : top, corr = top == -INFINITY ? 0.f : expf(top - most), e = expf(s - most);
+        top = most;
+        sum = sum * corr + e;
+        const float w = e * c.vs[block];
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[i] = fmaf(w, static_cast<float>(c.v[off + lane + 32 * i]), acc[i] * corr);
+    }
+    if (bad && a.status && lane == 0) *a.status = RMLK_ERR_INVALID_ARG;
+    T* o = static_cast<T*>(a.out) + row * a.os + static_cast<int64_t>(h) * D;
+#pragma unroll
+    for (int i = 0; i < N; i++) o[lane + 32 * i] = static_cast<T>(bad ? __int_as_float(0x7fc00000) : see <= 0 ? 0.f : acc[i] / sum);
+}
+
+}  // namespace paged
+}  // namespace rmlk
+
+using namespace rmlk;
+
+extern "C" size_t rmlk_b200_paged_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int) { return 0; }
+
+extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const rmlk_paged_cache* cache, int64_t tokens, int64_t batch, int64_t q_heads, const int32_t* starts,
+                                         const int32_t* lens, const int32_t* table, int64_t table_width, const void* q, int64_t q_stride, float scale, void* out,
+                                         int64_t out_stride, void* workspace, size_t workspace_bytes, int* status) {
+    (void)workspace;
+    (void)workspace_bytes;
+    if (dtype != RMLK_F32 && dtype != RMLK_F16) return fail(RMLK_ERR_UNSUPPORTED_DTYPE, "unsupported data type for paged_attention (f32, f16)");
+    paged::Cache c;
+    paged::Batch s;
+    const int rc = paged::take("paged_attention", cache, tokens, batch, starts, lens, table, table_width, c, s);
+    if (rc != RMLK_OK) return rc;
+    if (q_heads < 1 || q_heads % c.kv_heads || q_heads / c.kv_heads > 64) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: q_heads must be a multiple of kv_heads, up to 64 for each");
+    if (tokens == 0 || batch == 0) return RMLK_OK;
+    if (!q || !out) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: NULL pointer");
+    const int64_t e = static_cast<int64_t>(dtype_size(dtype)), per = 16 / e;
+    if (q_stride < q_heads * c.d || out_stride < q_heads * c.d) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: rows overlap");
+    if (!aligned_to(q, 16) || !aligned_to(out, 16) || q_stride % per || out_stride % per) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: rows must lie on 16-byte boundaries");
+    paged::Attend a = {q, out, q_stride, out_stride, static_cast<int>(q_heads), static_cast<int>(q_heads / c.kv_heads), scale, status};
+    const int64_t ctas = ceil_div64(tokens * q_heads, 4);
+    if (ctas > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");
+    const dim3 grid(static_cast<unsigned>(ctas));
+    if (dtype == RMLK_F32) launch_dep(c.d == 64 ? paged::row_kernel<float, 64> : paged::row_kernel<float, 128>, grid, dim3(128), 0, as_stream(stream), c, s, a);
+    else launch_dep(c.d == 64 ? paged::row_kernel<__half, 64> : paged::row_kernel<__half, 128>, grid, dim3(128), 0, as_stream(stream), c, s, a);
+    RMLK_CHECK_LAUNCH("paged_attention row_kernel");
+    return RMLK_OK;
+}

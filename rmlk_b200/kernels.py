@@ -8,7 +8,7 @@ these helpers with `torch.empty` — the library itself never allocates.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -527,4 +527,196 @@ def scale_mask_softmax(scores: torch.Tensor, scale: float, mask: torch.Tensor) -
     m4 = mask.reshape([1] * (4 - mask.dim()) + list(mask.shape)).expand(scores.shape)
     _check(lib().rmlk_b200_scale_mask_softmax(_stream(), dt.from_torch(scores.dtype), _i64(list(scores.shape[:3])), ctypes.c_int64(scores.shape[3]),
                                               _i64(list(m4.stride()[:3])), ctypes.c_float(scale), _ptr(scores), _ptr(mask), _ptr(out)))
+    return out
+
+
+# ---- serving in 8 bits ------------------------------------------------------------------------------------------
+def _rows_of(t: torch.Tensor, dtypes, what: str) -> int:
+    """Elements between the rows of a CUDA tensor [rows, ...] whose rows are dense."""
+    if not t.is_cuda or t.dtype not in dtypes or (t.numel() and (t.stride(-1) != 1 or (t.dim() == 3 and t.stride(1) != t.shape[2]))):
+        raise ValueError(f"{what}: a CUDA tensor of {' or '.join(str(d)[6:] for d in dtypes)} with dense rows is wanted")
+    if t.shape[0] > 1:
+        return t.stride(0)
+    return (t.shape[1] * (t.shape[2] if t.dim() == 3 else 1) + 15) // 16 * 16  # nothing follows a single row: any distance does
+
+
+def _one_device(first: torch.Tensor, *ts) -> None:
+    if not first.is_cuda:
+        raise ValueError("rmlk_b200 kernels take CUDA tensors")
+    if first.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors of {first.device} while cuda:{torch._C._cuda_getDevice()} is current")
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors of {first.device} and of {t.device} in one call")
+
+
+_FLOATS = (torch.float32, torch.float16)
+_I8 = (torch.int8,)
+
+
+def _dense(t: Optional[torch.Tensor], dtype: torch.dtype, shape, what: str) -> int:
+    """Address of a dense CUDA tensor of this type and shape; 0 for None."""
+    if t is None:
+        return 0
+    if not t.is_cuda or t.dtype != dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise ValueError(f"{what}: a contiguous CUDA tensor {list(shape) if shape is not None else ''} of {str(dtype)[6:]} is wanted")
+    return t.data_ptr()
+
+
+def _raw_stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def quantize_rows(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
+    """x [m, k] (f32 or f16; rows may lie apart) -> (int8 codes [m, k], fp32 scales [m]) with x ~ codes * scales[:, None]; a scale is the row's
+    largest magnitude over 127, a code the nearest integer to the real quotient.  Rows of the codes start on 16-byte boundaries, as matmul_i8
+    wants them.  A row with an infinity or a NaN gets the scale NaN."""
+    if x.dim() != 2:
+        raise ValueError("quantize_rows: x must be [rows, cols]")
+    m, k = x.shape
+    ldx = _rows_of(x, _FLOATS, "quantize_rows: x")
+    if codes is None:
+        ld = (k + 15) // 16 * 16
+        codes = torch.empty((m, ld), dtype=torch.int8, device=x.device)
+        if ld != k:
+            codes = codes[:, :k]
+    elif codes.shape != x.shape:
+        raise ValueError("quantize_rows: codes must have the shape of x")
+    if scales is None:
+        scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    _one_device(x, codes, scales)
+    _check(lib().rmlk_b200_quantize_rows(_raw_stream(), dt.from_torch(x.dtype), m, k, x.data_ptr(), ldx, codes.data_ptr(),
+                                         _rows_of(codes, _I8, "quantize_rows: codes"), _dense(scales, torch.float32, (m,), "quantize_rows: scales")))
+    return codes, scales
+
+
+def quantize_weight(w: torch.Tensor):
+    """w [k, n] as `matmul` takes it (f32 or f16) -> (int8 codes [n, k], fp32 scales [n]) as `matmul_i8` takes them, done once per weight."""
+    _require_cuda(w)
+    return quantize_rows(transpose(w, [1, 0]))
+
+
+def matmul_i8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, dtype: torch.dtype = torch.float32,
+              out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """(x @ w.T) * x_scales[:, None] * w_scales for int8 codes x [m, k], w [n, k] (rows on 16-byte boundaries; k <= 131071): [m, n] of
+    `dtype` (f32 or f16).  The sums are exact 32-bit integers."""
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError("matmul_i8: x must be [m, k] and w [n, k]")
+    (m, k), n = x.shape, w.shape[0]
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=x.device)
+    elif out.shape != (m, n) or out.dtype != dtype:
+        raise ValueError("matmul_i8: out must be [m, n] of dtype")
+    _one_device(x, x_scales, w, w_scales, out, status)
+    _check(lib().rmlk_b200_matmul_i8(_raw_stream(), dt.from_torch(dtype), m, n, k, x.data_ptr(), _rows_of(x, _I8, "matmul_i8: x"),
+                                     _dense(x_scales, torch.float32, (m,), "matmul_i8: x_scales"), w.data_ptr(), _rows_of(w, _I8, "matmul_i8: w"),
+                                     _dense(w_scales, torch.float32, (n,), "matmul_i8: w_scales"), out.data_ptr(),
+                                     _rows_of(out, _FLOATS, "matmul_i8: out"), _dense(status, torch.int32, None, "matmul_i8: status")))
+    return out
+
+
+class PagedCache(NamedTuple):
+    """Keys and values in pages: int8 codes k, v [pages, kv_heads, page_size, head_dim] (page_size 16 / 32 / 64 / 128, head_dim 64 / 128) and an fp32
+    scale for each page and head, k_scales, v_scales [pages, kv_heads].  Token t of sequence b lies in page table[b, t // page_size]."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def paged_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> PagedCache:
+    """An empty cache.  (Nothing needs clearing when a page is given to another sequence: its first slot begins it anew.)"""
+    shape = (pages, kv_heads, page_size, head_dim)
+    k, v = (torch.zeros(shape, dtype=torch.int8, device=device) for _ in range(2))
+    return PagedCache(k, v, *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
+
+
+class _PagedCacheC(ctypes.Structure):
+    """rmlk_paged_cache of include/rmlk_b200.h."""
+    _fields_ = [("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("page_size", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p)]
+
+
+def _paged(what: str, cache: PagedCache, lens: torch.Tensor, table: torch.Tensor, starts: Optional[torch.Tensor]):
+    """The cache for the C call, addresses of the batch's index tensors, and its size."""
+    shape = cache.k.shape
+    if len(shape) != 4 or table.dim() != 2:
+        raise ValueError(f"{what}: cache.k must be [pages, kv_heads, page_size, head_dim], table [batch, width]")
+    batch = table.shape[0]
+    c = _PagedCacheC(*shape, _dense(cache.k, torch.int8, None, what + ": cache.k"), _dense(cache.v, torch.int8, shape, what + ": cache.v"),
+                     _dense(cache.k_scales, torch.float32, shape[:2], what + ": cache.k_scales"),
+                     _dense(cache.v_scales, torch.float32, shape[:2], what + ": cache.v_scales"))
+    _one_device(cache.k, cache.v, cache.k_scales, cache.v_scales, lens, table, starts)
+    return (c, _dense(lens, torch.int32, (batch,), what + ": lens"), _dense(table, torch.int32, None, what + ": table"),
+            _dense(starts, torch.int32, (batch + 1,), what + ": starts"), batch)
+
+
+def _paged_rows(what: str, t: torch.Tensor, tokens: int, heads: Optional[int], cache: PagedCache, dtype) -> int:
+    if t.dim() != 3 or t.shape[0] != tokens or (heads is not None and t.shape[1] != heads) or t.shape[2] != cache.k.shape[3] or t.dtype != dtype:
+        raise ValueError(f"{what}: [{tokens}, {'heads' if heads is None else heads}, {cache.k.shape[3]}] of {str(dtype)[6:]} is wanted, got {list(t.shape)} of {str(t.dtype)[6:]}")
+    return _rows_of(t, _FLOATS, what)
+
+
+def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, cos: Optional[torch.Tensor] = None,
+                 sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None,
+                 q_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Puts the keys and values k, v [tokens, kv_heads, head_dim] (f32 or f16; rows may lie apart, as columns of a merged product) of the LAST
+    tokens of each sequence into the cache: lens [batch] int32 counts them, table [batch, width] int32 names the pages; sequence b has rows
+    starts[b]:starts[b+1] (int32 [batch + 1]), or tokens / batch rows where starts is None.  With tables cos, sin [positions, head_dim] fp32 the
+    keys are rotated as `rope` does, and the queries q [tokens, q_heads, head_dim] too: they are returned (rows that no sequence has are left
+    unwritten).  Scales of blocks are powers of two; a block that fills over several calls keeps or raises its scale.  status [1] int32 becomes 1
+    where a token has no page or no row in the tables; it is not stored.  No page may receive tokens of two sequences in one call."""
+    c, p_lens, p_table, p_starts, batch = _paged("paged_append", cache, lens, table, starts)
+    tokens = k.shape[0]
+    ldk = _paged_rows("paged_append: k", k, tokens, cache.k.shape[1], cache, k.dtype)
+    ldv = _paged_rows("paged_append: v", v, tokens, cache.k.shape[1], cache, k.dtype)
+    rows = ldq = ldo = p_q = p_out = heads = 0
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape[1] != cache.k.shape[3]:
+            raise ValueError("paged_append: cos and sin must be [positions, head_dim]")
+        rows = cos.shape[0]
+    if q is not None:
+        ldq = _paged_rows("paged_append: q", q, tokens, None, cache, k.dtype)
+        heads, p_q = q.shape[1], q.data_ptr()
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ldo = _paged_rows("paged_append: q_out", q_out, tokens, heads, cache, k.dtype)
+        p_out = q_out.data_ptr()
+    _one_device(cache.k, k, v, cos, sin, q, q_out, status)
+    _check(lib().rmlk_b200_paged_append(_raw_stream(), dt.from_torch(k.dtype), ctypes.addressof(c), tokens, batch, p_starts, p_lens, p_table, table.shape[1],
+                                        k.data_ptr(), ldk, v.data_ptr(), ldv, _dense(cos, torch.float32, None, "paged_append: cos"),
+                                        _dense(sin, torch.float32, None if cos is None else cos.shape, "paged_append: sin"), rows, heads, p_q, ldq, p_out, ldo,
+                                        _dense(status, torch.int32, None, "paged_append: status")))
+    return q_out if q is not None else None
+
+
+def paged_attention_workspace(q: torch.Tensor, cache: PagedCache, batch: int, ragged: bool = False) -> torch.Tensor:
+    """A zero-filled workspace for paged_attention on queries of this shape.  It can be used again and again, also for calls that need less, but
+    not by two calls that may overlap on the GPU."""
+    need = lib().rmlk_b200_paged_attention_workspace_bytes(q.shape[0], batch, q.shape[1], cache.k.shape[1], cache.k.shape[3], int(ragged))
+    return torch.zeros(max(need, 16), dtype=torch.uint8, device=q.device)
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, lens: torch.Tensor, table: torch.Tensor, scale: float, starts: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v for the queries q [tokens, q_heads, head_dim] (f32 or f16; rows may lie apart) of the last tokens of each sequence, each
+    of which sees the sequence up to itself: one token per sequence, a few, or whole prompts (lens, table, starts as for paged_append, by which
+    their keys and values are in the cache already) -> [tokens, q_heads, head_dim].  A row that sees nothing is 0; one that sees a token without a
+    valid page is NaN and status [1] int32 becomes 1.  workspace: see paged_attention_workspace; without one the call makes its own."""
+    c, p_lens, p_table, p_starts, batch = _paged("paged_attention", cache, lens, table, starts)
+    if q.dim() != 3:
+        raise ValueError("paged_attention: q must be [tokens, q_heads, head_dim]")
+    tokens, heads = q.shape[0], q.shape[1]
+    ldq = _paged_rows("paged_attention: q", q, tokens, None, cache, q.dtype)
+    if out is None:
+        out = torch.empty((tokens, heads, q.shape[2]), dtype=q.dtype, device=q.device)
+    ldo = _paged_rows("paged_attention: out", out, tokens, heads, cache, q.dtype)
+    if workspace is None:
+        workspace = paged_attention_workspace(q, cache, batch, starts is not None)
+    _one_device(cache.k, q, out, workspace, status)
+    if not workspace.is_contiguous():
+        raise ValueError("paged_attention: the workspace must be contiguous")
+    _check(lib().rmlk_b200_paged_attention(_raw_stream(), dt.from_torch(q.dtype), ctypes.addressof(c), tokens, batch, heads, p_starts, p_lens, p_table, table.shape[1],
+                                           q.data_ptr(), ldq, scale, out.data_ptr(), ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                                           _dense(status, torch.int32, None, "paged_attention: status")))
     return out
