@@ -23,10 +23,12 @@ int take(const char* what, const rmlk_paged_cache* cache, int64_t tokens, int64_
     if (d != 64 && d != 128) return bad("head_dim must be 64 or 128");
     if (cache->pages < 0 || cache->pages >= (1ll << 31) || cache->kv_heads < 1 || cache->kv_heads > 65535) return bad("bad cache extent");
     if (tokens < 0 || tokens >= (1ll << 31) || batch < 0 || batch >= (1ll << 24) || table_width < 0 || table_width >= (1ll << 31) / page) return bad("bad extent");
+    if (static_cast<double>(batch) * static_cast<double>(table_width + 1) * static_cast<double>(cache->kv_heads) > 1e13) return bad("bad extent");  // (unit counts times CTAs stay in 63 bits)
     if (tokens > 0 && batch > 0 && !starts && tokens % batch) return bad("without starts, tokens must be a multiple of batch");
     if (tokens > 0 && batch > 0) {
         if (!lens || (!table && table_width > 0)) return bad("NULL pointer");
-        if (cache->pages > 0 && (!cache->k || !cache->v || !cache->k_scales || !cache->v_scales)) return bad("NULL pointer in the cache");
+        if (cache->pages < 1) return bad("a cache without pages");
+        if (!cache->k || !cache->v || !cache->k_scales || !cache->v_scales) return bad("NULL pointer in the cache");
         if (!aligned_to(cache->k, 16) || !aligned_to(cache->v, 16) || !aligned_to(cache->k_scales, 4) || !aligned_to(cache->v_scales, 4) || !aligned_to(lens, 4) ||
             !aligned_to(table, 4) || !aligned_to(starts, 4))
             return bad("misaligned pointer");

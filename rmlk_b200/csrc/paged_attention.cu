@@ -1,17 +1,10 @@
 // Attention over a paged cache of 8-bit codes (paged.cuh): softmax(scale q k^T) v, k and v = code times the scale of their page and head.
-#include "paged.cuh"
+#include <mutex>
+
+#include "paged_few.cuh"
 
 namespace rmlk {
 namespace paged {
-
-struct Attend {
-    const void* q;
-    void* out;
-    int64_t qs, os;  // row strides
-    int q_heads, group;
-    float scale;
-    int* status;
-};
 
 __device__ __forceinline__ float as_f32(float x) { return x; }
 __device__ __forceinline__ float as_f32(__half x) { return __half2float(x); }
@@ -74,18 +67,40 @@ __global__ void __launch_bounds__(128) row_kernel(const Cache c, const Batch q, 
     for (int i = 0; i < N; i++) o[lane + 32 * i] = static_cast<T>(bad ? __int_as_float(0x7fc00000) : see <= 0 ? 0.f : acc[i] / sum);
 }
 
+template <typename T, int D>
+static int launch_few(cudaStream_t st, const Cache& c, const Batch& s, const Attend& a, void* workspace) {
+    using L = Few<T, D>;
+    auto kernel = few_kernel<T, D>;
+    static std::once_flag configured[64];  // the dynamic shared memory limit is raised once per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaError_t cfg_err = cudaSuccess;
+    if (dev >= 0 && dev < 64) std::call_once(configured[dev], [&] { cfg_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM); });
+    RMLK_CUDA(cfg_err);
+    const int rows = s.each * a.group, tiles = (rows + L::ROWS - 1) / L::ROWS;
+    RMLK_CUDA(launch_dep(kernel, dim3(static_cast<unsigned>(sm_count() * L::PER_SM)), dim3(128), L::SMEM, st, c, s, a, tiles, static_cast<unsigned*>(workspace),
+                         reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + COUNTERS * 4)));
+    RMLK_CHECK_LAUNCH("paged_attention few_kernel");
+    return RMLK_OK;
+}
+
 }  // namespace paged
 }  // namespace rmlk
 
 using namespace rmlk;
 
-extern "C" size_t rmlk_b200_paged_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int) { return 0; }
+// Rows of a KV head (new tokens x query heads that share it) up to which few_kernel takes a call.
+constexpr int64_t FEW_ROWS = 64;
+static bool takes_few(int64_t tokens, int64_t batch, int64_t group, bool ragged) { return !ragged && batch > 0 && tokens / batch * group <= FEW_ROWS; }
+
+extern "C" size_t rmlk_b200_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int ragged) {
+    if (kv_heads < 1 || q_heads < kv_heads || !takes_few(tokens, batch, q_heads / kv_heads, ragged != 0)) return 0;
+    return paged::few_workspace(head_dim);
+}
 
 extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const rmlk_paged_cache* cache, int64_t tokens, int64_t batch, int64_t q_heads, const int32_t* starts,
                                          const int32_t* lens, const int32_t* table, int64_t table_width, const void* q, int64_t q_stride, float scale, void* out,
                                          int64_t out_stride, void* workspace, size_t workspace_bytes, int* status) {
-    (void)workspace;
-    (void)workspace_bytes;
     if (dtype != RMLK_F32 && dtype != RMLK_F16) return fail(RMLK_ERR_UNSUPPORTED_DTYPE, "unsupported data type for paged_attention (f32, f16)");
     paged::Cache c;
     paged::Batch s;
@@ -98,6 +113,13 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
     if (q_stride < q_heads * c.d || out_stride < q_heads * c.d) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: rows overlap");
     if (!aligned_to(q, 16) || !aligned_to(out, 16) || q_stride % per || out_stride % per) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: rows must lie on 16-byte boundaries");
     paged::Attend a = {q, out, q_stride, out_stride, static_cast<int>(q_heads), static_cast<int>(q_heads / c.kv_heads), scale, status};
+    if (takes_few(tokens, batch, a.group, starts != nullptr)) {
+        if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
+            return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
+        const cudaStream_t st = as_stream(stream);
+        if (dtype == RMLK_F32) return c.d == 64 ? paged::launch_few<float, 64>(st, c, s, a, workspace) : paged::launch_few<float, 128>(st, c, s, a, workspace);
+        return c.d == 64 ? paged::launch_few<__half, 64>(st, c, s, a, workspace) : paged::launch_few<__half, 128>(st, c, s, a, workspace);
+    }
     const int64_t ctas = ceil_div64(tokens * q_heads, 4);
     if (ctas > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");
     const dim3 grid(static_cast<unsigned>(ctas));

@@ -92,7 +92,8 @@ def attention(q, cache, lens, table, scale, starts=None):
 
     Scores are sums of D / 16 steps in fp32 that may truncate (2^-23 each), of pairs that hold 22 bits of q against its largest, scaled by two factors and rounded
     in the exponent's argument: (D / 16 + 8) 2^-23 of S = |scale| sum |q| |k|.  A weight is off by that share, twice (its sum too), and by 2^-21 for the
-    exponential and its pair; the sums over T keys by 2^-23 for each of T / 16 + 16 steps, twice.  All of it times the largest |v|."""
+    exponential and its pair; the sums over T keys by 2^-23 for each of T / 16 + 16 steps, twice.  All of it times the largest |v|.
+    f16 queries: the weights are rounded to f16, each by at most 2^-11 of itself, and so the sum of w v by at most 2^-11 sum w |v| <= 2^-11 max |v|."""
     page, d, group = cache.k.shape[2], cache.k.shape[3], q.shape[1] // cache.k.shape[1]
     dev = q.device
     out = torch.full(q.shape, math.nan, dtype=torch.float64, device=dev)
@@ -117,20 +118,20 @@ def attention(q, cache, lens, table, scale, starts=None):
         s = s.masked_fill(hidden, -math.inf)
         w = torch.softmax(s, -1)
         w = torch.where(hidden.all(-1)[None, :, None], torch.zeros((), dtype=w.dtype, device=dev), w)
-        seen = w > 0
         v_ok = torch.nan_to_num(v, nan=0.0)
         o = torch.einsum("hnt,htd->nhd", w, v_ok)
         poison = torch.einsum("hnt,htd->nhd", (~hidden).double().expand(w.shape), torch.isnan(v).double()) > 0
         out[starts[b]: starts[b + 1]] = torch.where(poison, torch.full_like(o, math.nan), o)
         most = torch.nan_to_num(size.masked_fill(hidden, 0).amax(-1))  # [heads, n]
         share = 2 * (d / 16 + 8) * 2.0 ** -23 * most + 2 * 2.0 ** -21 + 2 * (total / 16 + 16) * 2.0 ** -23
+        if q.dtype == torch.float16:
+            share = share + 2.0 ** -11
         bound[starts[b]: starts[b + 1]] = (share * v_ok.abs().amax((1, 2))[:, None]).t()[..., None]
-        del seen
     return out, bound
 
 
 def close(got, want, bound):
-    """got against want; f16 results: the weights are f16 too (half a step, 2^-11 of a share of the largest value), and so is the result."""
+    """got against want, within the bound and, for f16 results, their rounding: half a step, 2^-11 of the value, 2^-25 among the subnormal ones."""
     known = ~torch.isnan(want)
     assert torch.equal(torch.isnan(got) & known, torch.zeros_like(known)), "NaN in a row that has a value"
     limit = bound.expand_as(want).clone()
