@@ -21,7 +21,8 @@ int take(const char* what, const rmlk_paged_cache* cache, int64_t tokens, int64_
     const int64_t page = cache->page_size, d = cache->head_dim;
     if (page != 16 && page != 32 && page != 64 && page != 128) return bad("page_size must be 16, 32, 64 or 128");
     if (d != 64 && d != 128) return bad("head_dim must be 64 or 128");
-    if (cache->pages < 0 || cache->pages >= (1ll << 31) || cache->kv_heads < 1 || cache->kv_heads > 65535) return bad("bad cache extent");
+    if (cache->pages < 0 || cache->pages >= (1ll << 31) || cache->kv_heads < 1 || cache->kv_heads > 65535 || cache->pages * cache->kv_heads >= (1ll << 31))
+        return bad("bad cache extent");
     if (tokens < 0 || tokens >= (1ll << 31) || batch < 0 || batch >= (1ll << 24) || table_width < 0 || table_width >= (1ll << 31) / page) return bad("bad extent");
     if (static_cast<double>(batch) * static_cast<double>(table_width + 1) * static_cast<double>(cache->kv_heads) > 1e13) return bad("bad extent");  // (unit counts times CTAs stay in 63 bits)
     if (tokens > 0 && batch > 0 && !starts && tokens % batch) return bad("without starts, tokens must be a multiple of batch");

@@ -14,8 +14,8 @@
 // bytes become f16 in registers: 0x6400 | (b ^ 0x80) is 1152 + b.
 //   scores  S[16 rows x 8 keys]  = Q K^T: fp32 queries as pairs of f16, the high parts in rows 0-7, the low parts (2^11 times their size) in rows 8-15; f16 queries: 16 rows
 //   values  O[16 rows x 8 dims] += P V over 16 keys: the accumulator fragment of S is the operand fragment of P as it is.
-// Codes are exact in f16.  Each 16 keys' O is formed from zero and added to fp32 sums times their page's scale of V: that keeps any ratio of scales, and
-// keeps the MMA's truncating accumulator short.  Weights are 2^14 exp2(s - max): as pairs for fp32, as f16 for f16 results (2^-11 of a weight, as much as the result's own rounding).
+// Codes are exact in f16.  For fp32 results a step's O is formed from zero and added to fp32 sums, which keeps the MMA's truncating accumulator short; for f16 the
+// accumulators stay in the MMAs.  Weights are 2^14 exp2(s - max): as pairs for fp32, as f16 for f16 results (2^-11 of a weight, as much as the result's own rounding).
 #pragma once
 
 #include "paged.cuh"
@@ -67,7 +67,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 // two bytes (of four that have 0x80 flipped) as f16: 1024 + u - 1152
 __device__ __forceinline__ uint32_t two_f16(uint32_t flipped, uint32_t selector) {
@@ -91,10 +91,15 @@ __device__ __forceinline__ float quad_sum(float x) {
 // a share of a softmax under another maximum: a share without keys has the maximum -inf and sums of zero (or NaN, which has to stay)
 __device__ __forceinline__ float share_weight(float m, float most) { return m == -INFINITY ? 1.f : ex2(m - most); }
 
+// a / b for 0 <= a, 0 < b: nearly always in 32 bits, where a division is a fifth of the instructions
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache c, const Batch q, const Attend a, const int tiles, unsigned* counters, float* partials) {
     using L = Few<T, D>;
-    constexpr int ROWS = L::ROWS, NR = L::NR, KS = L::KS, NC = L::NC, PIECES = D / 64;
+    constexpr int ROWS = L::ROWS, NR = L::NR, KS = L::KS, NC = L::NC, PIECES = D / 64, ACC = 2 * NR, SLOT = SLOT_ROWS * (D + 2);
     dep_sync();
     extern __shared__ __align__(16) uint8_t smem[];
     float2* s_scales = reinterpret_cast<float2*>(smem + L::BODY);                  // [warp][stage][NC] scales of K and V
@@ -109,11 +114,16 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
     const int64_t items = static_cast<int64_t>(c.kv_heads) * tiles;  // problems of a sequence
 
     // ---- this CTA's share of the line ----
-    int64_t total, lo, hi, seq_first;  // seq_first: where sequence b begins on the line
+    int64_t total, per, lo, hi, seq_first;  // seq_first: where sequence b begins on the line
     int b;
-    unsigned workers;
+    unsigned workers, longer;  // the first `longer` workers have per + 1 units, the others per
+    auto begin_of = [&](unsigned w) { return per * w + min(w, longer); };
+    auto worker_of = [&](int64_t unit) {
+        const int64_t head = (per + 1) * longer;
+        return static_cast<unsigned>(unit < head ? divide(unit, per + 1) : longer + divide(unit - head, per));
+    };
     {
-        const int per = (q.batch + 127) / 128, b0 = min(tid * per, q.batch), b1 = min(b0 + per, q.batch);
+        const int each = (q.batch + 127) / 128, b0 = min(tid * each, q.batch), b1 = min(b0 + each, q.batch);
         int64_t own = 0;
         for (int i = b0; i < b1; i++) own += units_of(i);
         own *= items;
@@ -129,8 +139,10 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
         for (int w = 0; w < warp; w++) upto += s_at[w];
         workers = static_cast<unsigned>(min(static_cast<int64_t>(gridDim.x), total));
         if (blockIdx.x >= workers) return;
-        lo = total * blockIdx.x / workers;
-        hi = total * (blockIdx.x + 1) / workers;
+        per = divide(total, workers);
+        longer = static_cast<unsigned>(total - per * workers);
+        lo = begin_of(blockIdx.x);
+        hi = begin_of(blockIdx.x + 1);
         __syncthreads();
         int64_t first = upto - own;
         if (first <= lo && lo < upto) {
@@ -148,8 +160,6 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
         b = static_cast<int>(s_at[0]);
         seq_first = s_at[1];
     }
-    auto worker_of = [&](int64_t unit) { return static_cast<unsigned>(((unit + 1) * workers - 1) / total); };
-
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (L::STAGES * L::STEP);
     const uint8_t* ring_ptr = smem + warp * (L::STAGES * L::STEP);
     float2* scales = s_scales + warp * (L::STAGES * NC);
@@ -157,121 +167,127 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
 
     for (int64_t unit = lo; unit < hi;) {
         const int64_t keys = keys_of(b), units = units_of(b);
-        const int64_t item = (unit - seq_first) / units, unit0 = (unit - seq_first) - item * units;
+        const int64_t item = divide(unit - seq_first, units), unit0 = (unit - seq_first) - item * units;
         const int64_t taken = min(units - unit0, hi - unit);
-        const int h = static_cast<int>(item / tiles), tile = static_cast<int>(item - static_cast<int64_t>(h) * tiles);
+        const int h = static_cast<int>(item) / tiles, tile = static_cast<int>(item - static_cast<int64_t>(h) * tiles);
         const int64_t key0 = unit0 * L::UNIT, key1 = min(keys, (unit0 + taken) * L::UNIT);
         const int64_t before = static_cast<int64_t>(q.lens[b]) - q.each;  // keys before the first new token
 
-        // ---- queries: fragments of the scores' MMAs, and what each lane's rows see ----
+        // ---- the warp's steps: keys key0 + (4 i + warp) KS ----
+        const int64_t first_key = key0 + warp * KS;
+        const int left = static_cast<int>(min(max(key1 - first_key, int64_t(0)), int64_t(0x7fffff00)));  // (keys behind the table are cut off, 2^31 of them are none of a cache's)
+        const int steps = (left + L::UNIT - 1) / L::UNIT;
+        int block = -1;  // page and head as one index; -1: no key there, -2: a key without a page
+        // blocks of PAGED_STEPS steps at a time, one per lane
+        constexpr int PAGED_STEPS = 32 / NC;
+        auto fetch_blocks = [&](int step) {
+            const int off = (step + lane / NC) * L::UNIT + (lane % NC) * 16;
+            block = -1;
+            if (off < left) {
+                const int64_t at = (first_key + off) >> c.page_log;
+                const int p = at < q.width ? q.table[static_cast<int64_t>(b) * q.width + at] : -1;
+                block = p >= 0 && p < c.pages ? p * c.kv_heads + h : -2;
+                if (block == -2 && a.status) *a.status = RMLK_ERR_INVALID_ARG;
+            }
+        };
+        const int slot_base = static_cast<int>(first_key & 127);  // (a page has 128 keys at most)
+        const int8_t* k_lane = c.k + g * D + c4 * 16;
+        const int8_t* v_lane = c.v + 2 * c4 * D + g * (D / 8);
+        const int block_bytes = c.page * D;
+        int fill = 0, fill_stage = 0;  // next step to be asked for, its place in the ring
+        auto issue = [&]() {
+            if (fill < steps) {
+                const int in_batch = fill % PAGED_STEPS;
+                if (in_batch == 0) fetch_blocks(fill);
+                const uint32_t dst = ring + fill_stage * L::STEP;
+#pragma unroll
+                for (int n = 0; n < NC; n++) {
+                    const int at = __shfl_sync(0xffffffffu, block, in_batch * NC + n), from = at < 0 ? h : at;  // (page 0 is read where there is none)
+                    if (lane < 2) {  // the scales of K and V: 0 where there is no key, NaN where a key has no page
+                        float* to = reinterpret_cast<float*>(scales + fill_stage * NC + n) + lane;
+                        if (at >= 0) copy_async<4>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), (lane ? c.vs : c.ks) + at);
+                        else *to = at == -1 ? 0.f : __int_as_float(0x7fc00000);
+                    }
+                    const int64_t off = static_cast<int64_t>(from) * block_bytes + ((slot_base + fill * L::UNIT + 16 * n) & (c.page - 1)) * D;
+                    const int8_t* ks = k_lane + off;
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int i = 0; i < PIECES; i++) copy_async<16>(dst + ((2 * n + j) * PIECES + i) * 512 + lane * 16, ks + j * 8 * D + i * 64);
+                    const int8_t* vs = v_lane + off;
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        copy_async<D / 8>(dst + 2048 + (4 * n + t) * (4 * D) + lane * (D / 8), vs + ((t & 1) + (t >> 1) * 8) * D);
+                }
+                fill++;
+                if (++fill_stage == L::STAGES) fill_stage = 0;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+
+        // ---- queries: fragments of the scores' MMAs, and what each lane's rows see.  (Asked for first, looked at when the first keys are on their way.) ----
+        auto relative = [&](int64_t key) { return static_cast<int>(max(min(key - first_key, int64_t(0x7fffff00)), int64_t(0))); };
         uint32_t qf[4 * PIECES][4];
+        float4 qx[L::PAIRS ? 4 * PIECES : 1];
         float factor[NR];
-        int64_t sees[NR];
+        int sees[NR];  // keys from the warp's first on that the lane's rows see
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             const int row = tile * ROWS + g + 8 * r, token = row / a.group;
             const bool in = row < rows;
-            sees[r] = in ? min(before + token + 1, keys) : 0;
+            sees[r] = in ? relative(min(before + token + 1, keys)) : 0;
+            factor[r] = a.scale * 1.44269504f;
             const T* src = static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * q.each + token) * a.qs + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D + 16 * c4;
-            if constexpr (L::PAIRS) {
-                float4 x[4 * PIECES];
-                uint32_t most = 0;
 #pragma unroll
-                for (int s = 0; s < 4 * PIECES; s++) {
-                    x[s] = in ? *reinterpret_cast<const float4*>(src + (s >> 2) * 64 + (s & 3) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    most = max(max(most, max(finite_abs_bits(x[s].x), finite_abs_bits(x[s].y))), max(finite_abs_bits(x[s].z), finite_abs_bits(x[s].w)));
-                }
-                most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const int e = scale_exponent(most);
-                const float up = exp2_int(e);
-                factor[r] = a.scale * 1.44269504f * exp2_int(-e);
-#pragma unroll
-                for (int s = 0; s < 4 * PIECES; s++) {
-                    split2(x[s].x * up, x[s].y * up, qf[s][0], qf[s][1]);
-                    split2(x[s].z * up, x[s].w * up, qf[s][2], qf[s][3]);
-                }
-            } else {
-                factor[r] = a.scale * 1.44269504f;
-#pragma unroll
-                for (int s = 0; s < 4 * PIECES; s++) {
-                    const uint2 x = in ? *reinterpret_cast<const uint2*>(src + (s >> 2) * 64 + (s & 3) * 4) : make_uint2(0u, 0u);
+            for (int s = 0; s < 4 * PIECES; s++) {
+                const T* at = src + (s >> 2) * 64 + (s & 3) * 4;
+                if constexpr (L::PAIRS) {
+                    qx[s] = in ? *reinterpret_cast<const float4*>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+                } else {
+                    const uint2 x = in ? *reinterpret_cast<const uint2*>(at) : make_uint2(0u, 0u);
                     qf[s][r] = x.x;
                     qf[s][2 + r] = x.y;
                 }
             }
         }
-        const int64_t all_see = max(min(before + 1 + (tile * ROWS) / a.group, keys), int64_t(0));  // keys that every row of the tile sees
-
-        // ---- the warp's steps: keys key0 + (4 i + warp) KS ----
-        const int64_t first_key = key0 + warp * KS;
-        const int steps = first_key < key1 ? static_cast<int>((key1 - first_key + L::UNIT - 1) / L::UNIT) : 0;
-        int page = 0;
-        float2 page_scales = make_float2(0.f, 0.f);
-        // pages of 32 / NC steps at a time, one per lane
-        auto fetch_pages = [&](int step) {
-            const int i = step + lane / NC;
-            const int64_t key = first_key + static_cast<int64_t>(i) * L::UNIT + (lane % NC) * 16;
-            page = 0;
-            page_scales = make_float2(0.f, 0.f);
-            if (i < steps && key < key1) {
-                const int64_t at = key >> c.page_log;
-                const int p = at < q.width ? q.table[static_cast<int64_t>(b) * q.width + at] : -1;
-                if (p >= 0 && p < c.pages) {
-                    page = p;
-                    const int64_t block = static_cast<int64_t>(p) * c.kv_heads + h;
-                    page_scales = make_float2(c.ks[block], c.vs[block]);
-                } else {  // what sees it becomes NaN; page 0 is read in its place
-                    page_scales = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
-                    if (a.status) *a.status = RMLK_ERR_INVALID_ARG;
-                }
+#pragma unroll
+        for (int s = 0; s < L::STAGES - 1; s++) issue();
+        if constexpr (L::PAIRS) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int s = 0; s < 4 * PIECES; s++)
+                most = max(max(most, max(finite_abs_bits(qx[s].x), finite_abs_bits(qx[s].y))), max(finite_abs_bits(qx[s].z), finite_abs_bits(qx[s].w)));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int e = scale_exponent(most);
+            const float up = exp2_int(e);
+            factor[0] *= exp2_int(-e);
+#pragma unroll
+            for (int s = 0; s < 4 * PIECES; s++) {
+                split2(qx[s].x * up, qx[s].y * up, qf[s][0], qf[s][1]);
+                split2(qx[s].z * up, qx[s].w * up, qf[s][2], qf[s][3]);
             }
-        };
-        auto issue = [&](int step) {
-            if (step < steps) {
-                if (step % (32 / NC) == 0) fetch_pages(step);
-                const int stage = step % L::STAGES, from = (step % (32 / NC)) * NC;
-                const uint32_t dst = ring + stage * L::STEP;
-                const int64_t key = first_key + static_cast<int64_t>(step) * L::UNIT;
-#pragma unroll
-                for (int n = 0; n < NC; n++) {
-                    const int64_t p = __shfl_sync(0xffffffffu, page, from + n);
-                    const int64_t off = ((p * c.kv_heads + h) * c.page + ((key + 16 * n) & (c.page - 1))) * D;
-                    const int8_t* ks = c.k + off + g * D + c4 * 16;
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int i = 0; i < PIECES; i++) copy_async<16>(dst + ((2 * n + j) * PIECES + i) * 512 + lane * 16, ks + j * 8 * D + i * 64);
-                    const int8_t* vs = c.v + off + 2 * c4 * D + g * (D / 8);
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-                        copy_async<D / 8>(dst + 2048 + (4 * n + t) * (4 * D) + lane * (D / 8), vs + ((t & 1) + (t >> 1) * 8) * D);
-                }
-                if (lane >= from && lane < from + NC) scales[stage * NC + lane - from] = page_scales;
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+        }
+        const int all_see = relative(min(before + 1 + (tile * ROWS) / a.group, keys));  // that every row of the tile sees
 
-        float acc[D / 8][2 * NR], top[NR], sum[NR];
+        float acc[D / 8][ACC], top[NR], sum[NR];
 #pragma unroll
         for (int i = 0; i < D / 8; i++)
 #pragma unroll
-            for (int r = 0; r < 2 * NR; r++) acc[i][r] = 0.f;
+            for (int r = 0; r < ACC; r++) acc[i][r] = 0.f;
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             top[r] = -INFINITY;
             sum[r] = 0.f;
         }
-#pragma unroll
-        for (int s = 0; s < L::STAGES - 1; s++) issue(s);
-        for (int step = 0; step < steps; step++) {
+        float v_ref = 0.f, v_inv = INFINITY, v_top = 0.f;  // the scale of V that the weights are relative to, its reciprocal, the largest so far
+        int stage = 0;
+        for (int step = 0; step < steps; step++, stage = stage + 1 == L::STAGES ? 0 : stage + 1) {
             __syncwarp();  // the slot that is filled next has been read, its scales too
-            issue(step + L::STAGES - 1);
+            issue();
             asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 1) : "memory");
             __syncwarp();  // (scales come from other lanes)
-            const int stage = step % L::STAGES;
             const uint8_t* at = ring_ptr + stage * L::STEP;
-            const int64_t key = first_key + static_cast<int64_t>(step) * L::UNIT;
             // ---- scores ----
             float x[NR][KS / 8][2];
             float most[NR];
@@ -305,15 +321,37 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
                     }
                 }
             }
-            float vs[NR][NC];
+            // Scales of V go into the weights, relative to one for all that an accumulator takes in (infinities and NaN as they are).
+            float vs[NR][NC], v_step = 0.f;
 #pragma unroll
-            for (int n = 0; n < NC; n++)
+            for (int n = 0; n < NC; n++) {
+                const float v = scales[stage * NC + n].y;
+                if (v < INFINITY) v_step = fmaxf(v_step, v);
+            }
+            if constexpr (L::PAIRS) {  // the step's largest
+                v_ref = v_step;
+                v_inv = 1.f / v_step;
+            } else if (v_step > v_ref || (v_step < v_ref * 2.44140625e-4f && v_step > v_top * 5.42101086e-20f)) {
+                // the one that the sums are in, as long as the ratio is moderate (2^-12; 2^-64: so far down sums might leave fp32's range)
+                const float f = v_ref / v_step;
 #pragma unroll
-                for (int r = 0; r < NR; r++) vs[r][n] = scales[stage * NC + n].y;
-            if (key + KS > all_see) {
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int r = 0; r < ACC; r++) acc[i][r] *= f;
+                v_ref = v_step;
+                v_inv = 1.f / v_step;
+                v_top = fmaxf(v_top, v_step);
+            }
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const float v = scales[stage * NC + n].y;
+#pragma unroll
+                for (int r = 0; r < NR; r++) vs[r][n] = v == v_ref ? 1.f : v * v_inv;
+            }
+            if (KS + step * L::UNIT > all_see) {
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
-                    const int see = static_cast<int>(max(min(sees[r] - key, static_cast<int64_t>(KS)), int64_t(0)));
+                    const int see = sees[r] - step * L::UNIT;
 #pragma unroll
                     for (int j = 0; j < KS / 8; j++) {
                         if (8 * j + 2 * c4 >= see) x[r][j][0] = -INFINITY;
@@ -356,56 +394,51 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
                 }
             }
             // ---- values ----
+            uint32_t p[NC][4], v[NC][4][D / 32];
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                uint32_t p[4];
                 if constexpr (L::PAIRS) {
-                    split2(x[0][2 * n][0], x[0][2 * n][1], p[0], p[1]);
-                    split2(x[0][2 * n + 1][0], x[0][2 * n + 1][1], p[2], p[3]);
+                    split2(x[0][2 * n][0] * vs[0][n], x[0][2 * n][1] * vs[0][n], p[n][0], p[n][1]);
+                    split2(x[0][2 * n + 1][0] * vs[0][n], x[0][2 * n + 1][1] * vs[0][n], p[n][2], p[n][3]);
                 } else {
 #pragma unroll
                     for (int r = 0; r < NR; r++) {
-                        p[r] = pack_f16(x[r][2 * n][0], x[r][2 * n][1]);
-                        p[2 + r] = pack_f16(x[r][2 * n + 1][0], x[r][2 * n + 1][1]);
+                        p[n][r] = pack_f16(x[r][2 * n][0] * vs[r][n], x[r][2 * n][1] * vs[r][n]);
+                        p[n][2 + r] = pack_f16(x[r][2 * n + 1][0] * vs[r][n], x[r][2 * n + 1][1] * vs[r][n]);
                     }
                 }
-                uint32_t v[4][D / 32];
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
                     const uint8_t* src = at + 2048 + (4 * n + t) * (4 * D) + lane * (D / 8);
                     if constexpr (D == 64) {
                         const uint2 w = *reinterpret_cast<const uint2*>(src);
-                        v[t][0] = w.x ^ 0x80808080u;
-                        v[t][1] = w.y ^ 0x80808080u;
+                        v[n][t][0] = w.x ^ 0x80808080u;
+                        v[n][t][1] = w.y ^ 0x80808080u;
                     } else {
                         const uint4 w = *reinterpret_cast<const uint4*>(src);
-                        v[t][0] = w.x ^ 0x80808080u;
-                        v[t][1] = w.y ^ 0x80808080u;
-                        v[t][2] = w.z ^ 0x80808080u;
-                        v[t][3] = w.w ^ 0x80808080u;
+                        v[n][t][0] = w.x ^ 0x80808080u;
+                        v[n][t][1] = w.y ^ 0x80808080u;
+                        v[n][t][2] = w.z ^ 0x80808080u;
+                        v[n][t][3] = w.w ^ 0x80808080u;
                     }
                 }
+            }
 #pragma unroll
-                for (int w = 0; w < D / 32; w++) {
-                    // tokens 2 c4, 2 c4 + 1 (and 8 further on) side by side, for each of four dims
-                    const uint32_t l01 = __byte_perm(v[0][w], v[1][w], 0x5140), l23 = __byte_perm(v[0][w], v[1][w], 0x7362);
-                    const uint32_t h01 = __byte_perm(v[2][w], v[3][w], 0x5140), h23 = __byte_perm(v[2][w], v[3][w], 0x7362);
+            for (int w = 0; w < D / 32; w++) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float o[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int k = 0; k < 4; k++) {
+                    float fresh[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int n = 0; n < NC; n++) {
+                        // tokens 2 c4, 2 c4 + 1 (and 8 further on) side by side, two dims at a time
+                        const uint32_t near = __byte_perm(v[n][0][w], v[n][1][w], k < 2 ? 0x5140 : 0x7362), far = __byte_perm(v[n][2][w], v[n][3][w], k < 2 ? 0x5140 : 0x7362);
                         const uint32_t sel = k & 1 ? 0x4342 : 0x4140;
-                        mma_16816(o, p[0], p[1], p[2], p[3], two_f16(k < 2 ? l01 : l23, sel), two_f16(k < 2 ? h01 : h23, sel));
-                        float(&d)[2 * NR] = acc[4 * w + k];
-                        if constexpr (L::PAIRS) {
-                            d[0] = fmaf(fmaf(o[2], 1.f / SPLIT_LO, o[0]), vs[0][n], d[0]);
-                            d[1] = fmaf(fmaf(o[3], 1.f / SPLIT_LO, o[1]), vs[0][n], d[1]);
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < NR; r++) {
-                                d[2 * r] = fmaf(o[2 * r], vs[r][n], d[2 * r]);
-                                d[2 * r + 1] = fmaf(o[2 * r + 1], vs[r][n], d[2 * r + 1]);
-                            }
-                        }
+                        if constexpr (L::PAIRS) mma_16816(fresh, p[n][0], p[n][1], p[n][2], p[n][3], two_f16(near, sel), two_f16(far, sel));
+                        else mma_16816(acc[4 * w + k], p[n][0], p[n][1], p[n][2], p[n][3], two_f16(near, sel), two_f16(far, sel));
+                    }
+                    if constexpr (L::PAIRS) {
+                        acc[4 * w + k][0] = fmaf(fmaf(fresh[2], 1.f / SPLIT_LO, fresh[0]), v_step, acc[4 * w + k][0]);
+                        acc[4 * w + k][1] = fmaf(fmaf(fresh[3], 1.f / SPLIT_LO, fresh[1]), v_step, acc[4 * w + k][1]);
                     }
                 }
             }
@@ -419,6 +452,7 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
         for (int r = 0; r < NR; r++) {
             sum[r] = quad_sum(sum[r]);
             const int row = g + 8 * r;
+            const float up = L::PAIRS ? 1.f : v_ref;
             if (c4 == 0) {
                 s_top[warp * ROWS + row] = top[r];
                 s_sum[warp * ROWS + row] = sum[r];
@@ -428,22 +462,22 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
                 float4* dst = reinterpret_cast<float4*>(merge + (warp * ROWS + row) * D + (2 * c4 + e) * (D / 8));
 #pragma unroll
                 for (int i = 0; i < D / 32; i++)
-                    dst[i] = make_float4(acc[4 * i][2 * r + e], acc[4 * i + 1][2 * r + e], acc[4 * i + 2][2 * r + e], acc[4 * i + 3][2 * r + e]);
+                    dst[i] = make_float4(acc[4 * i][2 * r + e] * up, acc[4 * i + 1][2 * r + e] * up, acc[4 * i + 2][2 * r + e] * up, acc[4 * i + 3][2 * r + e] * up);
             }
         }
         __syncthreads();
         const int64_t item_first = seq_first + item * units;
         const bool whole = taken == units;
-        float* slot = partials + (static_cast<int64_t>(blockIdx.x) * 2 + (unit == lo ? 0 : 1)) * (SLOT_ROWS * (D + 2));
+        const int valid = min(ROWS, rows - tile * ROWS);
+        float* slot = partials + (static_cast<int64_t>(blockIdx.x) * 2 + (unit == lo ? 0 : 1)) * SLOT;
         auto put = [&](int row, int col, float4 o, float l) {
             const int at_row = tile * ROWS + row, token = at_row / a.group;
-            if (at_row >= rows) return;
             const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is 0
             T* dst = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * q.each + token) * a.os + (static_cast<int64_t>(h) * a.group + at_row - token * a.group) * D + col;
             if constexpr (L::PAIRS) *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
             else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(o.x * inv, o.y * inv), pack_f16(o.z * inv, o.w * inv));
         };
-        for (int e = tid; e < ROWS * D / 4; e += 128) {
+        for (int e = tid; e < valid * D / 4; e += 128) {
             const int row = e / (D / 4), col = e % (D / 4) * 4;
             float m = s_top[row], l = 0.f;
 #pragma unroll
@@ -474,23 +508,42 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
             __syncthreads();
             if (s_at[2]) {
                 __threadfence();
-                for (int e = tid; e < ROWS * D / 4; e += 128) {
-                    const int row = e / (D / 4), col = e % (D / 4) * 4;
-                    auto part = [&](unsigned w) {  // the first one's may be its second piece of the line
-                        const bool second = w == w0 && total * w / workers != item_first;
-                        return partials + (static_cast<int64_t>(w) * 2 + (second ? 1 : 0)) * (SLOT_ROWS * (D + 2));
-                    };
-                    float m = -INFINITY, l = 0.f;
-                    for (unsigned w = w0; w <= w1; w++) m = fmaxf(m, __ldcg(part(w) + SLOT_ROWS * D + row));
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (unsigned w = w0; w <= w1; w++) {
-                        const float* p = part(w);
-                        const float f = share_weight(__ldcg(p + SLOT_ROWS * D + row), m);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p + row * D + col));
-                        l = fmaf(f, __ldcg(p + SLOT_ROWS * (D + 1) + row), l);
-                        o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
+                // the first one's may be its second piece of the line
+                const float* first = partials + (static_cast<int64_t>(w0) * 2 + (begin_of(w0) != item_first ? 1 : 0)) * SLOT;
+                auto part = [&](unsigned w) { return w == w0 ? first : partials + static_cast<int64_t>(w) * 2 * SLOT; };
+                // The maxima first, a thread to a row and a part; then each part's sums, eight of them on their way at a time.
+                const unsigned parts = w1 - w0 + 1;
+                for (int row = warp; row < valid; row += 4) {
+                    float m = -INFINITY;
+                    for (unsigned w = lane; w < parts; w += 32) m = fmaxf(m, __ldcg(part(w0 + w) + SLOT_ROWS * D + row));
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    float l = 0.f;
+                    for (unsigned w = lane; w < parts; w += 32) {
+                        const float f = share_weight(__ldcg(part(w0 + w) + SLOT_ROWS * D + row), m);
+                        merge[w * ROWS + row] = f;
+                        l = fmaf(f, __ldcg(part(w0 + w) + SLOT_ROWS * (D + 1) + row), l);
                     }
-                    put(row, col, o, l);
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                    if (lane == 0) s_sum[row] = l;
+                }
+                __syncthreads();
+                for (int e = tid; e < valid * D / 4; e += 128) {
+                    const int row = e / (D / 4), col = e % (D / 4) * 4;
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (unsigned w = 0; w < parts; w += 8) {
+                        float4 x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[i] = __ldcg(reinterpret_cast<const float4*>(part(w0 + min(w + i, parts - 1)) + row * D + col));
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (w + i < parts) {
+                                const float f = merge[(w + i) * ROWS + row];
+                                o = make_float4(fmaf(f, x[i].x, o.x), fmaf(f, x[i].y, o.y), fmaf(f, x[i].z, o.z), fmaf(f, x[i].w, o.w));
+                            }
+                    }
+                    put(row, col, o, s_sum[row]);
                 }
             }
         }

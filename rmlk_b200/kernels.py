@@ -531,67 +531,91 @@ def scale_mask_softmax(scores: torch.Tensor, scale: float, mask: torch.Tensor) -
 
 
 # ---- serving in 8 bits ------------------------------------------------------------------------------------------
-def _rows_of(t: torch.Tensor, dtypes, what: str) -> int:
-    """Elements between the rows of a CUDA tensor [rows, ...] whose rows are dense."""
-    if not t.is_cuda or t.dtype not in dtypes or (t.numel() and (t.stride(-1) != 1 or (t.dim() == 3 and t.stride(1) != t.shape[2]))):
-        raise ValueError(f"{what}: a CUDA tensor of {' or '.join(str(d)[6:] for d in dtypes)} with dense rows is wanted")
-    if t.shape[0] > 1:
-        return t.stride(0)
-    return (t.shape[1] * (t.shape[2] if t.dim() == 3 else 1) + 15) // 16 * 16  # nothing follows a single row: any distance does
+# (A step makes these calls once per layer on tensors that take the GPU a few microseconds: their checks are plain conditions, and what was
+# wrong is looked for only when one fails.)
+_I8, _F32, _I32 = torch.int8, torch.float32, torch.int32
+_FLOATS = {torch.float32: dt.F32, torch.float16: dt.F16}
+_stream_of = torch._C._cuda_getCurrentRawStream
 
 
-def _one_device(first: torch.Tensor, *ts) -> None:
-    if not first.is_cuda:
-        raise ValueError("rmlk_b200 kernels take CUDA tensors")
-    if first.device.index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors of {first.device} while cuda:{torch._C._cuda_getDevice()} is current")
-    for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors of {first.device} and of {t.device} in one call")
+def _device_of(what: str, t: torch.Tensor) -> int:
+    """The device of a call's tensors, which has to be the current one."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{what}: CUDA tensors are wanted")
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{what}: tensors on cuda:{dev}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return dev
 
 
-_FLOATS = (torch.float32, torch.float16)
-_I8 = (torch.int8,)
+def _dense(t: torch.Tensor, dtype: torch.dtype, dev: int) -> bool:
+    return t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
 
 
-def _dense(t: Optional[torch.Tensor], dtype: torch.dtype, shape, what: str) -> int:
-    """Address of a dense CUDA tensor of this type and shape; 0 for None."""
-    if t is None:
+def _rows_apart(t: torch.Tensor) -> int:
+    """Elements between the rows of t [rows, ...], whose rows are dense; 0 where they are not."""
+    st = t.stride()
+    shape = t.shape
+    width = shape[1]
+    if len(st) == 3:
+        if st[1] != shape[2] and width > 1:
+            return 0
+        width *= shape[2]
+    if st[-1] != 1 and shape[-1] > 1:
         return 0
-    if not t.is_cuda or t.dtype != dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise ValueError(f"{what}: a contiguous CUDA tensor {list(shape) if shape is not None else ''} of {str(dtype)[6:]} is wanted")
-    return t.data_ptr()
+    # nothing follows a single row: any distance does
+    return st[0] if shape[0] > 1 else (width + 15) // 16 * 16
 
 
-def _raw_stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+def _told(what: str, dev: int, *tensors) -> ValueError:
+    """What is wrong with the tensors of a refused call: (name, tensor, type or types, shape, rows may lie apart) each."""
+    for name, t, dtypes, shape, apart in tensors:
+        if t is None:
+            continue
+        dtypes = dtypes if isinstance(dtypes, (tuple, dict)) else (dtypes,)
+        if not t.is_cuda:
+            return ValueError(f"{what}: {name} is not a CUDA tensor")
+        if t.get_device() != dev:
+            return ValueError(f"{what}: {name} is on {t.device}, the current device is cuda:{dev}")
+        if t.dtype not in dtypes:
+            return ValueError(f"{what}: {name} is {str(t.dtype)[6:]}, not {' or '.join(str(d)[6:] for d in dtypes)}")
+        if t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
+            return ValueError(f"{what}: {name} is {list(t.shape)}, not {['any' if w is None else w for w in shape]}")
+        if not (t.is_contiguous() or (apart and _rows_apart(t))):
+            return ValueError(f"{what}: {name} has strides {t.stride()}: {'its rows must be dense' if apart else 'it must be contiguous'}")
+    return ValueError(f"{what}: tensors do not fit together")
 
 
 def quantize_rows(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
     """x [m, k] (f32 or f16; rows may lie apart) -> (int8 codes [m, k], fp32 scales [m]) with x ~ codes * scales[:, None]; a scale is the row's
     largest magnitude over 127, a code the nearest integer to the real quotient.  Rows of the codes start on 16-byte boundaries, as matmul_i8
     wants them.  A row with an infinity or a NaN gets the scale NaN."""
-    if x.dim() != 2:
-        raise ValueError("quantize_rows: x must be [rows, cols]")
-    m, k = x.shape
-    ldx = _rows_of(x, _FLOATS, "quantize_rows: x")
+    dev = _device_of("quantize_rows", x)
+    shape = x.shape
+    if len(shape) != 2 or x.dtype not in _FLOATS:
+        raise _told("quantize_rows", dev, ("x", x, _FLOATS, (None, None), True))
+    m, k = shape
+    ldx = _rows_apart(x)
     if codes is None:
-        ld = (k + 15) // 16 * 16
-        codes = torch.empty((m, ld), dtype=torch.int8, device=x.device)
-        if ld != k:
+        ldc = (k + 15) // 16 * 16
+        codes = x.new_empty((m, ldc), dtype=_I8)
+        if ldc != k:
             codes = codes[:, :k]
-    elif codes.shape != x.shape:
-        raise ValueError("quantize_rows: codes must have the shape of x")
+    else:
+        ldc = _rows_apart(codes) if codes.dim() == 2 else 0
     if scales is None:
-        scales = torch.empty(m, dtype=torch.float32, device=x.device)
-    _one_device(x, codes, scales)
-    _check(lib().rmlk_b200_quantize_rows(_raw_stream(), dt.from_torch(x.dtype), m, k, x.data_ptr(), ldx, codes.data_ptr(),
-                                         _rows_of(codes, _I8, "quantize_rows: codes"), _dense(scales, torch.float32, (m,), "quantize_rows: scales")))
+        scales = x.new_empty(m, dtype=_F32)
+    if (ldx < k or ldc < k or codes.shape != shape or codes.dtype is not _I8 or codes.get_device() != dev or scales.shape != shape[:1] or not _dense(scales, _F32, dev)):
+        raise _told("quantize_rows", dev, ("x", x, _FLOATS, (m, k), True), ("codes", codes, _I8, (m, k), True), ("scales", scales, _F32, (m,), False))
+    _check(lib().rmlk_b200_quantize_rows(_stream_of(dev), _FLOATS[x.dtype], m, k, x.data_ptr(), ldx, codes.data_ptr(), ldc, scales.data_ptr()))
     return codes, scales
 
 
 def quantize_weight(w: torch.Tensor):
     """w [k, n] as `matmul` takes it (f32 or f16) -> (int8 codes [n, k], fp32 scales [n]) as `matmul_i8` takes them, done once per weight."""
+    dev = _device_of("quantize_weight", w)
+    if w.dim() != 2 or w.dtype not in _FLOATS:
+        raise _told("quantize_weight", dev, ("w", w, _FLOATS, (None, None), False))
     _require_cuda(w)
     return quantize_rows(transpose(w, [1, 0]))
 
@@ -600,18 +624,25 @@ def matmul_i8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales
               out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(x @ w.T) * x_scales[:, None] * w_scales for int8 codes x [m, k], w [n, k] (rows on 16-byte boundaries; k <= 131071): [m, n] of
     `dtype` (f32 or f16).  The sums are exact 32-bit integers."""
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
-        raise ValueError("matmul_i8: x must be [m, k] and w [n, k]")
-    (m, k), n = x.shape, w.shape[0]
+    dev = _device_of("matmul_i8", x)
+    xs, ws = x.shape, w.shape
+    if len(xs) != 2 or len(ws) != 2 or dtype not in _FLOATS:
+        raise _told("matmul_i8", dev, ("x", x, _I8, (None, None), True), ("w", w, _I8, (None, None), True))
+    m, k = xs
+    n = ws[0]
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=x.device)
-    elif out.shape != (m, n) or out.dtype != dtype:
-        raise ValueError("matmul_i8: out must be [m, n] of dtype")
-    _one_device(x, x_scales, w, w_scales, out, status)
-    _check(lib().rmlk_b200_matmul_i8(_raw_stream(), dt.from_torch(dtype), m, n, k, x.data_ptr(), _rows_of(x, _I8, "matmul_i8: x"),
-                                     _dense(x_scales, torch.float32, (m,), "matmul_i8: x_scales"), w.data_ptr(), _rows_of(w, _I8, "matmul_i8: w"),
-                                     _dense(w_scales, torch.float32, (n,), "matmul_i8: w_scales"), out.data_ptr(),
-                                     _rows_of(out, _FLOATS, "matmul_i8: out"), _dense(status, torch.int32, None, "matmul_i8: status")))
+        out = x.new_empty((m, n), dtype=dtype)
+        ldo = n
+    else:
+        ldo = _rows_apart(out) if out.dim() == 2 else -1
+    ldx, ldw = _rows_apart(x), _rows_apart(w)
+    if (ws[1] != k or ldx < k or ldw < k or ldo < n or out.shape != (m, n) or out.dtype is not dtype or out.get_device() != dev or x.dtype is not _I8 or w.dtype is not _I8
+            or w.get_device() != dev or x_scales.shape != (m,) or w_scales.shape != (n,) or not _dense(x_scales, _F32, dev) or not _dense(w_scales, _F32, dev)
+            or (status is not None and not _dense(status, _I32, dev))):
+        raise _told("matmul_i8", dev, ("x", x, _I8, (None, None), True), ("w", w, _I8, (None, k), True), ("out", out, dtype, (m, n), True), ("x_scales", x_scales, _F32, (m,), False),
+                    ("w_scales", w_scales, _F32, (n,), False), ("status", status, _I32, (1,), False))
+    _check(lib().rmlk_b200_matmul_i8(_stream_of(dev), _FLOATS[dtype], m, n, k, x.data_ptr(), ldx, x_scales.data_ptr(), w.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(), ldo,
+                                     None if status is None else status.data_ptr()))
     return out
 
 
@@ -637,24 +668,19 @@ class _PagedCacheC(ctypes.Structure):
                 ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p)]
 
 
-def _paged(what: str, cache: PagedCache, lens: torch.Tensor, table: torch.Tensor, starts: Optional[torch.Tensor]):
-    """The cache for the C call, addresses of the batch's index tensors, and its size."""
-    shape = cache.k.shape
-    if len(shape) != 4 or table.dim() != 2:
-        raise ValueError(f"{what}: cache.k must be [pages, kv_heads, page_size, head_dim], table [batch, width]")
-    batch = table.shape[0]
-    c = _PagedCacheC(*shape, _dense(cache.k, torch.int8, None, what + ": cache.k"), _dense(cache.v, torch.int8, shape, what + ": cache.v"),
-                     _dense(cache.k_scales, torch.float32, shape[:2], what + ": cache.k_scales"),
-                     _dense(cache.v_scales, torch.float32, shape[:2], what + ": cache.v_scales"))
-    _one_device(cache.k, cache.v, cache.k_scales, cache.v_scales, lens, table, starts)
-    return (c, _dense(lens, torch.int32, (batch,), what + ": lens"), _dense(table, torch.int32, None, what + ": table"),
-            _dense(starts, torch.int32, (batch + 1,), what + ": starts"), batch)
-
-
-def _paged_rows(what: str, t: torch.Tensor, tokens: int, heads: Optional[int], cache: PagedCache, dtype) -> int:
-    if t.dim() != 3 or t.shape[0] != tokens or (heads is not None and t.shape[1] != heads) or t.shape[2] != cache.k.shape[3] or t.dtype != dtype:
-        raise ValueError(f"{what}: [{tokens}, {'heads' if heads is None else heads}, {cache.k.shape[3]}] of {str(dtype)[6:]} is wanted, got {list(t.shape)} of {str(t.dtype)[6:]}")
-    return _rows_of(t, _FLOATS, what)
+def _paged(what: str, dev: int, cache: PagedCache, lens: torch.Tensor, table: torch.Tensor, starts: Optional[torch.Tensor], status: Optional[torch.Tensor]):
+    """The cache for the C call; its shape; the batch and the width of its table."""
+    k, v, ks, vs = cache
+    shape, at = k.shape, table.shape
+    if (len(shape) != 4 or len(at) != 2 or not _dense(k, _I8, dev) or not _dense(v, _I8, dev) or not _dense(ks, _F32, dev) or not _dense(vs, _F32, dev) or v.shape != shape
+            or ks.shape != shape[:2] or vs.shape != shape[:2] or not _dense(lens, _I32, dev) or lens.shape != at[:1] or not _dense(table, _I32, dev)
+            or (starts is not None and (not _dense(starts, _I32, dev) or starts.shape != (at[0] + 1,))) or (status is not None and not _dense(status, _I32, dev))):
+        some = tuple(shape[:2]) if len(shape) == 4 else (None, None)
+        batch = at[0] if len(at) == 2 else None
+        raise _told(what, dev, ("cache.k", k, _I8, (None,) * 4, False), ("cache.v", v, _I8, tuple(shape), False), ("cache.k_scales", ks, _F32, some, False),
+                    ("cache.v_scales", vs, _F32, some, False), ("table", table, _I32, (None, None), False), ("lens", lens, _I32, (batch,), False),
+                    ("starts", starts, _I32, (None if batch is None else batch + 1,), False), ("status", status, _I32, (1,), False))
+    return _PagedCacheC(*shape, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()), shape, at
 
 
 def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, cos: Optional[torch.Tensor] = None,
@@ -666,27 +692,32 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lens: torc
     keys are rotated as `rope` does, and the queries q [tokens, q_heads, head_dim] too: they are returned (rows that no sequence has are left
     unwritten).  Scales of blocks are powers of two; a block that fills over several calls keeps or raises its scale.  status [1] int32 becomes 1
     where a token has no page or no row in the tables; it is not stored.  No page may receive tokens of two sequences in one call."""
-    c, p_lens, p_table, p_starts, batch = _paged("paged_append", cache, lens, table, starts)
-    tokens = k.shape[0]
-    ldk = _paged_rows("paged_append: k", k, tokens, cache.k.shape[1], cache, k.dtype)
-    ldv = _paged_rows("paged_append: v", v, tokens, cache.k.shape[1], cache, k.dtype)
-    rows = ldq = ldo = p_q = p_out = heads = 0
-    if cos is not None:
-        if cos.dim() != 2 or cos.shape[1] != cache.k.shape[3]:
-            raise ValueError("paged_append: cos and sin must be [positions, head_dim]")
-        rows = cos.shape[0]
-    if q is not None:
-        ldq = _paged_rows("paged_append: q", q, tokens, None, cache, k.dtype)
-        heads, p_q = q.shape[1], q.data_ptr()
+    dev = _device_of("paged_append", cache.k)
+    c, shape, at = _paged("paged_append", dev, cache, lens, table, starts, status)
+    dtype, want = k.dtype, (k.shape[0] if k.dim() else 0, shape[1], shape[3])
+    tokens = want[0]
+    ldk, ldv = (_rows_apart(t) if t.dim() == 3 else 0 for t in (k, v))
+    heads = ldq = ldo = rows = 0
+    fits = (dtype in _FLOATS and v.dtype is dtype and k.shape == want and v.shape == want and ldk and ldv and k.get_device() == dev and v.get_device() == dev
+            and (cos is None) == (sin is None))
+    if fits and cos is not None:
+        rows = cos.shape[0] if cos.dim() == 2 else -1
+        fits = _dense(cos, _F32, dev) and _dense(sin, _F32, dev) and cos.shape == (rows, shape[3]) == sin.shape
+    if fits and q is not None:
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ldo = _paged_rows("paged_append: q_out", q_out, tokens, heads, cache, k.dtype)
-        p_out = q_out.data_ptr()
-    _one_device(cache.k, k, v, cos, sin, q, q_out, status)
-    _check(lib().rmlk_b200_paged_append(_raw_stream(), dt.from_torch(k.dtype), ctypes.addressof(c), tokens, batch, p_starts, p_lens, p_table, table.shape[1],
-                                        k.data_ptr(), ldk, v.data_ptr(), ldv, _dense(cos, torch.float32, None, "paged_append: cos"),
-                                        _dense(sin, torch.float32, None if cos is None else cos.shape, "paged_append: sin"), rows, heads, p_q, ldq, p_out, ldo,
-                                        _dense(status, torch.int32, None, "paged_append: status")))
+            q_out = q.new_empty(q.shape)
+        heads = q.shape[1] if q.dim() == 3 else 0
+        fits = q.dtype is dtype and q.shape == (tokens, heads, shape[3]) == q_out.shape and q_out.dtype is dtype and q.get_device() == dev and q_out.get_device() == dev
+        if fits:
+            ldq, ldo = _rows_apart(q), _rows_apart(q_out)
+            fits = ldq and ldo
+    if not fits:
+        raise _told("paged_append", dev, ("k", k, _FLOATS, want, True), ("v", v, dtype, want, True), ("cos", cos, _F32, (None, shape[3]), False), ("sin", sin, _F32, (None, shape[3]), False),
+                    ("q", q, dtype, (tokens, None, shape[3]), True), ("q_out", q_out, dtype, (tokens, None, shape[3]), True))
+    _check(lib().rmlk_b200_paged_append(_stream_of(dev), _FLOATS[dtype], ctypes.addressof(c), tokens, at[0], None if starts is None else starts.data_ptr(), lens.data_ptr(),
+                                        table.data_ptr(), at[1], k.data_ptr(), ldk, v.data_ptr(), ldv, None if cos is None else cos.data_ptr(),
+                                        None if sin is None else sin.data_ptr(), rows, heads, None if q is None else q.data_ptr(), ldq, None if q is None else q_out.data_ptr(), ldo,
+                                        None if status is None else status.data_ptr()))
     return q_out if q is not None else None
 
 
@@ -703,20 +734,23 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lens: torch.Tensor, tabl
     of which sees the sequence up to itself: one token per sequence, a few, or whole prompts (lens, table, starts as for paged_append, by which
     their keys and values are in the cache already) -> [tokens, q_heads, head_dim].  A row that sees nothing is 0; one that sees a token without a
     valid page is NaN and status [1] int32 becomes 1.  workspace: see paged_attention_workspace; without one the call makes its own."""
-    c, p_lens, p_table, p_starts, batch = _paged("paged_attention", cache, lens, table, starts)
-    if q.dim() != 3:
-        raise ValueError("paged_attention: q must be [tokens, q_heads, head_dim]")
-    tokens, heads = q.shape[0], q.shape[1]
-    ldq = _paged_rows("paged_attention: q", q, tokens, None, cache, q.dtype)
-    if out is None:
-        out = torch.empty((tokens, heads, q.shape[2]), dtype=q.dtype, device=q.device)
-    ldo = _paged_rows("paged_attention: out", out, tokens, heads, cache, q.dtype)
-    if workspace is None:
-        workspace = paged_attention_workspace(q, cache, batch, starts is not None)
-    _one_device(cache.k, q, out, workspace, status)
-    if not workspace.is_contiguous():
-        raise ValueError("paged_attention: the workspace must be contiguous")
-    _check(lib().rmlk_b200_paged_attention(_raw_stream(), dt.from_torch(q.dtype), ctypes.addressof(c), tokens, batch, heads, p_starts, p_lens, p_table, table.shape[1],
-                                           q.data_ptr(), ldq, scale, out.data_ptr(), ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                           _dense(status, torch.int32, None, "paged_attention: status")))
+    dev = _device_of("paged_attention", cache.k)
+    c, shape, at = _paged("paged_attention", dev, cache, lens, table, starts, status)
+    dtype, qs = q.dtype, q.shape
+    fits = len(qs) == 3 and dtype in _FLOATS and qs[2] == shape[3] and q.get_device() == dev
+    ldq = ldo = 0
+    if fits:
+        if out is None:
+            out = q.new_empty(qs)
+        ldq = _rows_apart(q)
+        ldo = _rows_apart(out) if out.dim() == 3 else 0
+        if workspace is None:
+            workspace = paged_attention_workspace(q, cache, at[0], starts is not None)
+        fits = ldq and ldo and out.shape == qs and out.dtype is dtype and out.get_device() == dev and workspace.is_contiguous() and workspace.get_device() == dev
+    if not fits:
+        raise _told("paged_attention", dev, ("q", q, _FLOATS, (None, None, shape[3]), True), ("out", out, dtype, tuple(qs), True),
+                    *([] if workspace is None else [("workspace", workspace, workspace.dtype, tuple(workspace.shape), False)]))
+    _check(lib().rmlk_b200_paged_attention(_stream_of(dev), _FLOATS[dtype], ctypes.addressof(c), qs[0], at[0], qs[1], None if starts is None else starts.data_ptr(), lens.data_ptr(),
+                                           table.data_ptr(), at[1], q.data_ptr(), ldq, scale, out.data_ptr(), ldo, workspace.data_ptr(), workspace.nbytes,
+                                           None if status is None else status.data_ptr()))
     return out
