@@ -67,10 +67,10 @@ __global__ void __launch_bounds__(128) row_kernel(const Cache c, const Batch q, 
     for (int i = 0; i < N; i++) o[lane + 32 * i] = static_cast<T>(bad ? __int_as_float(0x7fc00000) : see <= 0 ? 0.f : acc[i] / sum);
 }
 
-template <typename T, int D>
+template <typename T, int D, int NR>
 static int launch_few(cudaStream_t st, const Cache& c, const Batch& s, const Attend& a, void* workspace) {
-    using L = Few<T, D>;
-    auto kernel = few_kernel<T, D>;
+    using L = Few<T, D, NR>;
+    auto kernel = few_kernel<T, D, NR>;
     static std::once_flag configured[64];  // the dynamic shared memory limit is raised once per device
     int dev = 0;
     cudaGetDevice(&dev);
@@ -117,8 +117,9 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
         if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
             return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
         const cudaStream_t st = as_stream(stream);
-        if (dtype == RMLK_F32) return c.d == 64 ? paged::launch_few<float, 64>(st, c, s, a, workspace) : paged::launch_few<float, 128>(st, c, s, a, workspace);
-        return c.d == 64 ? paged::launch_few<__half, 64>(st, c, s, a, workspace) : paged::launch_few<__half, 128>(st, c, s, a, workspace);
+        if (dtype == RMLK_F32) return c.d == 64 ? paged::launch_few<float, 64, 1>(st, c, s, a, workspace) : paged::launch_few<float, 128, 1>(st, c, s, a, workspace);
+        if (s.each * a.group <= 8) return c.d == 64 ? paged::launch_few<__half, 64, 1>(st, c, s, a, workspace) : paged::launch_few<__half, 128, 1>(st, c, s, a, workspace);
+        return c.d == 64 ? paged::launch_few<__half, 64, 2>(st, c, s, a, workspace) : paged::launch_few<__half, 128, 2>(st, c, s, a, workspace);
     }
     const int64_t ctas = ceil_div64(tokens * q_heads, 4);
     if (ctas > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");

@@ -9,11 +9,12 @@
 // own, and a partial one (sums, maximum, weights' sum) of a problem that it shares to the workspace; the CTA that finishes last adds them up in their order
 // along the keys, so the result does not depend on which one that is.
 //
-// A warp's step: KS keys (32 of 64 values, 16 of 128).  Each lane copies by cp.async just the bytes that it will read itself, three steps deep; no
-// lane waits for another.  The order of a contraction is free, so a lane's 16 consecutive bytes of a key are its operands of four MMAs (four dims to each), and
-// bytes become f16 in registers: 0x6400 | (b ^ 0x80) is 1152 + b.
-//   scores  S[16 rows x 8 keys]  = Q K^T: fp32 queries as pairs of f16, the high parts in rows 0-7, the low parts (2^11 times their size) in rows 8-15; f16 queries: 16 rows
-//   values  O[16 rows x 8 dims] += P V over 16 keys: the accumulator fragment of S is the operand fragment of P as it is.
+// A warp's step: 32 keys.  Each lane copies by cp.async just the bytes that it will read itself; no lane waits for another.  The order of a contraction is
+// free, so a lane's 16 consecutive bytes of a key are its operands of four MMAs (four dims to each), and bytes become f16 in registers:
+// 0x6400 | (b ^ 0x80) is 1152 + b.
+//   scores  S[16 rows x 8 keys]     = Q K^T: fp32 queries as pairs of f16, the high parts in rows 0-7, the low parts (2^11 times their size) in rows 8-15; f16
+//                                     queries: 8 or 16 rows
+//   values  O^T[16 dims x 8 rows] += V^T P^T over 16 keys: the accumulator fragment of S is the operand fragment of P^T as it is; two tokens' bytes side by side are V^T's
 // Codes are exact in f16.  For fp32 results a step's O is formed from zero and added to fp32 sums, which keeps the MMA's truncating accumulator short; for f16 the
 // accumulators stay in the MMAs.  Weights are 2^14 exp2(s - max): as pairs for fp32, as f16 for f16 results (2^-11 of a weight, as much as the result's own rounding).
 #pragma once
@@ -35,21 +36,21 @@ struct Attend {
 
 constexpr int COUNTERS = 4096;  // arrival counters at the head of a workspace; one for each CTA that begins a shared problem
 
-template <typename T, int D>
+template <typename T, int D, int NR_>
 struct Few {
     static constexpr bool PAIRS = sizeof(T) == 4;
-    static constexpr int ROWS = PAIRS ? 8 : 16;  // query rows of a tile
-    static constexpr int NR = ROWS / 8;          // of them a lane's
-    static constexpr int KS = 2048 / D;          // keys of a warp's step
-    static constexpr int NC = KS / 16;           // groups of 16 keys: one page each
+    static constexpr int NR = NR_;               // groups of 8 query rows in a tile
+    static constexpr int ROWS = 8 * NR;
+    static constexpr int KS = 32, NC = KS / 16;  // keys of a warp's step; groups of 16 of them: one page each
     static constexpr int UNIT = 4 * KS;
-    static constexpr int STAGES = 3;
-    static constexpr int STEP = 4096;            // bytes of a step: keys, then values
+    static constexpr int STAGES = D == 64 ? 3 : 2;
+    static constexpr int K_BYTES = KS * D, STEP = 2 * K_BYTES;
     static constexpr int RING = 4 * STAGES * STEP;
     static constexpr int MERGE = 4 * ROWS * D * 4;  // the warps' sums, in the place of the ring
     static constexpr int BODY = RING > MERGE ? RING : MERGE;
     static constexpr int SMEM = BODY + 4 * STAGES * NC * 8 + 4 * ROWS * 8 + 64;
     static constexpr int PER_SM = 3;
+    static_assert(!PAIRS || NR == 1, "the low parts take rows 8-15");
 };
 constexpr int SLOT_ROWS = 16;
 inline size_t few_workspace(int64_t d) { return COUNTERS * 4 + static_cast<size_t>(sm_count()) * 4 * 2 * SLOT_ROWS * (d + 2) * 4; }
@@ -96,10 +97,10 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache c, const Batch q, const Attend a, const int tiles, unsigned* counters, float* partials) {
-    using L = Few<T, D>;
-    constexpr int ROWS = L::ROWS, NR = L::NR, KS = L::KS, NC = L::NC, PIECES = D / 64, ACC = 2 * NR, SLOT = SLOT_ROWS * (D + 2);
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const Cache c, const Batch q, const Attend a, const int tiles, unsigned* counters, float* partials) {
+    using L = Few<T, D, NR>;
+    constexpr int ROWS = L::ROWS, KS = L::KS, NC = L::NC, PIECES = D / 64, SLOT = SLOT_ROWS * (D + 2);
     dep_sync();
     extern __shared__ __align__(16) uint8_t smem[];
     float2* s_scales = reinterpret_cast<float2*>(smem + L::BODY);                  // [warp][stage][NC] scales of K and V
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
                     const int8_t* vs = v_lane + off;
 #pragma unroll
                     for (int t = 0; t < 4; t++)
-                        copy_async<D / 8>(dst + 2048 + (4 * n + t) * (4 * D) + lane * (D / 8), vs + ((t & 1) + (t >> 1) * 8) * D);
+                        copy_async<D / 8>(dst + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8), vs + ((t & 1) + (t >> 1) * 8) * D);
                 }
                 fill++;
                 if (++fill_stage == L::STAGES) fill_stage = 0;
@@ -227,7 +228,8 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
 
         // ---- queries: fragments of the scores' MMAs, and what each lane's rows see.  (Asked for first, looked at when the first keys are on their way.) ----
         auto relative = [&](int64_t key) { return static_cast<int>(max(min(key - first_key, int64_t(0x7fffff00)), int64_t(0))); };
-        uint32_t qf[4 * PIECES][4];
+        constexpr int QF = L::PAIRS ? 4 : 2 * NR;  // registers of a fragment: rows g (high, low), or g and g + 8
+        uint32_t qf[4 * PIECES][QF];
         float4 qx[L::PAIRS ? 4 * PIECES : 1];
         float factor[NR];
         int sees[NR];  // keys from the warp's first on that the lane's rows see
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
                 } else {
                     const uint2 x = in ? *reinterpret_cast<const uint2*>(at) : make_uint2(0u, 0u);
                     qf[s][r] = x.x;
-                    qf[s][2 + r] = x.y;
+                    qf[s][NR + r] = x.y;
                 }
             }
         }
@@ -270,17 +272,17 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
         }
         const int all_see = relative(min(before + 1 + (tile * ROWS) / a.group, keys));  // that every row of the tile sees
 
-        float acc[D / 8][ACC], top[NR], sum[NR];
+        float acc[D / 16][NR][4], top[NR], sum[NR];  // acc: dims (D / 8) g + 2 i (and + 1: the upper two) of rows 2 c4, 2 c4 + 1
 #pragma unroll
-        for (int i = 0; i < D / 8; i++)
+        for (int i = 0; i < D / 16; i++)
 #pragma unroll
-            for (int r = 0; r < ACC; r++) acc[i][r] = 0.f;
+            for (int r = 0; r < NR; r++) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.f;
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             top[r] = -INFINITY;
             sum[r] = 0.f;
         }
-        float v_ref = 0.f, v_inv = INFINITY, v_top = 0.f;  // the scale of V that the weights are relative to, its reciprocal, the largest so far
+        float v_ref = 0.f, v_inv = 0.f, v_top = 0.f;  // the scale of V that the weights are relative to, its reciprocal, the largest so far
         int stage = 0;
         for (int step = 0; step < steps; step++, stage = stage + 1 == L::STAGES ? 0 : stage + 1) {
             __syncwarp();  // the slot that is filled next has been read, its scales too
@@ -289,65 +291,48 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
             __syncwarp();  // (scales come from other lanes)
             const uint8_t* at = ring_ptr + stage * L::STEP;
             // ---- scores ----
+            float s[KS / 8][4];
+#pragma unroll
+            for (int j = 0; j < KS / 8; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+#pragma unroll
+                for (int j = 0; j < KS / 8; j++) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(at + (j * PIECES + i) * 512 + lane * 16);
+                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t f = word[k] ^ 0x80808080u;
+                        const uint32_t(&qa)[QF] = qf[4 * i + k];
+                        mma_16816(s[j], qa[0], QF == 4 ? qa[1] : 0u, QF == 4 ? qa[2] : qa[1], QF == 4 ? qa[3] : 0u, two_f16(f, 0x4140), two_f16(f, 0x4342));
+                    }
+                }
+            }
             float x[NR][KS / 8][2];
             float most[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) most[r] = top[r];
 #pragma unroll
             for (int j = 0; j < KS / 8; j++) {
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < PIECES; i++) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(at + (j * PIECES + i) * 512 + lane * 16);
-                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t f = word[k] ^ 0x80808080u;
-                        const uint32_t(&qa)[4] = qf[4 * i + k];
-                        mma_16816(s, qa[0], qa[1], qa[2], qa[3], two_f16(f, 0x4140), two_f16(f, 0x4342));
-                    }
-                }
                 const float ks = scales[stage * NC + j / 2].x;
                 if constexpr (L::PAIRS) {
                     const float t = factor[0] * ks;
-                    x[0][j][0] = fmaf(s[2], 1.f / SPLIT_LO, s[0]) * t;
-                    x[0][j][1] = fmaf(s[3], 1.f / SPLIT_LO, s[1]) * t;
+                    x[0][j][0] = fmaf(s[j][2], 1.f / SPLIT_LO, s[j][0]) * t;
+                    x[0][j][1] = fmaf(s[j][3], 1.f / SPLIT_LO, s[j][1]) * t;
                 } else {
 #pragma unroll
                     for (int r = 0; r < NR; r++) {
                         const float t = factor[r] * ks;
-                        x[r][j][0] = s[2 * r] * t;
-                        x[r][j][1] = s[2 * r + 1] * t;
+                        x[r][j][0] = s[j][2 * r] * t;
+                        x[r][j][1] = s[j][2 * r + 1] * t;
                     }
                 }
             }
-            // Scales of V go into the weights, relative to one for all that an accumulator takes in (infinities and NaN as they are).
-            float vs[NR][NC], v_step = 0.f;
+            float vs[NR][NC];  // scales of V as the lane's rows see them
 #pragma unroll
-            for (int n = 0; n < NC; n++) {
-                const float v = scales[stage * NC + n].y;
-                if (v < INFINITY) v_step = fmaxf(v_step, v);
-            }
-            if constexpr (L::PAIRS) {  // the step's largest
-                v_ref = v_step;
-                v_inv = 1.f / v_step;
-            } else if (v_step > v_ref || (v_step < v_ref * 2.44140625e-4f && v_step > v_top * 5.42101086e-20f)) {
-                // the one that the sums are in, as long as the ratio is moderate (2^-12; 2^-64: so far down sums might leave fp32's range)
-                const float f = v_ref / v_step;
+            for (int n = 0; n < NC; n++)
 #pragma unroll
-                for (int i = 0; i < D / 8; i++)
-#pragma unroll
-                    for (int r = 0; r < ACC; r++) acc[i][r] *= f;
-                v_ref = v_step;
-                v_inv = 1.f / v_step;
-                v_top = fmaxf(v_top, v_step);
-            }
-#pragma unroll
-            for (int n = 0; n < NC; n++) {
-                const float v = scales[stage * NC + n].y;
-#pragma unroll
-                for (int r = 0; r < NR; r++) vs[r][n] = v == v_ref ? 1.f : v * v_inv;
-            }
+                for (int r = 0; r < NR; r++) vs[r][n] = scales[stage * NC + n].y;
             if (KS + step * L::UNIT > all_see) {
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
@@ -376,10 +361,13 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
                     const float corr = top[r] == -INFINITY ? 0.f : ex2(top[r] - most[r]);
                     top[r] = most[r];
                     sum[r] *= corr;
+                    const float even = __shfl_sync(0xffffffffu, corr, 8 * c4), odd = __shfl_sync(0xffffffffu, corr, 8 * c4 + 4);  // of rows 2 c4, 2 c4 + 1
 #pragma unroll
-                    for (int i = 0; i < D / 8; i++) {
-                        acc[i][2 * r] *= corr;
-                        acc[i][2 * r + 1] *= corr;
+                    for (int i = 0; i < D / 16; i++) {
+                        acc[i][r][0] *= even;
+                        acc[i][r][1] *= odd;
+                        acc[i][r][2] *= even;
+                        acc[i][r][3] *= odd;
                     }
                 }
             }
@@ -394,53 +382,88 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
                 }
             }
             // ---- values ----
-            uint32_t p[NC][4], v[NC][4][D / 32];
+            // Scales of V go into the weights, relative to the one that the accumulators are in: that of the 16 keys before, as long as the ratio is
+            // between 2 (weights stay in f16's range) and 2^-12.  (Infinities and NaN go into the weights as they are.)
+            float fresh[L::PAIRS ? D / 16 : 1][4];
 #pragma unroll
             for (int n = 0; n < NC; n++) {
+                const float scale = scales[stage * NC + n].y, ref = scale < INFINITY ? fmaxf(scale, 1.17549435e-38f) : 1.f;
                 if constexpr (L::PAIRS) {
-                    split2(x[0][2 * n][0] * vs[0][n], x[0][2 * n][1] * vs[0][n], p[n][0], p[n][1]);
-                    split2(x[0][2 * n + 1][0] * vs[0][n], x[0][2 * n + 1][1] * vs[0][n], p[n][2], p[n][3]);
-                } else {
+                    const bool other = n > 0 && (ref > 2.f * v_ref || ref < v_ref * 2.44140625e-4f);
+                    if (other) {
 #pragma unroll
-                    for (int r = 0; r < NR; r++) {
-                        p[n][r] = pack_f16(x[r][2 * n][0] * vs[r][n], x[r][2 * n][1] * vs[r][n]);
-                        p[n][2 + r] = pack_f16(x[r][2 * n + 1][0] * vs[r][n], x[r][2 * n + 1][1] * vs[r][n]);
+                        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[i][0][e] = fmaf(fresh[i][e], v_ref, acc[i][0][e]);
+                    }
+                    if (n == 0 || other) {
+#pragma unroll
+                        for (int i = 0; i < D / 16; i++) fresh[i][0] = fresh[i][1] = fresh[i][2] = fresh[i][3] = 0.f;
+                        v_ref = ref;
+                        v_inv = 1.f / ref;
+                    }
+                } else if (scale < INFINITY && (ref > 2.f * v_ref || (ref < v_ref * 2.44140625e-4f && ref > v_top * 5.42101086e-20f))) {  // (2^-64: further down sums might leave fp32's range)
+                    const float f = v_ref / ref;
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                        for (int r = 0; r < 4 * NR; r++) acc[i][r >> 2][r & 3] *= f;
+                    v_ref = ref;
+                    v_inv = 1.f / ref;
+                    v_top = fmaxf(v_top, ref);
+                }
+                uint32_t p[2][2];  // rows 0-7 and 8-15, or the high and low parts: tokens 2 c4, 2 c4 + 1 and 8 further on
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    if constexpr (L::PAIRS) {
+                        const float w = vs[0][n] * v_inv, y0 = x[0][2 * n + e][0] * w, y1 = x[0][2 * n + e][1] * w;
+                        const __half2 high = __floats2half2_rn(y0, y1);
+                        const float2 back = __half22float2(high);
+                        p[0][e] = *reinterpret_cast<const uint32_t*>(&high);
+                        p[1][e] = pack_f16(y0 - back.x, y1 - back.y);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < NR; r++) {
+                            const float w = vs[r][n] * v_inv;
+                            p[r][e] = pack_f16(x[r][2 * n + e][0] * w, x[r][2 * n + e][1] * w);
+                        }
+                    }
+                }
+                uint32_t v[4][D / 32];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const uint8_t* src = at + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8);
+                    if constexpr (D == 64) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(src);
+                        v[t][0] = w.x ^ 0x80808080u;
+                        v[t][1] = w.y ^ 0x80808080u;
+                    } else {
+                        const uint4 w = *reinterpret_cast<const uint4*>(src);
+                        v[t][0] = w.x ^ 0x80808080u;
+                        v[t][1] = w.y ^ 0x80808080u;
+                        v[t][2] = w.z ^ 0x80808080u;
+                        v[t][3] = w.w ^ 0x80808080u;
                     }
                 }
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const uint8_t* src = at + 2048 + (4 * n + t) * (4 * D) + lane * (D / 8);
-                    if constexpr (D == 64) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(src);
-                        v[n][t][0] = w.x ^ 0x80808080u;
-                        v[n][t][1] = w.y ^ 0x80808080u;
+                for (int i = 0; i < D / 16; i++) {
+                    // two tokens side by side, of dims 2 i and 2 i + 1 of the lane's
+                    const uint32_t near = __byte_perm(v[0][i / 2], v[1][i / 2], i & 1 ? 0x7362 : 0x5140), far = __byte_perm(v[2][i / 2], v[3][i / 2], i & 1 ? 0x7362 : 0x5140);
+                    const uint32_t a0 = two_f16(near, 0x4140), a1 = two_f16(near, 0x4342), a2 = two_f16(far, 0x4140), a3 = two_f16(far, 0x4342);
+                    if constexpr (L::PAIRS) {
+                        mma_16816(fresh[i], a0, a1, a2, a3, p[1][0], p[1][1]);
+                        mma_16816(fresh[i], a0, a1, a2, a3, p[0][0], p[0][1]);
                     } else {
-                        const uint4 w = *reinterpret_cast<const uint4*>(src);
-                        v[n][t][0] = w.x ^ 0x80808080u;
-                        v[n][t][1] = w.y ^ 0x80808080u;
-                        v[n][t][2] = w.z ^ 0x80808080u;
-                        v[n][t][3] = w.w ^ 0x80808080u;
+#pragma unroll
+                        for (int r = 0; r < NR; r++) mma_16816(acc[i][r], a0, a1, a2, a3, p[r][0], p[r][1]);
                     }
                 }
             }
+            if constexpr (L::PAIRS) {
 #pragma unroll
-            for (int w = 0; w < D / 32; w++) {
+                for (int i = 0; i < D / 16; i++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    float fresh[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int n = 0; n < NC; n++) {
-                        // tokens 2 c4, 2 c4 + 1 (and 8 further on) side by side, two dims at a time
-                        const uint32_t near = __byte_perm(v[n][0][w], v[n][1][w], k < 2 ? 0x5140 : 0x7362), far = __byte_perm(v[n][2][w], v[n][3][w], k < 2 ? 0x5140 : 0x7362);
-                        const uint32_t sel = k & 1 ? 0x4342 : 0x4140;
-                        if constexpr (L::PAIRS) mma_16816(fresh, p[n][0], p[n][1], p[n][2], p[n][3], two_f16(near, sel), two_f16(far, sel));
-                        else mma_16816(acc[4 * w + k], p[n][0], p[n][1], p[n][2], p[n][3], two_f16(near, sel), two_f16(far, sel));
-                    }
-                    if constexpr (L::PAIRS) {
-                        acc[4 * w + k][0] = fmaf(fmaf(fresh[2], 1.f / SPLIT_LO, fresh[0]), v_step, acc[4 * w + k][0]);
-                        acc[4 * w + k][1] = fmaf(fmaf(fresh[3], 1.f / SPLIT_LO, fresh[1]), v_step, acc[4 * w + k][1]);
-                    }
-                }
+                    for (int e = 0; e < 4; e++) acc[i][0][e] = fmaf(fresh[i][e], v_ref, acc[i][0][e]);
             }
         }
 
@@ -451,18 +474,16 @@ __global__ void __launch_bounds__(128, Few<T, D>::PER_SM) few_kernel(const Cache
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             sum[r] = quad_sum(sum[r]);
-            const int row = g + 8 * r;
-            const float up = L::PAIRS ? 1.f : v_ref;
             if (c4 == 0) {
-                s_top[warp * ROWS + row] = top[r];
-                s_sum[warp * ROWS + row] = sum[r];
+                s_top[warp * ROWS + g + 8 * r] = top[r];
+                s_sum[warp * ROWS + g + 8 * r] = sum[r];
             }
+            const float up = L::PAIRS ? 1.f : v_ref;
+            float* dst = merge + (warp * ROWS + 2 * c4 + 8 * r) * D + g * (D / 8);
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float4* dst = reinterpret_cast<float4*>(merge + (warp * ROWS + row) * D + (2 * c4 + e) * (D / 8));
-#pragma unroll
-                for (int i = 0; i < D / 32; i++)
-                    dst[i] = make_float4(acc[4 * i][2 * r + e] * up, acc[4 * i + 1][2 * r + e] * up, acc[4 * i + 2][2 * r + e] * up, acc[4 * i + 3][2 * r + e] * up);
+            for (int i = 0; i < D / 16; i++) {
+                *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc[i][r][0] * up, acc[i][r][2] * up);
+                *reinterpret_cast<float2*>(dst + D + 2 * i) = make_float2(acc[i][r][1] * up, acc[i][r][3] * up);
             }
         }
         __syncthreads();
