@@ -4,10 +4,12 @@
 // the memory system, and the products go to mma.sync on registers: a tcgen05 tile has 128 rows, of which a step would fill 4 or 8, and wants its operands in
 // shared memory as f16, which costs more than the products themselves.
 //
-// Shares.  The keys of all (sequence, KV head, row tile) problems lie behind one another in units of 4 x KS keys, and the CTAs - as many as are resident
-// at once - take equal parts of that line, whatever the lengths of the sequences; the host does not know them.  A CTA writes the result of a problem that is all its
-// own, and a partial one (sums, maximum, weights' sum) of a problem that it shares to the workspace; the CTA that finishes last adds them up in their order
-// along the keys, so the result does not depend on which one that is.
+// Shares.  The keys of all (sequence, KV head, row tile) problems lie behind one another in units of 4 x 32 keys, and the CTAs - as many as are resident
+// at once - take equal parts of that line, whatever the lengths of the sequences; the host does not know them.  A CTA's piece of a problem is a segment.  A warp
+// asks for the keys of its next segment while it still works on the one before, so the stream of loads does not stop between them; a segment's four shares are joined
+// warp to warp, and a warp that has handed its own on goes on.  (With the whole CTA waiting at each end, 64 requests over 1000 keys took 24 us.)
+// A problem that several CTAs share leaves partial results (sums, maximum, weights' sum) in the workspace; the CTA that comes last adds them up in their
+// order along the keys, so the result does not depend on which one that is.
 //
 // A warp's step: 32 keys.  Each lane copies by cp.async just the bytes that it will read itself; no lane waits for another.  The order of a contraction is
 // free, so a lane's 16 consecutive bytes of a key are its operands of four MMAs (four dims to each), and bytes become f16 in registers:
@@ -46,14 +48,14 @@ struct Few {
     static constexpr int STAGES = D == 64 ? 3 : 2;
     static constexpr int K_BYTES = KS * D, STEP = 2 * K_BYTES;
     static constexpr int RING = 4 * STAGES * STEP;
-    static constexpr int MERGE = 4 * ROWS * D * 4;  // the warps' sums, in the place of the ring
-    static constexpr int BODY = RING > MERGE ? RING : MERGE;
-    static constexpr int SMEM = BODY + 4 * STAGES * NC * 8 + 4 * ROWS * 8 + 64;
-    static constexpr int PER_SM = 3;
+    static constexpr int FRAGS = D / 16 * NR;    // groups of four sums per lane
+    static constexpr int HAND = 32 * (FRAGS * 16 + NR * 8);  // a warp's share on its way to another: sums, maxima, weights' sums
+    static constexpr int SCALES = RING + 2 * HAND, SCAN = SCALES + 4 * STAGES * NC * 8, SMEM = SCAN + 64;
+    static constexpr int PER_SM = NR == 2 && D == 128 ? 2 : 3;
     static_assert(!PAIRS || NR == 1, "the low parts take rows 8-15");
 };
-constexpr int SLOT_ROWS = 16;
-inline size_t few_workspace(int64_t d) { return COUNTERS * 4 + static_cast<size_t>(sm_count()) * 4 * 2 * SLOT_ROWS * (d + 2) * 4; }
+constexpr int MOST_PARTS = 32;  // CTAs for a problem, on average: each costs the last one a fraction of a microsecond
+inline size_t few_workspace(int64_t d) { return COUNTERS * 4 + static_cast<size_t>(sm_count()) * 4 * 2 * (32 * (d / 16 * 2 * 16 + 2 * 8)); }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -89,24 +91,117 @@ __device__ __forceinline__ float quad_sum(float x) {
     x += __shfl_xor_sync(0xffffffffu, x, 1);
     return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
-// a share of a softmax under another maximum: a share without keys has the maximum -inf and sums of zero (or NaN, which has to stay)
-__device__ __forceinline__ float share_weight(float m, float most) { return m == -INFINITY ? 1.f : ex2(m - most); }
-
 // a / b for 0 <= a, 0 < b: nearly always in 32 bits, where a division is a fifth of the instructions
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
 }
 
+// named barriers between two warps: one hands over and goes on, the other waits
+template <int ID>
+__device__ __forceinline__ void pair_arrive() { asm volatile("bar.arrive %0, 64;" ::"n"(ID) : "memory"); }
+template <int ID>
+__device__ __forceinline__ void pair_wait() { asm volatile("bar.sync %0, 64;" ::"n"(ID) : "memory"); }
+enum { HAND_0 = 1, HAND_1, HAND_UP, FREE_0, FREE_1 };
+
+// What a lane knows of a tile's rows: sums over keys of w v (dims (D / 8) g + 2 i, and + 1 in the upper two, of rows 2 c4, 2 c4 + 1), the largest score and the sum of
+// the weights of rows g (and g + 8).
+template <int D, int NR>
+struct Share {
+    float acc[D / 16][NR][4], top[NR], sum[NR];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            top[r] = -INFINITY;
+            sum[r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.f;
+        }
+    }
+    // rows 2 c4 and 2 c4 + 1 of something that lanes hold for row g
+    static __device__ __forceinline__ float2 of_sums(float f, int c4) { return make_float2(__shfl_sync(0xffffffffu, f, 8 * c4), __shfl_sync(0xffffffffu, f, 8 * c4 + 4)); }
+    __device__ __forceinline__ void scale(int r, float f, int c4) {
+        const float2 k = of_sums(f, c4);
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) {
+            acc[i][r][0] *= k.x;
+            acc[i][r][1] *= k.y;
+            acc[i][r][2] *= k.x;
+            acc[i][r][3] *= k.y;
+        }
+    }
+    // to and from memory that holds it lane by lane
+    __device__ __forceinline__ void put(float* at, int lane) const {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            *reinterpret_cast<float2*>(at + 128 * (D / 16) * NR + 64 * r + 2 * lane) = make_float2(top[r], sum[r]);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+                *reinterpret_cast<float4*>(at + 128 * (i * NR + r) + 4 * lane) = make_float4(acc[i][r][0], acc[i][r][1], acc[i][r][2], acc[i][r][3]);
+        }
+    }
+    __device__ __forceinline__ void get(const float* at, int lane) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            const float2 t = __ldcg(reinterpret_cast<const float2*>(at + 128 * (D / 16) * NR + 64 * r + 2 * lane));
+            top[r] = t.x;
+            sum[r] = t.y;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(at + 128 * (i * NR + r) + 4 * lane));
+                acc[i][r][0] = x.x;
+                acc[i][r][1] = x.y;
+                acc[i][r][2] = x.z;
+                acc[i][r][3] = x.w;
+            }
+        }
+    }
+    // A share without keys has the maximum -inf and sums of zero (or NaN, which has to stay).
+    __device__ __forceinline__ void join(int r, float other_top, float other_sum, int c4, float2& own, float2& other) {
+        const float most = fmaxf(top[r], other_top);
+        const float f = top[r] == -INFINITY ? 1.f : ex2(top[r] - most), o = other_top == -INFINITY ? 1.f : ex2(other_top - most);
+        top[r] = most;
+        sum[r] = fmaf(other_sum, o, sum[r] * f);
+        own = of_sums(f, c4);
+        other = of_sums(o, c4);
+    }
+    __device__ __forceinline__ void join(const Share& x, int c4) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            float2 f, o;
+            join(r, x.top[r], x.sum[r], c4, f, o);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][r][e] = fmaf(x.acc[i][r][e], e & 1 ? o.y : o.x, acc[i][r][e] * (e & 1 ? f.y : f.x));
+        }
+    }
+    __device__ __forceinline__ void join_shared(const float* at, int lane, int c4) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            const float2 t = *reinterpret_cast<const float2*>(at + 128 * (D / 16) * NR + 64 * r + 2 * lane);
+            float2 f, o;
+            join(r, t.x, t.y, c4, f, o);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const float4 x = *reinterpret_cast<const float4*>(at + 128 * (i * NR + r) + 4 * lane);
+                acc[i][r][0] = fmaf(x.x, o.x, acc[i][r][0] * f.x);
+                acc[i][r][1] = fmaf(x.y, o.y, acc[i][r][1] * f.y);
+                acc[i][r][2] = fmaf(x.z, o.x, acc[i][r][2] * f.x);
+                acc[i][r][3] = fmaf(x.w, o.y, acc[i][r][3] * f.y);
+            }
+        }
+    }
+};
+
 template <typename T, int D, int NR>
 __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const Cache c, const Batch q, const Attend a, const int tiles, unsigned* counters, float* partials) {
     using L = Few<T, D, NR>;
-    constexpr int ROWS = L::ROWS, KS = L::KS, NC = L::NC, PIECES = D / 64, SLOT = SLOT_ROWS * (D + 2);
+    constexpr int ROWS = L::ROWS, KS = L::KS, NC = L::NC, PIECES = D / 64, SLOT = L::HAND / 4;
     dep_sync();
     extern __shared__ __align__(16) uint8_t smem[];
-    float2* s_scales = reinterpret_cast<float2*>(smem + L::BODY);                  // [warp][stage][NC] scales of K and V
-    float* s_top = reinterpret_cast<float*>(smem + L::BODY + 4 * L::STAGES * NC * 8);  // [warp][ROWS]
-    float* s_sum = s_top + 4 * ROWS;
-    int64_t* s_at = reinterpret_cast<int64_t*>(smem + L::SMEM - 64);  // scan, then where the share begins
+    float* s_hand = reinterpret_cast<float*>(smem + L::RING);
+    int64_t* s_at = reinterpret_cast<int64_t*>(smem + L::SCAN);  // scan, where the share begins, at the end whether this CTA was the last one
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
     const int64_t table_keys = q.width << c.page_log;
     // keys behind the table have no page: one of them stands for all
@@ -115,8 +210,8 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
     const int64_t items = static_cast<int64_t>(c.kv_heads) * tiles;  // problems of a sequence
 
     // ---- this CTA's share of the line ----
-    int64_t total, per, lo, hi, seq_first;  // seq_first: where sequence b begins on the line
-    int b;
+    int64_t total, per, lo, hi, share_seq;  // share_seq: where the sequence that the share begins in begins on the line
+    int share_b;
     unsigned workers, longer;  // the first `longer` workers have per + 1 units, the others per
     auto begin_of = [&](unsigned w) { return per * w + min(w, longer); };
     auto worker_of = [&](int64_t unit) {
@@ -138,7 +233,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
         __syncthreads();
         total = s_at[0] + s_at[1] + s_at[2] + s_at[3];
         for (int w = 0; w < warp; w++) upto += s_at[w];
-        workers = static_cast<unsigned>(min(static_cast<int64_t>(gridDim.x), total));
+        workers = static_cast<unsigned>(min(min(static_cast<int64_t>(gridDim.x), total), MOST_PARTS * items * q.batch));
         if (blockIdx.x >= workers) return;
         per = divide(total, workers);
         longer = static_cast<unsigned>(total - per * workers);
@@ -158,73 +253,122 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             }
         }
         __syncthreads();
-        b = static_cast<int>(s_at[0]);
-        seq_first = s_at[1];
+        share_b = static_cast<int>(s_at[0]);
+        share_seq = s_at[1];
     }
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (L::STAGES * L::STEP);
     const uint8_t* ring_ptr = smem + warp * (L::STAGES * L::STEP);
-    float2* scales = s_scales + warp * (L::STAGES * NC);
+    float2* scales = reinterpret_cast<float2*>(smem + L::SCALES) + warp * (L::STAGES * NC);  // of K and V, [stage][NC]
     const int rows = q.each * a.group;
 
-    for (int64_t unit = lo; unit < hi;) {
-        const int64_t keys = keys_of(b), units = units_of(b);
-        const int64_t item = divide(unit - seq_first, units), unit0 = (unit - seq_first) - item * units;
-        const int64_t taken = min(units - unit0, hi - unit);
-        const int h = static_cast<int>(item) / tiles, tile = static_cast<int>(item - static_cast<int64_t>(h) * tiles);
-        const int64_t key0 = unit0 * L::UNIT, key1 = min(keys, (unit0 + taken) * L::UNIT);
-        const int64_t before = static_cast<int64_t>(q.lens[b]) - q.each;  // keys before the first new token
+    // A segment, as a warp sees it: its steps are the keys first_key + i UNIT.
+    struct Segment {
+        int b, h, tile, steps, left;  // left: keys from the warp's first to the segment's end
+        int64_t seq, unit, units, taken, first_key;  // where the sequence and the segment begin on the line; units of a problem, of them in the segment
+    };
+    auto look = [&](Segment& s) {
+        const int64_t keys = keys_of(s.b);
+        s.units = units_of(s.b);
+        const int64_t item = divide(s.unit - s.seq, s.units), unit0 = (s.unit - s.seq) - item * s.units;
+        s.taken = min(s.units - unit0, hi - s.unit);
+        s.h = static_cast<int>(item) / tiles;
+        s.tile = static_cast<int>(item) - s.h * tiles;
+        s.first_key = unit0 * L::UNIT + warp * KS;
+        const int64_t left = min(keys, (unit0 + s.taken) * L::UNIT) - s.first_key;
+        s.left = static_cast<int>(min(max(left, int64_t(0)), int64_t(0x7fffff00)));  // (2^31 keys are none of a cache's)
+        s.steps = (s.left + L::UNIT - 1) / L::UNIT;
+    };
+    auto move_on = [&](Segment& s) {
+        s.unit += s.taken;
+        if (s.unit - s.seq == s.units * items) {
+            s.seq = s.unit;
+            s.b++;
+        }
+        if (s.unit < hi) look(s);
+    };
 
-        // ---- the warp's steps: keys key0 + (4 i + warp) KS ----
-        const int64_t first_key = key0 + warp * KS;
-        const int left = static_cast<int>(min(max(key1 - first_key, int64_t(0)), int64_t(0x7fffff00)));  // (keys behind the table are cut off, 2^31 of them are none of a cache's)
-        const int steps = (left + L::UNIT - 1) / L::UNIT;
-        int block = -1;  // page and head as one index; -1: no key there, -2: a key without a page
-        // blocks of PAGED_STEPS steps at a time, one per lane
-        constexpr int PAGED_STEPS = 32 / NC;
-        auto fetch_blocks = [&](int step) {
-            const int off = (step + lane / NC) * L::UNIT + (lane % NC) * 16;
-            block = -1;
-            if (off < left) {
-                const int64_t at = (first_key + off) >> c.page_log;
-                const int p = at < q.width ? q.table[static_cast<int64_t>(b) * q.width + at] : -1;
-                block = p >= 0 && p < c.pages ? p * c.kv_heads + h : -2;
-                if (block == -2 && a.status) *a.status = RMLK_ERR_INVALID_ARG;
-            }
-        };
-        const int slot_base = static_cast<int>(first_key & 127);  // (a page has 128 keys at most)
-        const int8_t* k_lane = c.k + g * D + c4 * 16;
-        const int8_t* v_lane = c.v + 2 * c4 * D + g * (D / 8);
-        const int block_bytes = c.page * D;
-        int fill = 0, fill_stage = 0;  // next step to be asked for, its place in the ring
-        auto issue = [&]() {
-            if (fill < steps) {
-                const int in_batch = fill % PAGED_STEPS;
-                if (in_batch == 0) fetch_blocks(fill);
-                const uint32_t dst = ring + fill_stage * L::STEP;
-#pragma unroll
-                for (int n = 0; n < NC; n++) {
-                    const int at = __shfl_sync(0xffffffffu, block, in_batch * NC + n), from = at < 0 ? h : at;  // (page 0 is read where there is none)
-                    if (lane < 2) {  // the scales of K and V: 0 where there is no key, NaN where a key has no page
-                        float* to = reinterpret_cast<float*>(scales + fill_stage * NC + n) + lane;
-                        if (at >= 0) copy_async<4>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), (lane ? c.vs : c.ks) + at);
-                        else *to = at == -1 ? 0.f : __int_as_float(0x7fc00000);
-                    }
-                    const int64_t off = static_cast<int64_t>(from) * block_bytes + ((slot_base + fill * L::UNIT + 16 * n) & (c.page - 1)) * D;
-                    const int8_t* ks = k_lane + off;
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int i = 0; i < PIECES; i++) copy_async<16>(dst + ((2 * n + j) * PIECES + i) * 512 + lane * 16, ks + j * 8 * D + i * 64);
-                    const int8_t* vs = v_lane + off;
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-                        copy_async<D / 8>(dst + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8), vs + ((t & 1) + (t >> 1) * 8) * D);
+    // ---- the stream of loads ----
+    Segment ask;
+    ask.b = share_b;
+    ask.seq = share_seq;
+    ask.unit = lo;
+    look(ask);
+    Segment now = ask;
+    int block = -1;  // page and head as one index; -1: no key there, -2: a key without a page
+    constexpr int PAGED_STEPS = 32 / NC;  // pages of so many steps are looked up at a time, one per lane
+    const int8_t* k_lane = c.k + g * D + c4 * 16;
+    const int8_t* v_lane = c.v + 2 * c4 * D + g * (D / 8);
+    const int block_bytes = c.page * D;
+    int fill = 0, fill_stage = 0;  // next step to be asked for, its place in the ring
+    auto issue = [&]() {
+        while (fill == ask.steps && ask.unit < hi) {
+            move_on(ask);
+            fill = 0;
+            if (ask.unit >= hi) ask.steps = 0;
+        }
+        if (fill < ask.steps) {
+            const int in_batch = fill % PAGED_STEPS;
+            if (in_batch == 0) {
+                const int off = (fill + lane / NC) * L::UNIT + (lane % NC) * 16;
+                block = -1;
+                if (off < ask.left) {
+                    const int64_t at = (ask.first_key + off) >> c.page_log;
+                    const int p = at < q.width ? q.table[static_cast<int64_t>(ask.b) * q.width + at] : -1;
+                    block = p >= 0 && p < c.pages ? p * c.kv_heads + ask.h : -2;
+                    if (block == -2 && a.status) *a.status = RMLK_ERR_INVALID_ARG;
                 }
-                fill++;
-                if (++fill_stage == L::STAGES) fill_stage = 0;
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+            const uint32_t dst = ring + fill_stage * L::STEP;
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const int at = __shfl_sync(0xffffffffu, block, in_batch * NC + n), from = at < 0 ? ask.h : at;  // (page 0 is read where there is none)
+                if (lane < 2) {  // the scales of K and V: 0 where there is no key, NaN where a key has no page
+                    float* to = reinterpret_cast<float*>(scales + fill_stage * NC + n) + lane;
+                    if (at >= 0) copy_async<4>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), (lane ? c.vs : c.ks) + at);
+                    else *to = at == -1 ? 0.f : __int_as_float(0x7fc00000);
+                }
+                const int64_t off = static_cast<int64_t>(from) * block_bytes + ((static_cast<int>(ask.first_key & 127) + fill * L::UNIT + 16 * n) & (c.page - 1)) * D;
+                const int8_t* ks = k_lane + off;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int i = 0; i < PIECES; i++) copy_async<16>(dst + ((2 * n + j) * PIECES + i) * 512 + lane * 16, ks + j * 8 * D + i * 64);
+                const int8_t* vs = v_lane + off;
+#pragma unroll
+                for (int t = 0; t < 4; t++) copy_async<D / 8>(dst + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8), vs + ((t & 1) + (t >> 1) * 8) * D);
+            }
+            fill++;
+            if (++fill_stage == L::STAGES) fill_stage = 0;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // a finished tile; a row that sees nothing is 0
+    auto store = [&](const Share<D, NR>& x, int b, int h, int tile) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            const float2 l = Share<D, NR>::of_sums(x.sum[r], c4);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int row = tile * ROWS + 8 * r + 2 * c4 + e, token = row / a.group;
+                if (row >= rows) continue;
+                const float sum = e ? l.y : l.x, inv = sum == 0.f ? 0.f : 1.f / sum;
+                T* dst = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * q.each + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D + g * (D / 8);
+#pragma unroll
+                for (int i = 0; i < D / 16; i += 2) {
+                    const float4 o = make_float4(x.acc[i][r][e] * inv, x.acc[i][r][2 + e] * inv, x.acc[i + 1][r][e] * inv, x.acc[i + 1][r][2 + e] * inv);
+                    if constexpr (L::PAIRS) *reinterpret_cast<float4*>(dst + 2 * i) = o;
+                    else *reinterpret_cast<uint2*>(dst + 2 * i) = make_uint2(pack_f16(o.x, o.y), pack_f16(o.z, o.w));
+                }
+            }
+        }
+    };
+    int stage = 0;
+    bool first = true, handed = false;  // first segment of the CTA; the hand-over places have been used
+
+    while (now.unit < hi) {
+        const int b = now.b, h = now.h, tile = now.tile;
+        const int64_t keys = keys_of(b), first_key = now.first_key;
+        const int64_t before = static_cast<int64_t>(q.lens[b]) - q.each;  // keys before the first new token
 
         // ---- queries: fragments of the scores' MMAs, and what each lane's rows see.  (Asked for first, looked at when the first keys are on their way.) ----
         auto relative = [&](int64_t key) { return static_cast<int>(max(min(key - first_key, int64_t(0x7fffff00)), int64_t(0))); };
@@ -252,8 +396,10 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                 }
             }
         }
+        if (first) {
 #pragma unroll
-        for (int s = 0; s < L::STAGES - 1; s++) issue();
+            for (int s = 0; s < L::STAGES - 1; s++) issue();
+        }
         if constexpr (L::PAIRS) {
             uint32_t most = 0;
 #pragma unroll
@@ -272,19 +418,13 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
         }
         const int all_see = relative(min(before + 1 + (tile * ROWS) / a.group, keys));  // that every row of the tile sees
 
-        float acc[D / 16][NR][4], top[NR], sum[NR];  // acc: dims (D / 8) g + 2 i (and + 1: the upper two) of rows 2 c4, 2 c4 + 1
-#pragma unroll
-        for (int i = 0; i < D / 16; i++)
-#pragma unroll
-            for (int r = 0; r < NR; r++) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.f;
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            top[r] = -INFINITY;
-            sum[r] = 0.f;
-        }
+        Share<D, NR> own;
+        own.clear();
+        float(&acc)[D / 16][NR][4] = own.acc;
+        float(&top)[NR] = own.top;
+        float(&sum)[NR] = own.sum;
         float v_ref = 0.f, v_inv = 0.f, v_top = 0.f;  // the scale of V that the weights are relative to, its reciprocal, the largest so far
-        int stage = 0;
-        for (int step = 0; step < steps; step++, stage = stage + 1 == L::STAGES ? 0 : stage + 1) {
+        for (int step = 0; step < now.steps; step++, stage = stage + 1 == L::STAGES ? 0 : stage + 1) {
             __syncwarp();  // the slot that is filled next has been read, its scales too
             issue();
             asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 1) : "memory");
@@ -361,14 +501,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                     const float corr = top[r] == -INFINITY ? 0.f : ex2(top[r] - most[r]);
                     top[r] = most[r];
                     sum[r] *= corr;
-                    const float even = __shfl_sync(0xffffffffu, corr, 8 * c4), odd = __shfl_sync(0xffffffffu, corr, 8 * c4 + 4);  // of rows 2 c4, 2 c4 + 1
-#pragma unroll
-                    for (int i = 0; i < D / 16; i++) {
-                        acc[i][r][0] *= even;
-                        acc[i][r][1] *= odd;
-                        acc[i][r][2] *= even;
-                        acc[i][r][3] *= odd;
-                    }
+                    own.scale(r, corr, c4);
                 }
             }
 #pragma unroll
@@ -467,114 +600,91 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             }
         }
 
-        // ---- the four warps' shares ----
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
-        float* merge = reinterpret_cast<float*>(smem);
+        // ---- the four warps' shares: 2 to 0, 3 to 1, 1 to 0 ----
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             sum[r] = quad_sum(sum[r]);
-            if (c4 == 0) {
-                s_top[warp * ROWS + g + 8 * r] = top[r];
-                s_sum[warp * ROWS + g + 8 * r] = sum[r];
-            }
-            const float up = L::PAIRS ? 1.f : v_ref;
-            float* dst = merge + (warp * ROWS + 2 * c4 + 8 * r) * D + g * (D / 8);
+            if constexpr (!L::PAIRS) {
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc[i][r][0] * up, acc[i][r][2] * up);
-                *reinterpret_cast<float2*>(dst + D + 2 * i) = make_float2(acc[i][r][1] * up, acc[i][r][3] * up);
+                for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][r][e] *= v_ref;
             }
+        }
+        if (warp >= 2) {
+            if (handed) {
+                if (warp == 2) pair_wait<FREE_0>();
+                else pair_wait<FREE_1>();
+            }
+            own.put(s_hand + (warp - 2) * SLOT, lane);
+            if (warp == 2) pair_arrive<HAND_0>();
+            else pair_arrive<HAND_1>();
+        } else if (warp == 1) {
+            pair_wait<HAND_1>();
+            own.join_shared(s_hand + SLOT, lane, c4);
+            own.put(s_hand + SLOT, lane);  // (each lane where it has just read)
+            pair_arrive<HAND_UP>();
+        } else {
+            pair_wait<HAND_0>();
+            own.join_shared(s_hand, lane, c4);
+            pair_arrive<FREE_0>();
+            pair_wait<HAND_UP>();
+            own.join_shared(s_hand + SLOT, lane, c4);
+            pair_arrive<FREE_1>();
+            if (now.taken == now.units) store(own, b, h, tile);
+            else own.put(partials + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * SLOT, lane);
+        }
+        handed = true;
+        first = false;
+        if (now.unit + now.taken == hi) break;
+        move_on(now);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (warp == 2) pair_wait<FREE_0>();  // (no arrival is left open)
+    if (warp == 3) pair_wait<FREE_1>();
+
+    // ---- problems that are shared with other CTAs: at most the share's first and last ----
+    // first: begun before the share; last: goes on behind it (one and the same, where the share lies within a problem)
+    auto finish = [&](const Segment& s) {
+        const int64_t begin = s.seq + divide(s.unit - s.seq, s.units) * s.units;
+        const unsigned w0 = worker_of(begin), w1 = worker_of(begin + s.units - 1), parts = w1 - w0 + 1;
+        __syncthreads();
+        if (tid == 0) {
+            __threadfence();
+            s_at[0] = atomicInc(&counters[w0], w1 - w0) == w1 - w0;  // back to zero with the last one
+            __threadfence();
         }
         __syncthreads();
-        const int64_t item_first = seq_first + item * units;
-        const bool whole = taken == units;
-        const int valid = min(ROWS, rows - tile * ROWS);
-        float* slot = partials + (static_cast<int64_t>(blockIdx.x) * 2 + (unit == lo ? 0 : 1)) * SLOT;
-        auto put = [&](int row, int col, float4 o, float l) {
-            const int at_row = tile * ROWS + row, token = at_row / a.group;
-            const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is 0
-            T* dst = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * q.each + token) * a.os + (static_cast<int64_t>(h) * a.group + at_row - token * a.group) * D + col;
-            if constexpr (L::PAIRS) *reinterpret_cast<float4*>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-            else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(o.x * inv, o.y * inv), pack_f16(o.z * inv, o.w * inv));
-        };
-        for (int e = tid; e < valid * D / 4; e += 128) {
-            const int row = e / (D / 4), col = e % (D / 4) * 4;
-            float m = s_top[row], l = 0.f;
-#pragma unroll
-            for (int w = 1; w < 4; w++) m = fmaxf(m, s_top[w * ROWS + row]);
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float f = share_weight(s_top[w * ROWS + row], m);
-                const float4 x = *reinterpret_cast<const float4*>(merge + (w * ROWS + row) * D + col);
-                l = fmaf(f, s_sum[w * ROWS + row], l);
-                o = make_float4(fmaf(f, x.x, o.x), fmaf(f, x.y, o.y), fmaf(f, x.z, o.z), fmaf(f, x.w, o.w));
-            }
-            if (whole) {
-                put(row, col, o, l);
-            } else {
-                *reinterpret_cast<float4*>(slot + row * D + col) = o;
-                if (col == 0) {
-                    slot[SLOT_ROWS * D + row] = m;
-                    slot[SLOT_ROWS * (D + 1) + row] = l;
-                }
-            }
+        if (!s_at[0]) return;
+        // each warp joins a run of the parts, then the warps as above
+        const int64_t second = begin_of(w0) != begin;  // the first CTA's may be its second piece of the line
+        const unsigned p0 = parts * warp / 4, p1 = parts * (warp + 1) / 4;
+        Share<D, NR> own;
+        own.clear();
+        for (unsigned p = p0; p < p1; p++) {
+            Share<D, NR> x;
+            x.get(partials + (static_cast<int64_t>(w0 + p) * 2 + (p == 0 ? second : 0)) * SLOT, lane);
+            own.join(x, c4);
         }
-        if (!whole) {
-            const unsigned w0 = worker_of(item_first), w1 = worker_of(item_first + units - 1);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) s_at[2] = atomicInc(&counters[w0], w1 - w0) == w1 - w0;  // back to zero with the last one
-            __syncthreads();
-            if (s_at[2]) {
-                __threadfence();
-                // the first one's may be its second piece of the line
-                const float* first = partials + (static_cast<int64_t>(w0) * 2 + (begin_of(w0) != item_first ? 1 : 0)) * SLOT;
-                auto part = [&](unsigned w) { return w == w0 ? first : partials + static_cast<int64_t>(w) * 2 * SLOT; };
-                // The maxima first, a thread to a row and a part; then each part's sums, eight of them on their way at a time.
-                const unsigned parts = w1 - w0 + 1;
-                for (int row = warp; row < valid; row += 4) {
-                    float m = -INFINITY;
-                    for (unsigned w = lane; w < parts; w += 32) m = fmaxf(m, __ldcg(part(w0 + w) + SLOT_ROWS * D + row));
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    float l = 0.f;
-                    for (unsigned w = lane; w < parts; w += 32) {
-                        const float f = share_weight(__ldcg(part(w0 + w) + SLOT_ROWS * D + row), m);
-                        merge[w * ROWS + row] = f;
-                        l = fmaf(f, __ldcg(part(w0 + w) + SLOT_ROWS * (D + 1) + row), l);
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-                    if (lane == 0) s_sum[row] = l;
-                }
-                __syncthreads();
-                for (int e = tid; e < valid * D / 4; e += 128) {
-                    const int row = e / (D / 4), col = e % (D / 4) * 4;
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (unsigned w = 0; w < parts; w += 8) {
-                        float4 x[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = __ldcg(reinterpret_cast<const float4*>(part(w0 + min(w + i, parts - 1)) + row * D + col));
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            if (w + i < parts) {
-                                const float f = merge[(w + i) * ROWS + row];
-                                o = make_float4(fmaf(f, x[i].x, o.x), fmaf(f, x[i].y, o.y), fmaf(f, x[i].z, o.z), fmaf(f, x[i].w, o.w));
-                            }
-                    }
-                    put(row, col, o, s_sum[row]);
-                }
-            }
+        // runs are joined from the front on: 1 to 0, 3 to 2, 2 to 0
+        if (warp & 1) own.put(s_hand + (warp >> 1) * SLOT, lane);
+        __syncthreads();
+        if (!(warp & 1)) own.join_shared(s_hand + (warp >> 1) * SLOT, lane, c4);
+        if (warp == 2) own.put(s_hand + SLOT, lane);
+        __syncthreads();
+        if (warp == 0) {
+            own.join_shared(s_hand + SLOT, lane, c4);
+            store(own, s.b, s.h, s.tile);
         }
-        __syncthreads();  // the ring and the flags are free again
-        unit += taken;
-        if (unit - seq_first == units * items && unit < hi) {
-            seq_first = unit;
-            b++;
-        }
-    }
+    };
+    Segment head;
+    head.b = share_b;
+    head.seq = share_seq;
+    head.unit = lo;
+    look(head);
+    const bool head_shared = head.taken != head.units, tail_shared = now.unit != lo && now.taken != now.units;
+    if (head_shared) finish(head);
+    if (tail_shared) finish(now);
 }
 
 }  // namespace paged
