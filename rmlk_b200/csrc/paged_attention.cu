@@ -117,9 +117,13 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
         if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
             return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
         const cudaStream_t st = as_stream(stream);
-        if (dtype == RMLK_F32) return c.d == 64 ? paged::launch_few<float, 64, 1>(st, c, s, a, workspace) : paged::launch_few<float, 128, 1>(st, c, s, a, workspace);
-        if (s.each * a.group <= 8) return c.d == 64 ? paged::launch_few<__half, 64, 1>(st, c, s, a, workspace) : paged::launch_few<__half, 128, 1>(st, c, s, a, workspace);
-        return c.d == 64 ? paged::launch_few<__half, 64, 2>(st, c, s, a, workspace) : paged::launch_few<__half, 128, 2>(st, c, s, a, workspace);
+        const bool one = s.each * a.group <= 8;
+        if (dtype == RMLK_F32) {
+            if (c.d == 64) return one ? paged::launch_few<float, 64, 1>(st, c, s, a, workspace) : paged::launch_few<float, 64, 2>(st, c, s, a, workspace);
+            return one ? paged::launch_few<float, 128, 1>(st, c, s, a, workspace) : paged::launch_few<float, 128, 2>(st, c, s, a, workspace);
+        }
+        if (c.d == 64) return one ? paged::launch_few<__half, 64, 1>(st, c, s, a, workspace) : paged::launch_few<__half, 64, 2>(st, c, s, a, workspace);
+        return one ? paged::launch_few<__half, 128, 1>(st, c, s, a, workspace) : paged::launch_few<__half, 128, 2>(st, c, s, a, workspace);
     }
     const int64_t ctas = ceil_div64(tokens * q_heads, 4);
     if (ctas > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");

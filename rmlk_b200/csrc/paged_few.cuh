@@ -1,8 +1,7 @@
 // Attention of a few query rows per KV head over the paged 8-bit cache: a step of decoding, or of a few drafted tokens.
 //
 // What bounds it: HBM, each code of the cache read once (a byte per value, against one multiply-add per query row).  So the work is laid out for
-// the memory system, and the products go to mma.sync on registers: a tcgen05 tile has 128 rows, of which a step would fill 4 or 8, and wants its operands in
-// shared memory as f16, which costs more than the products themselves.
+// the memory system, and the products go to mma.sync on registers: a tcgen05 tile has 128 rows, of which a step would fill 4 or 8.
 //
 // Shares.  The keys of all (sequence, KV head, row tile) problems lie behind one another in units of 4 x 32 keys, and the CTAs - as many as are resident
 // at once - take equal parts of that line, whatever the lengths of the sequences; the host does not know them.  A CTA's piece of a problem is a segment.  A warp
@@ -11,14 +10,16 @@
 // A problem that several CTAs share leaves partial results (sums, maximum, weights' sum) in the workspace; the CTA that comes last adds them up in their
 // order along the keys, so the result does not depend on which one that is.
 //
-// A warp's step: 32 keys.  Each lane copies by cp.async just the bytes that it will read itself; no lane waits for another.  The order of a contraction is
-// free, so a lane's 16 consecutive bytes of a key are its operands of four MMAs (four dims to each), and bytes become f16 in registers:
-// 0x6400 | (b ^ 0x80) is 1152 + b.
-//   scores  S[16 rows x 8 keys]     = Q K^T: fp32 queries as pairs of f16, the high parts in rows 0-7, the low parts (2^11 times their size) in rows 8-15; f16
-//                                     queries: 8 or 16 rows
-//   values  O^T[16 dims x 8 rows] += V^T P^T over 16 keys: the accumulator fragment of S is the operand fragment of P^T as it is; two tokens' bytes side by side are V^T's
-// Codes are exact in f16.  For fp32 results a step's O is formed from zero and added to fp32 sums, which keeps the MMA's truncating accumulator short; for f16 the
-// accumulators stay in the MMAs.  Weights are 2^14 exp2(s - max): as pairs for fp32, as f16 for f16 results (2^-11 of a weight, as much as the result's own rounding).
+// A warp's step: 4 KB of keys and of values.  Each lane copies by cp.async just the bytes that it will read itself; no lane waits for another.
+// Both contractions are products of 8-bit integers (mma.sync m16n8k32, exact 32-bit sums), so the codes are operands as they lie there.  (As f16, four
+// instructions went into each pair of codes: 530 per step of 4 KB, and the SMs, not HBM, were the bound: 5.0 TB/s.)
+//   scores  S[16 rows x 8 keys] = Q K^T.  Queries are fixed-point numbers under a power of two per row: 15 bits and sign for f16, 22 for fp32 - half a
+//           step is 2^-15 or 2^-23 of the row's largest value - as two or three signed digits of 8 bits, a row of the MMA each.
+//   values  O^T[16 dims x 8 rows] = V^T P^T.  Weights exp2(s - m), m the row's largest score in the step, are fixed-point numbers of 16 bits (f16 results) or 23
+//           (fp32): half a step is 2^-17 or 2^-24 of the largest weight of the step.  Unsigned digits, an MMA each; the accumulator fragment of S holds just the
+//           weights that the operand fragment wants, four tokens' bytes to a register, and a 4 x 4 transpose of bytes puts four tokens' codes side by side.
+// A step's sums, joined from the digits, times exp2(m - running maximum) and the page's scale are added to fp32 sums.  The order of a contraction is free, so a
+// lane's 16 consecutive bytes of a key are its operands of two MMAs.
 #pragma once
 
 #include "paged.cuh"
@@ -40,19 +41,20 @@ constexpr int COUNTERS = 4096;  // arrival counters at the head of a workspace; 
 
 template <typename T, int D, int NR_>
 struct Few {
-    static constexpr bool PAIRS = sizeof(T) == 4;
+    static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int NR = NR_;               // groups of 8 query rows in a tile
     static constexpr int ROWS = 8 * NR;
-    static constexpr int KS = 32, NC = KS / 16;  // keys of a warp's step; groups of 16 of them: one page each
+    static constexpr int KS = 4096 / D, NC = KS / 16;  // keys of a warp's step; groups of 16 of them: one page each
     static constexpr int UNIT = 4 * KS;
-    static constexpr int STAGES = D == 64 ? 3 : 2;
+    static constexpr int STAGES = 2;
     static constexpr int K_BYTES = KS * D, STEP = 2 * K_BYTES;
+    static constexpr int QT = F32 ? NR + 1 : NR;  // row tiles of the scores' MMAs: (high, low digit) of each group, and the third digits of both
+    static constexpr int DIGITS = F32 ? 3 : 2;
     static constexpr int RING = 4 * STAGES * STEP;
     static constexpr int FRAGS = D / 16 * NR;    // groups of four sums per lane
     static constexpr int HAND = 32 * (FRAGS * 16 + NR * 8);  // a warp's share on its way to another: sums, maxima, weights' sums
     static constexpr int SCALES = RING + 2 * HAND, SCAN = SCALES + 4 * STAGES * NC * 8, SMEM = SCAN + 64;
-    static constexpr int PER_SM = NR == 2 && D == 128 ? 2 : 3;
-    static_assert(!PAIRS || NR == 1, "the low parts take rows 8-15");
+    static constexpr int PER_SM = NR == 2 ? 2 : 3;
 };
 constexpr int MOST_PARTS = 32;  // CTAs for a problem, on average: each costs the last one a fraction of a microsecond
 inline size_t few_workspace(int64_t d) { return COUNTERS * 4 + static_cast<size_t>(sm_count()) * 4 * 2 * (32 * (d / 16 * 2 * 16 + 2 * 8)); }
@@ -62,9 +64,15 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+// signed x signed (queries and keys), signed x unsigned (values and weights)
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <int BYTES>
@@ -72,12 +80,10 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-// two bytes (of four that have 0x80 flipped) as f16: 1024 + u - 1152
-__device__ __forceinline__ uint32_t two_f16(uint32_t flipped, uint32_t selector) {
-    const uint32_t biased = __byte_perm(flipped, 0x64646464u, selector);
-    const uint32_t offset = 0x64806480u;
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), *reinterpret_cast<const __half2*>(&offset));
-    return *reinterpret_cast<const uint32_t*>(&v);
+// byte B of four words, in order
+template <int B>
+__device__ __forceinline__ uint32_t bytes_of(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+    return __byte_perm(__byte_perm(w0, w1, B | (B + 4) << 4), __byte_perm(w2, w3, B | (B + 4) << 4), 0x5410);
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
 #pragma unroll
                 for (int i = 0; i < D / 16; i += 2) {
                     const float4 o = make_float4(x.acc[i][r][e] * inv, x.acc[i][r][2 + e] * inv, x.acc[i + 1][r][e] * inv, x.acc[i + 1][r][2 + e] * inv);
-                    if constexpr (L::PAIRS) *reinterpret_cast<float4*>(dst + 2 * i) = o;
+                    if constexpr (L::F32) *reinterpret_cast<float4*>(dst + 2 * i) = o;
                     else *reinterpret_cast<uint2*>(dst + 2 * i) = make_uint2(pack_f16(o.x, o.y), pack_f16(o.z, o.w));
                 }
             }
@@ -372,9 +378,8 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
 
         // ---- queries: fragments of the scores' MMAs, and what each lane's rows see.  (Asked for first, looked at when the first keys are on their way.) ----
         auto relative = [&](int64_t key) { return static_cast<int>(max(min(key - first_key, int64_t(0x7fffff00)), int64_t(0))); };
-        constexpr int QF = L::PAIRS ? 4 : 2 * NR;  // registers of a fragment: rows g (high, low), or g and g + 8
-        uint32_t qf[4 * PIECES][QF];
-        float4 qx[L::PAIRS ? 4 * PIECES : 1];
+        using Four = typename std::conditional<L::F32, float4, uint2>::type;  // four values
+        Four qx[NR][4 * PIECES];
         float factor[NR];
         int sees[NR];  // keys from the warp's first on that the lane's rows see
 #pragma unroll
@@ -382,38 +387,64 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             const int row = tile * ROWS + g + 8 * r, token = row / a.group;
             const bool in = row < rows;
             sees[r] = in ? relative(min(before + token + 1, keys)) : 0;
-            factor[r] = a.scale * 1.44269504f;
             const T* src = static_cast<const T*>(a.q) + (static_cast<int64_t>(b) * q.each + token) * a.qs + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D + 16 * c4;
 #pragma unroll
             for (int s = 0; s < 4 * PIECES; s++) {
-                const T* at = src + (s >> 2) * 64 + (s & 3) * 4;
-                if constexpr (L::PAIRS) {
-                    qx[s] = in ? *reinterpret_cast<const float4*>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
-                } else {
-                    const uint2 x = in ? *reinterpret_cast<const uint2*>(at) : make_uint2(0u, 0u);
-                    qf[s][r] = x.x;
-                    qf[s][NR + r] = x.y;
-                }
+                Four x = {};
+                if (in) x = *reinterpret_cast<const Four*>(src + (s >> 2) * 64 + (s & 3) * 4);
+                qx[r][s] = x;
             }
         }
         if (first) {
 #pragma unroll
             for (int s = 0; s < L::STAGES - 1; s++) issue();
         }
-        if constexpr (L::PAIRS) {
+        // digits: [32 dims][row tile]: rows g and g + 8 of the lane's first four dims, then of the next four
+        uint32_t qf[2 * PIECES][L::QT][4];
+        if constexpr (L::F32 && NR == 1) {
+#pragma unroll
+            for (int s = 0; s < 2 * PIECES; s++) qf[s][NR][1] = qf[s][NR][3] = 0;  // no second group
+        }
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            auto four = [&](int s) {
+                if constexpr (L::F32) {
+                    return qx[r][s];
+                } else {
+                    const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&qx[r][s].x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&qx[r][s].y));
+                    return make_float4(lo.x, lo.y, hi.x, hi.y);
+                }
+            };
             uint32_t most = 0;
 #pragma unroll
-            for (int s = 0; s < 4 * PIECES; s++)
-                most = max(max(most, max(finite_abs_bits(qx[s].x), finite_abs_bits(qx[s].y))), max(finite_abs_bits(qx[s].z), finite_abs_bits(qx[s].w)));
+            for (int s = 0; s < 4 * PIECES; s++) {
+                const float4 x = four(s);
+                most = max(max(most, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu)), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
+            }
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int e = scale_exponent(most);
-            const float up = exp2_int(e);
-            factor[0] *= exp2_int(-e);
+            // 2^e: the largest in [2^14, 2^15) - times 2^8 for three digits - but not above what signed digits hold, 127 127 (127)
+            int e = scale_exponent(most < 0x7f800000u ? most : 0u);
+            if (__uint_as_float(most) * exp2_int(e) > (L::F32 ? 32639.49f : 32639.f)) e--;
+            const float up = exp2_int(e), more = L::F32 ? 256.f : 1.f;
+            // an infinity or a NaN makes NaN of the row
+            factor[r] = most < 0x7f800000u ? a.scale * 1.44269504f / more * exp2_int(-e) : __int_as_float(0x7fc00000);
 #pragma unroll
             for (int s = 0; s < 4 * PIECES; s++) {
-                split2(qx[s].x * up, qx[s].y * up, qf[s][0], qf[s][1]);
-                split2(qx[s].z * up, qx[s].w * up, qf[s][2], qf[s][3]);
+                const float4 x = four(s);
+                const int v[4] = {__float2int_rn(x.x * up * more), __float2int_rn(x.y * up * more), __float2int_rn(x.z * up * more), __float2int_rn(x.w * up * more)};
+                // signed digits: the byte of v + 0x80 (+ 0x8000) carries what the digits below borrow
+                const uint32_t d0 = bytes_of<0>(v[0], v[1], v[2], v[3]), d1 = bytes_of<1>(v[0] + 0x80, v[1] + 0x80, v[2] + 0x80, v[3] + 0x80);
+                uint32_t(&f)[L::QT][4] = qf[s >> 1];
+                const int at = 2 * (s & 1);
+                if constexpr (L::F32) {
+                    f[r][at] = bytes_of<2>(v[0] + 0x8080, v[1] + 0x8080, v[2] + 0x8080, v[3] + 0x8080);
+                    f[r][at + 1] = d1;
+                    f[NR][at + r] = d0;
+                } else {
+                    f[r][at] = d1;
+                    f[r][at + 1] = d0;
+                }
             }
         }
         const int all_see = relative(min(before + 1 + (tile * ROWS) / a.group, keys));  // that every row of the tile sees
@@ -423,7 +454,6 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
         float(&acc)[D / 16][NR][4] = own.acc;
         float(&top)[NR] = own.top;
         float(&sum)[NR] = own.sum;
-        float v_ref = 0.f, v_inv = 0.f, v_top = 0.f;  // the scale of V that the weights are relative to, its reciprocal, the largest so far
         for (int step = 0; step < now.steps; step++, stage = stage + 1 == L::STAGES ? 0 : stage + 1) {
             __syncwarp();  // the slot that is filled next has been read, its scales too
             issue();
@@ -431,48 +461,40 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             __syncwarp();  // (scales come from other lanes)
             const uint8_t* at = ring_ptr + stage * L::STEP;
             // ---- scores ----
-            float s[KS / 8][4];
-#pragma unroll
-            for (int j = 0; j < KS / 8; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-#pragma unroll
-            for (int i = 0; i < PIECES; i++) {
-#pragma unroll
-                for (int j = 0; j < KS / 8; j++) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(at + (j * PIECES + i) * 512 + lane * 16);
-                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t f = word[k] ^ 0x80808080u;
-                        const uint32_t(&qa)[QF] = qf[4 * i + k];
-                        mma_16816(s[j], qa[0], QF == 4 ? qa[1] : 0u, QF == 4 ? qa[2] : qa[1], QF == 4 ? qa[3] : 0u, two_f16(f, 0x4140), two_f16(f, 0x4342));
-                    }
-                }
-            }
             float x[NR][KS / 8][2];
-            float most[NR];
-#pragma unroll
-            for (int r = 0; r < NR; r++) most[r] = top[r];
 #pragma unroll
             for (int j = 0; j < KS / 8; j++) {
-                const float ks = scales[stage * NC + j / 2].x;
-                if constexpr (L::PAIRS) {
-                    const float t = factor[0] * ks;
-                    x[0][j][0] = fmaf(s[j][2], 1.f / SPLIT_LO, s[j][0]) * t;
-                    x[0][j][1] = fmaf(s[j][3], 1.f / SPLIT_LO, s[j][1]) * t;
-                } else {
+                int s[L::QT][4] = {};
 #pragma unroll
-                    for (int r = 0; r < NR; r++) {
-                        const float t = factor[r] * ks;
-                        x[r][j][0] = s[j][2 * r] * t;
-                        x[r][j][1] = s[j][2 * r + 1] * t;
+                for (int i = 0; i < PIECES; i++) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(at + (j * PIECES + i) * 512 + lane * 16);
+#pragma unroll
+                    for (int t = 0; t < L::QT; t++) {
+                        mma_s8(s[t], qf[2 * i][t][0], qf[2 * i][t][1], qf[2 * i][t][2], qf[2 * i][t][3], w.x, w.y);
+                        mma_s8(s[t], qf[2 * i + 1][t][0], qf[2 * i + 1][t][1], qf[2 * i + 1][t][2], qf[2 * i + 1][t][3], w.z, w.w);
+                    }
+                }
+                const float ks = scales[stage * NC + j / 2].x;
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    const float t = factor[r] * ks;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float high = static_cast<float>(s[r][e] * 256 + s[r][2 + e]);
+                        x[r][j][e] = (L::F32 ? fmaf(high, 256.f, static_cast<float>(s[L::QT - 1][2 * r + e])) : high) * t;
                     }
                 }
             }
-            float vs[NR][NC];  // scales of V as the lane's rows see them
+            // scales of V: the largest, and whether the others are of its size
+            float v_top = 0.f, v_low = INFINITY;
+            bool broken = false;
 #pragma unroll
-            for (int n = 0; n < NC; n++)
-#pragma unroll
-                for (int r = 0; r < NR; r++) vs[r][n] = scales[stage * NC + n].y;
+            for (int n = 0; n < NC; n++) {
+                const float v = scales[stage * NC + n].y;
+                broken = broken || !(v < INFINITY);
+                v_top = fmaxf(v_top, v);
+                if (v > 0.f) v_low = fminf(v_low, v);
+            }
             if (KS + step * L::UNIT > all_see) {
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
@@ -482,135 +504,130 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                         if (8 * j + 2 * c4 >= see) x[r][j][0] = -INFINITY;
                         if (8 * j + 2 * c4 + 1 >= see) x[r][j][1] = -INFINITY;
                     }
-#pragma unroll
-                    for (int n = 0; n < NC; n++)
-                        if (16 * n >= see) vs[r][n] = 0.f;  // (a NaN there is no part of the row)
                 }
             }
+            if (broken) {  // rows that see such a page become NaN
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+                        if (!(scales[stage * NC + n].y < INFINITY) && 16 * n < sees[r] - step * L::UNIT) sum[r] = __int_as_float(0x7fc00000);
+            }
+            float weight[NR];  // of the step's sums: exp2(largest score of the step - running maximum)
             bool more = false;
+            float most[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) {
+                float m = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < KS / 8; j++) most[r] = fmaxf(most[r], fmaxf(x[r][j][0], x[r][j][1]));
-                most[r] = quad_max(most[r]);
+                for (int j = 0; j < KS / 8; j++) m = fmaxf(m, fmaxf(x[r][j][0], x[r][j][1]));
+                most[r] = quad_max(m);
                 more = more || most[r] > top[r];
             }
             if (__any_sync(0xffffffffu, more)) {
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
-                    const float corr = top[r] == -INFINITY ? 0.f : ex2(top[r] - most[r]);
-                    top[r] = most[r];
+                    const float m = fmaxf(top[r], most[r]), corr = top[r] == -INFINITY ? 0.f : ex2(top[r] - m);
+                    top[r] = m;
                     sum[r] *= corr;
                     own.scale(r, corr, c4);
                 }
             }
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                const float shift = (top[r] == -INFINITY ? 0.f : top[r]) - 14.f;
+                const float shift = most[r] == -INFINITY ? 0.f : most[r];
+                weight[r] = most[r] == -INFINITY ? 0.f : ex2(most[r] - top[r]);
+                float part = 0.f;
 #pragma unroll
                 for (int j = 0; j < KS / 8; j++) {
                     x[r][j][0] = ex2(x[r][j][0] - shift);
                     x[r][j][1] = ex2(x[r][j][1] - shift);
-                    sum[r] += x[r][j][0] + x[r][j][1];
+                    part += x[r][j][0] + x[r][j][1];
                 }
+                sum[r] = fmaf(part, weight[r], sum[r]);
             }
             // ---- values ----
-            // Scales of V go into the weights, relative to the one that the accumulators are in: that of the 16 keys before, as long as the ratio is
-            // between 2 (weights stay in f16's range) and 2^-12.  (Infinities and NaN go into the weights as they are.)
-            float fresh[L::PAIRS ? D / 16 : 1][4];
+            // Scales of V go into the weights, relative to the step's largest.  Where they differ by more than 2^3 a page at a time is taken, under its own.
+            const bool even = v_low * 8.f >= v_top;
+            constexpr float MOST = L::F32 ? 8388607.f : 65535.f;
+            const int passes = NC == 1 || even ? 1 : NC;
+#pragma unroll 1
+            for (int pass = 0; pass < passes; pass++) {
+                const float ref = passes == 1 ? v_top : scales[stage * NC + pass].y;
+                if (!(ref > 0.f && ref < INFINITY)) continue;  // nothing but zeros (or NaN, seen to above)
+                const float per = MOST / ref;
+                uint32_t p[NR][NC][L::DIGITS];
 #pragma unroll
-            for (int n = 0; n < NC; n++) {
-                const float scale = scales[stage * NC + n].y, ref = scale < INFINITY ? fmaxf(scale, 1.17549435e-38f) : 1.f;
-                if constexpr (L::PAIRS) {
-                    const bool other = n > 0 && (ref > 2.f * v_ref || ref < v_ref * 2.44140625e-4f);
-                    if (other) {
+                for (int n = 0; n < NC; n++) {
+                    const float v = scales[stage * NC + n].y, k = passes > 1 ? (n == pass ? MOST : 0.f) : v == ref ? MOST : v * per;
 #pragma unroll
-                        for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) acc[i][0][e] = fmaf(fresh[i][e], v_ref, acc[i][0][e]);
+                    for (int r = 0; r < NR; r++) {
+                        // the lower bits of 2^23 + a number below 2^23 are that number
+                        const uint32_t w0 = __float_as_uint(fmaf(x[r][2 * n][0], k, 8388608.f)), w1 = __float_as_uint(fmaf(x[r][2 * n][1], k, 8388608.f));
+                        const uint32_t w2 = __float_as_uint(fmaf(x[r][2 * n + 1][0], k, 8388608.f)), w3 = __float_as_uint(fmaf(x[r][2 * n + 1][1], k, 8388608.f));
+                        const uint32_t t01 = __byte_perm(w0, w1, 0x5140), t23 = __byte_perm(w2, w3, 0x5140);
+                        p[r][n][0] = __byte_perm(t01, t23, 0x5410);
+                        p[r][n][1] = __byte_perm(t01, t23, 0x7632);
+                        if constexpr (L::F32) p[r][n][2] = bytes_of<2>(w0, w1, w2, w3);
                     }
-                    if (n == 0 || other) {
-#pragma unroll
-                        for (int i = 0; i < D / 16; i++) fresh[i][0] = fresh[i][1] = fresh[i][2] = fresh[i][3] = 0.f;
-                        v_ref = ref;
-                        v_inv = 1.f / ref;
-                    }
-                } else if (scale < INFINITY && (ref > 2.f * v_ref || (ref < v_ref * 2.44140625e-4f && ref > v_top * 5.42101086e-20f))) {  // (2^-64: further down sums might leave fp32's range)
-                    const float f = v_ref / ref;
-#pragma unroll
-                    for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                        for (int r = 0; r < 4 * NR; r++) acc[i][r >> 2][r & 3] *= f;
-                    v_ref = ref;
-                    v_inv = 1.f / ref;
-                    v_top = fmaxf(v_top, ref);
                 }
-                uint32_t p[2][2];  // rows 0-7 and 8-15, or the high and low parts: tokens 2 c4, 2 c4 + 1 and 8 further on
+                float2 f[NR];
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if constexpr (L::PAIRS) {
-                        const float w = vs[0][n] * v_inv, y0 = x[0][2 * n + e][0] * w, y1 = x[0][2 * n + e][1] * w;
-                        const __half2 high = __floats2half2_rn(y0, y1);
-                        const float2 back = __half22float2(high);
-                        p[0][e] = *reinterpret_cast<const uint32_t*>(&high);
-                        p[1][e] = pack_f16(y0 - back.x, y1 - back.y);
-                    } else {
+                for (int r = 0; r < NR; r++) f[r] = Share<D, NR>::of_sums(weight[r] * (ref * (1.f / MOST)), c4);
+                uint32_t v[NC][4][D / 32];
+#pragma unroll
+                for (int n = 0; n < NC; n++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        const uint8_t* src = at + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8);
+                        if constexpr (D == 64) {
+                            const uint2 w = *reinterpret_cast<const uint2*>(src);
+                            v[n][t][0] = w.x;
+                            v[n][t][1] = w.y;
+                        } else {
+                            const uint4 w = *reinterpret_cast<const uint4*>(src);
+                            v[n][t][0] = w.x;
+                            v[n][t][1] = w.y;
+                            v[n][t][2] = w.z;
+                            v[n][t][3] = w.w;
+                        }
+                    }
+#pragma unroll
+                for (int w = 0; w < D / 32; w++) {
+                    uint32_t tr[NC][4];  // four tokens of each of the word's four dims
+#pragma unroll
+                    for (int n = 0; n < NC; n++) {
+                        const uint32_t a01 = __byte_perm(v[n][0][w], v[n][1][w], 0x5140), a23 = __byte_perm(v[n][2][w], v[n][3][w], 0x5140);
+                        const uint32_t b01 = __byte_perm(v[n][0][w], v[n][1][w], 0x7362), b23 = __byte_perm(v[n][2][w], v[n][3][w], 0x7362);
+                        tr[n][0] = __byte_perm(a01, a23, 0x5410);
+                        tr[n][1] = __byte_perm(a01, a23, 0x7632);
+                        tr[n][2] = __byte_perm(b01, b23, 0x5410);
+                        tr[n][3] = __byte_perm(b01, b23, 0x7632);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
 #pragma unroll
                         for (int r = 0; r < NR; r++) {
-                            const float w = vs[r][n] * v_inv;
-                            p[r][e] = pack_f16(x[r][2 * n + e][0] * w, x[r][2 * n + e][1] * w);
+                            int o[L::DIGITS][4] = {};
+#pragma unroll
+                            for (int n = 0; n < NC; n += 2)
+#pragma unroll
+                                for (int t = 0; t < L::DIGITS; t++) mma_u8(o[t], tr[n][2 * k], tr[n][2 * k + 1], tr[n + 1][2 * k], tr[n + 1][2 * k + 1], p[r][n][t], p[r][n + 1][t]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float value = L::F32 ? fmaf(static_cast<float>(o[L::DIGITS - 1][e] * 256 + o[1][e]), 256.f, static_cast<float>(o[0][e]))
+                                                           : static_cast<float>(o[1][e] * 256 + o[0][e]);
+                                acc[2 * w + k][r][e] = fmaf(value, e & 1 ? f[r].y : f[r].x, acc[2 * w + k][r][e]);
+                            }
                         }
                     }
                 }
-                uint32_t v[4][D / 32];
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const uint8_t* src = at + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8);
-                    if constexpr (D == 64) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(src);
-                        v[t][0] = w.x ^ 0x80808080u;
-                        v[t][1] = w.y ^ 0x80808080u;
-                    } else {
-                        const uint4 w = *reinterpret_cast<const uint4*>(src);
-                        v[t][0] = w.x ^ 0x80808080u;
-                        v[t][1] = w.y ^ 0x80808080u;
-                        v[t][2] = w.z ^ 0x80808080u;
-                        v[t][3] = w.w ^ 0x80808080u;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    // two tokens side by side, of dims 2 i and 2 i + 1 of the lane's
-                    const uint32_t near = __byte_perm(v[0][i / 2], v[1][i / 2], i & 1 ? 0x7362 : 0x5140), far = __byte_perm(v[2][i / 2], v[3][i / 2], i & 1 ? 0x7362 : 0x5140);
-                    const uint32_t a0 = two_f16(near, 0x4140), a1 = two_f16(near, 0x4342), a2 = two_f16(far, 0x4140), a3 = two_f16(far, 0x4342);
-                    if constexpr (L::PAIRS) {
-                        mma_16816(fresh[i], a0, a1, a2, a3, p[1][0], p[1][1]);
-                        mma_16816(fresh[i], a0, a1, a2, a3, p[0][0], p[0][1]);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < NR; r++) mma_16816(acc[i][r], a0, a1, a2, a3, p[r][0], p[r][1]);
-                    }
-                }
-            }
-            if constexpr (L::PAIRS) {
-#pragma unroll
-                for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][0][e] = fmaf(fresh[i][e], v_ref, acc[i][0][e]);
             }
         }
 
         // ---- the four warps' shares: 2 to 0, 3 to 1, 1 to 0 ----
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            sum[r] = quad_sum(sum[r]);
-            if constexpr (!L::PAIRS) {
-#pragma unroll
-                for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[i][r][e] *= v_ref;
-            }
-        }
+        for (int r = 0; r < NR; r++) sum[r] = quad_sum(sum[r]);
         if (warp >= 2) {
             if (handed) {
                 if (warp == 2) pair_wait<FREE_0>();
