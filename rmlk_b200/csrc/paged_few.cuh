@@ -10,7 +10,7 @@
 // A problem that several CTAs share leaves partial results (sums, maximum, weights' sum) in the workspace; the CTA that comes last adds them up in their
 // order along the keys, so the result does not depend on which one that is.
 //
-// A warp's step: 4 KB of keys and of values.  Each lane copies by cp.async just the bytes that it will read itself; no lane waits for another.
+// A warp's step: 4 KB of keys and of values, copied by its own lanes with cp.async: no warp waits for another.
 // Both contractions are products of 8-bit integers (mma.sync m16n8k32, exact 32-bit sums), so the codes are operands as they lie there.  (As f16, four
 // instructions went into each pair of codes: 530 per step of 4 KB, and the SMs, not HBM, were the bound: 5.0 TB/s.)
 //   scores  S[16 rows x 8 keys] = Q K^T.  Queries are fixed-point numbers under a power of two per row: 15 bits and sign for f16, 22 for fp32 - half a
@@ -19,7 +19,7 @@
 //           (fp32): half a step is 2^-17 or 2^-24 of the largest weight of the step.  Unsigned digits, an MMA each; the accumulator fragment of S holds just the
 //           weights that the operand fragment wants, four tokens' bytes to a register, and a 4 x 4 transpose of bytes puts four tokens' codes side by side.
 // A step's sums, joined from the digits, times exp2(m - running maximum) and the page's scale are added to fp32 sums.  The order of a contraction is free, so a
-// lane's 16 consecutive bytes of a key are its operands of two MMAs.
+// 16 consecutive bytes of a key are a lane's operands of two MMAs.
 #pragma once
 
 #include "paged.cuh"
@@ -79,6 +79,14 @@ template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+// Where 16-byte unit u of key r (of 16) lies in shared memory.  A warp copies 512 consecutive bytes at a time - half-filled lines in flight cost a quarter of the
+// bandwidth - and reads units of keys r .. r + 7 (keys), or the same units of every other key (values): the units of a 128-byte line are exchanged so that
+// neither meets bank conflicts.
+template <int D>
+__device__ __forceinline__ int unit_at(int r, int u) {
+    if constexpr (D == 64) return (r >> 1) * 128 + ((((r & 1) * 4 + u) ^ (r & 6)) << 4);
+    return r * 128 + ((u ^ (r & 6) ^ (r & 1) * 4) << 4);
 }
 // byte B of four words, in order
 template <int B>
@@ -302,8 +310,6 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
     Segment now = ask;
     int block = -1;  // page and head as one index; -1: no key there, -2: a key without a page
     constexpr int PAGED_STEPS = 32 / NC;  // pages of so many steps are looked up at a time, one per lane
-    const int8_t* k_lane = c.k + g * D + c4 * 16;
-    const int8_t* v_lane = c.v + 2 * c4 * D + g * (D / 8);
     const int block_bytes = c.page * D;
     int fill = 0, fill_stage = 0;  // next step to be asked for, its place in the ring
     auto issue = [&]() {
@@ -334,14 +340,12 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                     else *to = at == -1 ? 0.f : __int_as_float(0x7fc00000);
                 }
                 const int64_t off = static_cast<int64_t>(from) * block_bytes + ((static_cast<int>(ask.first_key & 127) + fill * L::UNIT + 16 * n) & (c.page - 1)) * D;
-                const int8_t* ks = k_lane + off;
 #pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int i = 0; i < PIECES; i++) copy_async<16>(dst + ((2 * n + j) * PIECES + i) * 512 + lane * 16, ks + j * 8 * D + i * 64);
-                const int8_t* vs = v_lane + off;
-#pragma unroll
-                for (int t = 0; t < 4; t++) copy_async<D / 8>(dst + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8), vs + ((t & 1) + (t >> 1) * 8) * D);
+                for (int j = 0; j < D / 32; j++) {
+                    const uint32_t to = dst + n * (16 * D) + unit_at<D>((512 / D) * j + lane / (D / 16), lane % (D / 16));
+                    copy_async<16>(to, c.k + off + j * 512 + lane * 16);
+                    copy_async<16>(to + L::K_BYTES, c.v + off + j * 512 + lane * 16);
+                }
             }
             fill++;
             if (++fill_stage == L::STAGES) fill_stage = 0;
@@ -458,7 +462,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             __syncwarp();  // the slot that is filled next has been read, its scales too
             issue();
             asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 1) : "memory");
-            __syncwarp();  // (scales come from other lanes)
+            __syncwarp();  // (of all lanes)
             const uint8_t* at = ring_ptr + stage * L::STEP;
             // ---- scores ----
             float x[NR][KS / 8][2];
@@ -467,7 +471,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                 int s[L::QT][4] = {};
 #pragma unroll
                 for (int i = 0; i < PIECES; i++) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(at + (j * PIECES + i) * 512 + lane * 16);
+                    const uint4 w = *reinterpret_cast<const uint4*>(at + j / 2 * (16 * D) + unit_at<D>(8 * (j & 1) + g, 4 * i + c4));
 #pragma unroll
                     for (int t = 0; t < L::QT; t++) {
                         mma_s8(s[t], qf[2 * i][t][0], qf[2 * i][t][1], qf[2 * i][t][2], qf[2 * i][t][3], w.x, w.y);
@@ -579,7 +583,8 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                 for (int n = 0; n < NC; n++)
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
-                        const uint8_t* src = at + L::K_BYTES + (4 * n + t) * (4 * D) + lane * (D / 8);
+                        const int token = 2 * c4 + (t & 1) + (t >> 1) * 8;
+                        const uint8_t* src = at + L::K_BYTES + n * (16 * D) + unit_at<D>(token, D == 64 ? g / 2 : g) + (D == 64 ? (g & 1) * 8 : 0);
                         if constexpr (D == 64) {
                             const uint2 w = *reinterpret_cast<const uint2*>(src);
                             v[n][t][0] = w.x;
