@@ -372,6 +372,20 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             }
         }
     };
+    // the CTAs that share a segment's problem, from `first` on; whether the first one's is its second piece of the line
+    struct Parts {
+        unsigned first, count;
+        int second;
+    };
+    auto parts_of = [&](const Segment& s) {
+        const int64_t begin = s.seq + divide(s.unit - s.seq, s.units) * s.units;
+        Parts p;
+        p.first = worker_of(begin);
+        p.count = worker_of(begin + s.units - 1) - p.first + 1;
+        p.second = begin_of(p.first) != begin;
+        return p;
+    };
+    bool last_first = false, last_second = false;  // (warp 0) this CTA was the last one to finish the problem of its first, its last segment
     int stage = 0;
     bool first = true, handed = false;  // first segment of the CTA; the hand-over places have been used
 
@@ -653,8 +667,19 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             pair_wait<HAND_UP>();
             own.join_shared(s_hand + SLOT, lane, c4);
             pair_arrive<FREE_1>();
-            if (now.taken == now.units) store(own, b, h, tile);
-            else own.put(partials + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * SLOT, lane);
+            if (now.taken == now.units) {
+                store(own, b, h, tile);
+            } else {
+                own.put(partials + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * SLOT, lane);
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) {
+                    const Parts p = parts_of(now);
+                    const bool last = atomicInc(&counters[p.first], p.count - 1) == p.count - 1;  // back to zero with the last one
+                    if (first) last_first = last;
+                    else last_second = last;
+                }
+            }
         }
         handed = true;
         first = false;
@@ -666,27 +691,27 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
     if (warp == 3) pair_wait<FREE_1>();
 
     // ---- problems that are shared with other CTAs: at most the share's first and last ----
-    // first: begun before the share; last: goes on behind it (one and the same, where the share lies within a problem)
+    if (warp == 0 && lane == 0) {
+        s_at[0] = last_first;
+        s_at[1] = last_second;
+    }
+    __syncthreads();
     auto finish = [&](const Segment& s) {
-        const int64_t begin = s.seq + divide(s.unit - s.seq, s.units) * s.units;
-        const unsigned w0 = worker_of(begin), w1 = worker_of(begin + s.units - 1), parts = w1 - w0 + 1;
-        __syncthreads();
-        if (tid == 0) {
-            __threadfence();
-            s_at[0] = atomicInc(&counters[w0], w1 - w0) == w1 - w0;  // back to zero with the last one
-            __threadfence();
-        }
-        __syncthreads();
-        if (!s_at[0]) return;
         // each warp joins a run of the parts, then the warps as above
-        const int64_t second = begin_of(w0) != begin;  // the first CTA's may be its second piece of the line
-        const unsigned p0 = parts * warp / 4, p1 = parts * (warp + 1) / 4;
+        const Parts p = parts_of(s);
+        const unsigned p0 = p.count * warp / 4, p1 = p.count * (warp + 1) / 4;
+        auto part = [&](unsigned i) { return partials + (static_cast<int64_t>(p.first + i) * 2 + (i == 0 ? p.second : 0)) * SLOT; };
+        constexpr int AHEAD = D / 16 * NR <= 8 ? 3 : 1;  // parts on their way at a time
         Share<D, NR> own;
         own.clear();
-        for (unsigned p = p0; p < p1; p++) {
-            Share<D, NR> x;
-            x.get(partials + (static_cast<int64_t>(w0 + p) * 2 + (p == 0 ? second : 0)) * SLOT, lane);
-            own.join(x, c4);
+        for (unsigned i = p0; i < p1; i += AHEAD) {
+            Share<D, NR> x[AHEAD];
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++)
+                if (i + e < p1) x[e].get(part(i + e), lane);
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++)
+                if (i + e < p1) own.join(x[e], c4);
         }
         // runs are joined from the front on: 1 to 0, 3 to 2, 2 to 0
         if (warp & 1) own.put(s_hand + (warp >> 1) * SLOT, lane);
@@ -699,14 +724,19 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             store(own, s.b, s.h, s.tile);
         }
     };
-    Segment head;
-    head.b = share_b;
-    head.seq = share_seq;
-    head.unit = lo;
-    look(head);
-    const bool head_shared = head.taken != head.units, tail_shared = now.unit != lo && now.taken != now.units;
-    if (head_shared) finish(head);
-    if (tail_shared) finish(now);
+    if (s_at[0] | s_at[1]) {
+        __threadfence();
+        if (s_at[0]) {
+            Segment head;
+            head.b = share_b;
+            head.seq = share_seq;
+            head.unit = lo;
+            look(head);
+            finish(head);
+        }
+        __syncthreads();
+        if (s_at[1]) finish(now);
+    }
 }
 
 }  // namespace paged
