@@ -182,7 +182,9 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     const int64_t row0 = static_cast<int64_t>(item) * ROWS;
     const int64_t table_keys = q.width << c.page_log;
     const int64_t len = q.lens[b], keys = min(len, table_keys + 1), before = len - count;
-    auto sees_of = [&](int64_t row) { return min(before + row / a.group + 1, keys); };  // row: of the sequence and head, from its first new token on
+    // rows of the sequence and head are counted from its first new token on (fewer than 2^31: tokens x 64)
+    auto token_of = [&](int64_t row) { return ((row | a.group) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(row) / static_cast<uint32_t>(a.group)) : row / a.group; };
+    auto sees_of = [&](int64_t row) { return min(before + token_of(row) + 1, keys); };
     const int64_t seen = max(sees_of(row0 + rows - 1), int64_t(0));                     // keys that the last row sees
 
     // ---- the pages that they see: all there, scales finite and not below zero, those of V of one size? ----
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     if (!plain || !(v_low * 1024.f >= v_top) || seen == 0) {
         for (int r = warp; r < rows; r += L::THREADS / 32) {
             const int64_t row = row0 + r;
-            const int64_t token = row / a.group;
+            const int64_t token = token_of(row);
             row_in_fp32<T, D>(c, q, a, b, first + token, h * a.group + static_cast<int>(row - token * a.group), sees_of(row));
         }
         return;
@@ -255,39 +257,44 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     // ---- queries ----
     if (warp < 4 * TILES) {
         const int t = warp >> 2;
-        constexpr int PER = D / 4, AT_ONCE = 32 / PER;  // lanes to a row (four values each), rows of a warp at a time
+        constexpr int PER = D / 4, AT_ONCE = 32 / PER, BATCH = 8;  // lanes to a row (four values each), rows of a warp at a time, loads on their way
+        using Four = typename std::conditional<L::F32, float4, uint2>::type;
         const int c4 = lane % PER;
-        for (int r = (warp & 3) * AT_ONCE + lane / PER; r < 128; r += 4 * AT_ONCE) {
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int at = t * 128 + r;
-            if (at < rows) {
-                const int64_t row = row0 + at, token = row / a.group;
-                const T* src = static_cast<const T*>(a.q) + (first + token) * a.qs + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D + 4 * c4;
-                if constexpr (L::F32) {
-                    x = *reinterpret_cast<const float4*>(src);
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(src);
-                    const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-                    x = make_float4(lo.x, lo.y, hi.x, hi.y);
+#pragma unroll 1
+        for (int r0 = (warp & 3) * AT_ONCE + lane / PER; r0 < 128; r0 += 4 * AT_ONCE * BATCH) {
+            Four raw[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
+                const int at = t * 128 + r0 + i * 4 * AT_ONCE;
+                raw[i] = Four{};
+                if (at < rows) {
+                    const int64_t row = row0 + at, token = token_of(row);
+                    raw[i] = *reinterpret_cast<const Four*>(static_cast<const T*>(a.q) + (first + token) * a.qs + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D + 4 * c4);
                 }
             }
-            if (negative) x = make_float4(-x.x, -x.y, -x.z, -x.w);
-            uint8_t* tile = sm + L::Q + (t * PARTS) * L::Q_TILE + (c4 >> 4) * (128 * 128);
-            const uint32_t to = swizzled(r, (c4 & 15) >> 1) + (c4 & 1) * 8;
-            if constexpr (L::F32) {
-                uint32_t most = max(max(finite_abs_bits(x.x), finite_abs_bits(x.y)), max(finite_abs_bits(x.z), finite_abs_bits(x.w)));
 #pragma unroll
-                for (int o = PER / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int e = scale_exponent(most);
-                const float up = exp2_int(e);
-                if (c4 == 0) s_row[at] = exp2_int(-e);
-                x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
-                const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
-                const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                *reinterpret_cast<uint2*>(tile + to) = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
-                *reinterpret_cast<uint2*>(tile + L::Q_TILE + to) = make_uint2(pack_f16(x.x - f0.x, x.y - f0.y), pack_f16(x.z - f1.x, x.w - f1.y));
-            } else {
-                *reinterpret_cast<uint2*>(tile + to) = make_uint2(pack_f16(x.x, x.y), pack_f16(x.z, x.w));
+            for (int i = 0; i < BATCH; i++) {
+                const int r = r0 + i * 4 * AT_ONCE;
+                uint8_t* tile = sm + L::Q + (t * PARTS) * L::Q_TILE + (c4 >> 4) * (128 * 128);
+                const uint32_t to = swizzled(r, (c4 & 15) >> 1) + (c4 & 1) * 8;
+                if constexpr (L::F32) {
+                    float4 x = raw[i];
+                    uint32_t most = max(max(finite_abs_bits(x.x), finite_abs_bits(x.y)), max(finite_abs_bits(x.z), finite_abs_bits(x.w)));
+#pragma unroll
+                    for (int o = PER / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    const int e = scale_exponent(most);
+                    const float up = negative ? -exp2_int(e) : exp2_int(e);
+                    if (c4 == 0) s_row[t * 128 + r] = exp2_int(-e);
+                    x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
+                    const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
+                    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                    *reinterpret_cast<uint2*>(tile + to) = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+                    *reinterpret_cast<uint2*>(tile + L::Q_TILE + to) = make_uint2(pack_f16(x.x - f0.x, x.y - f0.y), pack_f16(x.z - f1.x, x.w - f1.y));
+                } else {
+                    uint2 x = raw[i];
+                    if (negative) x = make_uint2(x.x ^ 0x80008000u, x.y ^ 0x80008000u);
+                    *reinterpret_cast<uint2*>(tile + to) = x;
+                }
             }
         }
         fence_proxy_async();
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         tc_fence_after();
         if (at < rows || own_blocks > 0) {
             const float inv = 1.f / sum * v_top;
-            const int64_t row = row0 + at, token = row / a.group;
+            const int64_t row = row0 + at, token = token_of(row);
             T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D;
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
@@ -491,10 +498,11 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         constexpr int PIECES = D / 16, N = KT * PIECES / 128;  // 16-byte pieces of a key; of a block's, a thread's: key first_key + i STEP, always the same piece
         constexpr int STEP = 128 / PIECES;
         const int me = tid - 128 * TILES, own_key = me / PIECES, piece = me % PIECES;
-        const int64_t head = static_cast<int64_t>(h) * c.page * D + piece * 16;
+        const int64_t head = static_cast<int64_t>(h) * c.page * D + piece * 16, page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
         const uint32_t tile_at = (piece >> 2) * (KT * 128);
+        // Pages are looked up three blocks ahead, codes asked for two ahead; keys of block j + 1 are put down before values of block j.
         int page[N];
-        uint4 kx[N], vx[N];
+        uint4 kx[2][N], vx[2][N];
         auto look_up = [&](int j) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
@@ -502,15 +510,15 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 page[i] = key < seen ? q.table[static_cast<int64_t>(b) * q.width + (key >> c.page_log)] : -1;
             }
         };
-        auto load = [&](int j) {
+        auto load = [&](int j, uint4 (&kr)[N], uint4 (&vr)[N]) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);  // (keys that no row sees)
+                kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);  // (keys that no row sees)
                 if (page[i] >= 0) {
-                    const int slot = static_cast<int>((static_cast<int64_t>(j) * KT + own_key + i * STEP) & (c.page - 1));
-                    const int64_t off = static_cast<int64_t>(page[i]) * c.kv_heads * c.page * D + head + slot * D;
-                    kx[i] = *reinterpret_cast<const uint4*>(c.k + off);
-                    vx[i] = *reinterpret_cast<const uint4*>(c.v + off);
+                    const int slot = (static_cast<int>(j * KT) + own_key + i * STEP) & (c.page - 1);
+                    const int64_t off = static_cast<int64_t>(page[i]) * page_bytes + head + slot * D;
+                    kr[i] = *reinterpret_cast<const uint4*>(c.k + off);
+                    vr[i] = *reinterpret_cast<const uint4*>(c.v + off);
                 }
             }
         };
@@ -523,24 +531,37 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             }
             fence_proxy_async();
         };
-        look_up(0);
-        load(0);
-        look_up(1);
         bool ok = true;
-        for (int j = 0; j < blocks; j++) {
-            const int buf = j & 1;
-            const uint32_t parity = ((j >> 1) - 1) & 1;
-            if (j >= 2) ok = mbar_wait(k_free(buf), parity, abort_flag, status);
-            if (!ok) break;
-            put(L::K + buf * L::KV_TILE, kx);
-            mbar_arrive(k_full(buf));
-            if (j >= 2) ok = mbar_wait(v_free(buf), parity, abort_flag, status);
-            if (!ok) break;
-            put(L::V + buf * L::KV_TILE, vx);
-            mbar_arrive(v_full(buf));
-            if (j + 1 < blocks) {
-                load(j + 1);
-                look_up(j + 2);
+        auto put_k = [&](int j, const uint4 (&x)[N]) {
+            if (j >= 2) ok = ok && mbar_wait(k_free(j & 1), ((j >> 1) - 1) & 1, abort_flag, status);
+            if (!ok) return;
+            put(L::K + (j & 1) * L::KV_TILE, x);
+            mbar_arrive(k_full(j & 1));
+        };
+        auto put_v = [&](int j, const uint4 (&x)[N]) {
+            if (j >= 2) ok = ok && mbar_wait(v_free(j & 1), ((j >> 1) - 1) & 1, abort_flag, status);
+            if (!ok) return;
+            put(L::V + (j & 1) * L::KV_TILE, x);
+            mbar_arrive(v_full(j & 1));
+        };
+        look_up(0);
+        load(0, kx[0], vx[0]);
+        look_up(1);
+        load(1, kx[1], vx[1]);
+        look_up(2);
+        put_k(0, kx[0]);
+        for (int j = 0; j < blocks && ok; j += 2) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int jj = j + e;
+                if (jj < blocks) {
+                    if (jj + 1 < blocks) put_k(jj + 1, kx[e ^ 1]);
+                    put_v(jj, vx[e]);
+                    if (jj + 2 < blocks) {
+                        load(jj + 2, kx[e], vx[e]);
+                        look_up(jj + 3);
+                    }
+                }
             }
         }
     } else if (lane == 0) {
