@@ -5,7 +5,8 @@
 // second the rounding error of the first), whose products go to the same accumulator.
 //   warps 0-3, 4-7   softmax of a tile, one thread to a row: scores out of TMEM, weights into shared memory
 //   warps 8-11       codes of K and V from the pages into f16 tiles, two blocks ahead
-//   warp 12          one thread issues the MMAs: scores of block j + 1 before the values of block j, so that a softmax never waits for its scores
+//   warp 12          one thread issues the MMAs: scores of block j + 1 before the values of block j, so that a softmax never waits for its scores.  (Its instructions are few on
+//                    purpose: with 64-bit descriptors and a barrier more for each thing it was the bound, 4700 cycles per block.)
 // What bounds it: the exponentials (16 per clock and SM; the products of a block take as long at 128 values per head, half as long at 64) and, around them, the
 // softmax warps' issue slots.
 // The output sums stay in TMEM.  They are brought under a new maximum only when a row's has grown by more than 2^8 (weights are up to 2^14 then), which after the first
@@ -25,9 +26,6 @@ using umma::fence_proxy_async;
 using umma::mbar_arrive;
 using umma::mbar_init;
 using umma::mbar_wait;
-using umma::mma_f16;
-using umma::smem_desc_k128;
-using umma::smem_desc_n128;
 using umma::smem_u32;
 using umma::tc_fence_after;
 using umma::tc_fence_before;
@@ -53,9 +51,10 @@ struct Prompt {
     static constexpr int TILES = F32 && D == 128 ? 1 : 2;  // (fp32 results: sums twice, in TMEM)
     static constexpr int PARTS = F32 ? 2 : 1;            // f16 numbers of a query or weight
     static constexpr int KT = 64;                        // keys of a block
+    static constexpr int STAGES = 3;
     static constexpr int THREADS = 128 * TILES + 128 + 32;
     static constexpr uint32_t Q_TILE = 128 * 128 * HALVES, P_TILE = 128 * 128, KV_TILE = KT * 128 * HALVES;
-    static constexpr uint32_t Q = 0, P = Q + TILES * PARTS * Q_TILE, K = P + TILES * PARTS * P_TILE, V = K + 2 * KV_TILE, EXTRA = V + 2 * KV_TILE;
+    static constexpr uint32_t Q = 0, P = Q + TILES * PARTS * Q_TILE, STAGE = 2 * KV_TILE, KV = P + TILES * PARTS * P_TILE, EXTRA = KV + STAGES * STAGE;  // a stage: K, then V
     static constexpr uint32_t ROW_SCALE = EXTRA, RED = ROW_SCALE + TILES * 512, BARS = RED + 128, TOTAL = BARS + 256 + 1024;
     static constexpr uint32_t O_AT = 256, O_PITCH = 128, KEPT = D == 64 ? 64 : 128;  // TMEM columns: scores [tile][2][64], sums, (fp32) kept sums behind them
     static constexpr int FLUSH = 4;                      // (fp32) blocks per accumulation
@@ -104,6 +103,35 @@ __device__ __noinline__ void row_in_fp32(const Cache& c, const Batch& q, const A
     for (int i = 0; i < N; i++) o[lane + 32 * i] = static_cast<T>(sees <= 0 ? 0.f : acc[i] / sum);
 }
 
+// two fp32 operations by one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// D[tmem] (+)= A x B, kind::f16, issued by one thread: the descriptors' lower halves (their addresses) vary, their upper halves are the same for all tiles here.
+template <bool ADD>
+__device__ __forceinline__ void mma_at(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    constexpr uint32_t upper = (1024 >> 4) | (1u << 14) | (2u << 29);  // 1 KB between groups of 8 rows, version 1, 128-byte swizzle
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(upper), "n"(ADD ? 1 : 0)
+        : "memory");
+}
+
 // 16-byte unit u of row r in a tile of 128-byte rows, 128-byte swizzle
 __device__ __forceinline__ uint32_t swizzled(int r, int u) { return static_cast<uint32_t>(r * 128 + ((u ^ (r & 7)) << 4)); }
 
@@ -130,17 +158,15 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     float* s_row = reinterpret_cast<float*>(sm + L::ROW_SCALE);
     volatile uint32_t* s_red = reinterpret_cast<volatile uint32_t*>(sm + L::RED);
     const uint32_t bars = base + L::BARS;
-    // barriers: K and V tiles filled and free, scores filled and read, weights filled and consumed
-    auto k_full = [&](int i) { return bars + 8u * i; };
-    auto k_free = [&](int i) { return bars + 8u * (2 + i); };
-    auto v_full = [&](int i) { return bars + 8u * (4 + i); };
-    auto v_free = [&](int i) { return bars + 8u * (6 + i); };
+    // barriers: keys and values of a stage in place and done with, scores in TMEM, weights in place and done with.  (A place for scores is free again when the
+    // weights made of them are there: nobody waits for that apart.)
+    auto kv_full = [&](int i) { return bars + 8u * i; };
+    auto kv_free = [&](int i) { return bars + 8u * (4 + i); };
     auto s_full = [&](int t, int i) { return bars + 8u * (8 + 2 * t + i); };
-    auto s_free = [&](int t, int i) { return bars + 8u * (12 + 2 * t + i); };
-    auto p_full = [&](int t) { return bars + 8u * (16 + t); };
-    auto p_free = [&](int t) { return bars + 8u * (18 + t); };
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::BARS + 8 * 20);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::BARS + 8 * 20 + 8);
+    auto p_full = [&](int t) { return bars + 8u * (12 + t); };
+    auto p_free = [&](int t) { return bars + 8u * (14 + t); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::BARS + 8 * 16);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::BARS + 8 * 16 + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // ---- which rows: sequence by sequence, the tiles that see most first ----
@@ -210,15 +236,13 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             s_red[2 * warp + 1] = l;
         }
         if (tid == 0) {
+            for (int i = 0; i < L::STAGES; i++) {
+                mbar_init(kv_full(i), 128);
+                mbar_init(kv_free(i), 1);
+            }
             for (int i = 0; i < 2; i++) {
-                mbar_init(k_full(i), 128);
-                mbar_init(k_free(i), 1);
-                mbar_init(v_full(i), 128);
-                mbar_init(v_free(i), 1);
-                for (int t2 = 0; t2 < 2; t2++) {
-                    mbar_init(s_full(t2, i), 1);
-                    mbar_init(s_free(t2, i), 128);
-                }
+                mbar_init(s_full(0, i), 1);
+                mbar_init(s_full(1, i), 1);
                 mbar_init(p_full(i), 128);
                 mbar_init(p_free(i), 1);
             }
@@ -320,26 +344,36 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         uint32_t s_phase = 0, p_phase = 0;
         bool ok = true, fresh = true;  // fresh: nothing kept yet (fp32)
         int in_run = 0;                // (fp32) blocks since the sums were last added up
-        // scales of 16 keys each, a block ahead; lanes 0-3 look them up
+        // scales of 16 keys each: lanes 0-3 look up pages two blocks ahead, scales one
+        int page_next = 0;
         float ks_next = 0.f, vs_next = 0.f;
-        auto scales_of = [&](int j) {
+        auto page_of = [&](int j) {
             const int64_t key = static_cast<int64_t>(j) * KT + (lane & 3) * 16;
+            page_next = -1;
+            if (lane < 4 && key < seen) page_next = q.table[static_cast<int64_t>(b) * q.width + (key >> c.page_log)];
+        };
+        auto scales_of = [&]() {
             ks_next = vs_next = 0.f;
-            if (lane < 4 && key < seen) {
-                const int64_t block = static_cast<int64_t>(q.table[static_cast<int64_t>(b) * q.width + (key >> c.page_log)]) * c.kv_heads + h;
+            if (page_next >= 0) {
+                const int64_t block = static_cast<int64_t>(page_next) * c.kv_heads + h;
                 ks_next = c.ks[block];
-                vs_next = c.vs[block] * v_inv;
+                vs_next = c.vs[block];
             }
         };
-        if (own_blocks > 0) scales_of(0);
+        if (own_blocks > 0) {
+            page_of(0);
+            scales_of();
+            page_of(1);
+        }
         for (int j = 0; j < own_blocks; j++) {
             float f[4], v[4];
 #pragma unroll
             for (int n = 0; n < 4; n++) {
                 f[n] = fmaxf(__shfl_sync(0xffffffffu, ks_next, n) * q_scale, 1e-38f);  // (not zero: hidden scores stay -inf)
-                v[n] = __shfl_sync(0xffffffffu, vs_next, n);
+                v[n] = __shfl_sync(0xffffffffu, vs_next, n) * v_inv;
             }
-            if (j + 1 < own_blocks) scales_of(j + 1);
+            scales_of();
+            page_of(j + 2);
             const int buf = j & 1;
             ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, buf), s_phase, abort_flag, status));
             if (!ok) break;
@@ -348,8 +382,6 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             tmem_ld_x32(s_at + buf * 64, *reinterpret_cast<uint32_t(*)[32]>(s));
             tmem_ld_x32(s_at + buf * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
             tmem_wait_ld();
-            tc_fence_before();
-            mbar_arrive(s_free(t, buf));
             if (buf) s_phase ^= 1;
             if (static_cast<int64_t>(j + 1) * KT > least) {
                 const int see = static_cast<int>(max(min(sees - static_cast<int64_t>(j) * KT, static_cast<int64_t>(KT)), int64_t(0)));
@@ -373,21 +405,32 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             top = new_top;
             sum *= move ? corr : 1.f;
             const float shift = (top == -INFINITY ? 0.f : top) - 6.f;  // weights are 2^6 exp2(s - top)
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 part[2] = {};
 #pragma unroll
             for (int n = 0; n < 4; n++) {
+                const float2 f2 = make_float2(f[n], f[n]), shift2 = make_float2(-shift, -shift);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    s[16 * n + i] = ex2(fmaf(s[16 * n + i], f[n], -shift));
-                    part[i & 3] += s[16 * n + i];
+                for (int i = 0; i < 16; i += 2) {
+                    float2 x = fma2(make_float2(s[16 * n + i], s[16 * n + i + 1]), f2, shift2);
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
+                    part[(i >> 1) & 1] = add2(part[(i >> 1) & 1], x);
+                    s[16 * n + i] = x.x;
+                    s[16 * n + i + 1] = x.y;
                 }
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            part[0] = add2(part[0], part[1]);
+            sum += part[0].x + part[0].y;
 #pragma unroll
             for (int n = 0; n < 4; n++) {
                 if (v[n] != 1.f) {
+                    const float2 v2 = make_float2(v[n], v[n]);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) s[16 * n + i] *= v[n];
+                    for (int i = 0; i < 16; i += 2) {
+                        const float2 x = mul2(make_float2(s[16 * n + i], s[16 * n + i + 1]), v2);
+                        s[16 * n + i] = x.x;
+                        s[16 * n + i + 1] = x.y;
+                    }
                 }
             }
             // the values of the block before have been added: their weights' place is free, and the sums can be touched
@@ -500,7 +543,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         const int me = tid - 128 * TILES, own_key = me / PIECES, piece = me % PIECES;
         const int64_t head = static_cast<int64_t>(h) * c.page * D + piece * 16, page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
         const uint32_t tile_at = (piece >> 2) * (KT * 128);
-        // Pages are looked up three blocks ahead, codes asked for two ahead; keys of block j + 1 are put down before values of block j.
+        // Pages are looked up three blocks ahead, codes asked for two ahead.
         int page[N];
         uint4 kx[2][N], vx[2][N];
         auto look_up = [&](int j) {
@@ -529,87 +572,95 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 *reinterpret_cast<uint4*>(sm + tile + tile_at + swizzled(r, u)) = eight_f16(x[i].x, x[i].y);
                 *reinterpret_cast<uint4*>(sm + tile + tile_at + swizzled(r, u + 1)) = eight_f16(x[i].z, x[i].w);
             }
-            fence_proxy_async();
         };
         bool ok = true;
-        auto put_k = [&](int j, const uint4 (&x)[N]) {
-            if (j >= 2) ok = ok && mbar_wait(k_free(j & 1), ((j >> 1) - 1) & 1, abort_flag, status);
+        int stage = 0;
+        uint32_t phase = 1;  // (the first pass over the stages goes through)
+        auto put_block = [&](const uint4 (&kr)[N], const uint4 (&vr)[N]) {
+            ok = mbar_wait(kv_free(stage), phase, abort_flag, status);
             if (!ok) return;
-            put(L::K + (j & 1) * L::KV_TILE, x);
-            mbar_arrive(k_full(j & 1));
-        };
-        auto put_v = [&](int j, const uint4 (&x)[N]) {
-            if (j >= 2) ok = ok && mbar_wait(v_free(j & 1), ((j >> 1) - 1) & 1, abort_flag, status);
-            if (!ok) return;
-            put(L::V + (j & 1) * L::KV_TILE, x);
-            mbar_arrive(v_full(j & 1));
+            put(L::KV + stage * L::STAGE, kr);
+            put(L::KV + stage * L::STAGE + L::KV_TILE, vr);
+            fence_proxy_async();
+            mbar_arrive(kv_full(stage));
+            if (++stage == L::STAGES) {
+                stage = 0;
+                phase ^= 1;
+            }
         };
         look_up(0);
         load(0, kx[0], vx[0]);
         look_up(1);
         load(1, kx[1], vx[1]);
         look_up(2);
-        put_k(0, kx[0]);
         for (int j = 0; j < blocks && ok; j += 2) {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const int jj = j + e;
-                if (jj < blocks) {
-                    if (jj + 1 < blocks) put_k(jj + 1, kx[e ^ 1]);
-                    put_v(jj, vx[e]);
-                    if (jj + 2 < blocks) {
-                        load(jj + 2, kx[e], vx[e]);
-                        look_up(jj + 3);
-                    }
+                if (j + e < blocks && ok) {
+                    put_block(kx[e], vx[e]);
+                    load(j + e + 2, kx[e], vx[e]);
+                    look_up(j + e + 3);
                 }
             }
         }
     } else if (lane == 0) {
         // ---------------- MMAs ----------------
         constexpr uint32_t qk = (1u << 4) | ((KT >> 3) << 17) | ((128 >> 4) << 24), pv = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);  // (values: keys along the rows)
-        const uint64_t q_desc = smem_desc_k128(base + L::Q), k_desc = smem_desc_k128(base + L::K), p_desc = smem_desc_k128(base + L::P), v_desc = smem_desc_n128(base + L::V);
+        // lower halves of the operands' descriptors: address / 16, and for the values 8 KB between blocks of 64 dims
+        const uint32_t q_at = (base + L::Q) >> 4 | 1u << 16, k_at = (base + L::KV) >> 4 | 1u << 16, p_at = (base + L::P) >> 4 | 1u << 16,
+                       v_at = (base + L::KV + L::KV_TILE) >> 4 | (8192u >> 4) << 16;
         bool ok = true;
-        auto scores = [&](int t, int j) {
-            if (j >= 2) ok = ok && mbar_wait(s_free(t, j & 1), ((j >> 1) - 1) & 1, abort_flag, status);
+        int ask = 0, use = 0;  // stages of the next scores and values
+        uint32_t ask_phase = 0;
+        auto block_scores = [&](int j) {
+            ok = ok && mbar_wait(kv_full(ask), ask_phase, abort_flag, status);
             if (!ok) return;
             tc_fence_after();
-            const uint32_t d = tmem + t * 128 + (j & 1) * 64;
+            const uint32_t kd = k_at + ask * (L::STAGE >> 4), d = tmem + (j & 1) * 64;
 #pragma unroll
-            for (int part = PARTS - 1; part >= 0; part--)  // the small products first
+            for (int t = 0; t < TILES; t++) {
+                if (t == 0 ? j < blocks0 : tiles == 2) {
 #pragma unroll
-                for (int half = 0; half < HALVES; half++)
+                    for (int part = PARTS - 1; part >= 0; part--)  // the small products first
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        mma_f16<1>(d, q_desc + (((t * PARTS + part) * L::Q_TILE + half * (128 * 128)) >> 4) + kk * 2, k_desc + (((j & 1) * L::KV_TILE + half * (KT * 128)) >> 4) + kk * 2, qk,
-                                   part < PARTS - 1 || half > 0 || kk > 0);
-            umma::commit<1>(s_full(t, j & 1));
-        };
-        auto block_scores = [&](int j) {
-            ok = ok && mbar_wait(k_full(j & 1), (j >> 1) & 1, abort_flag, status);
-            if (j < blocks0) scores(0, j);
-            if (TILES == 2 && tiles == 2) scores(1, j);
-            if (ok) umma::commit<1>(k_free(j & 1));
+                        for (int half = 0; half < HALVES; half++)
+#pragma unroll
+                            for (int kk = 0; kk < 4; kk++) {
+                                const uint32_t qa = q_at + (((t * PARTS + part) * L::Q_TILE + half * (128 * 128)) >> 4) + kk * 2, kb = kd + ((half * (KT * 128)) >> 4) + kk * 2;
+                                if (part < PARTS - 1 || half > 0 || kk > 0) mma_at<true>(d + t * 128, qa, kb, qk);
+                                else mma_at<false>(d + t * 128, qa, kb, qk);
+                            }
+                    umma::commit<1>(s_full(t, j & 1));
+                }
+            }
+            if (++ask == L::STAGES) {
+                ask = 0;
+                ask_phase ^= 1;
+            }
         };
         block_scores(0);
         for (int j = 0; j < blocks && ok; j++) {
             if (j + 1 < blocks) block_scores(j + 1);
-            ok = ok && mbar_wait(v_full(j & 1), (j >> 1) & 1, abort_flag, status);
+            const uint32_t vd = v_at + use * (L::STAGE >> 4);
 #pragma unroll
             for (int t = 0; t < TILES; t++) {
-                if (t < tiles && j < (t == 0 ? blocks0 : blocks)) {
+                if (t == 0 ? j < blocks0 : tiles == 2) {
                     ok = ok && mbar_wait(p_full(t), j & 1, abort_flag, status);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
                     for (int part = PARTS - 1; part >= 0; part--)
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++)
-                            mma_f16<1>(tmem + L::O_AT + t * L::O_PITCH, p_desc + (((t * PARTS + part) * L::P_TILE) >> 4) + kk * 2, v_desc + (((j & 1) * L::KV_TILE) >> 4) + kk * 128, pv,
-                                       j > 0 || part < PARTS - 1 || kk > 0);
+                        for (int kk = 0; kk < 4; kk++) {
+                            const uint32_t d = tmem + L::O_AT + t * L::O_PITCH, pa = p_at + (((t * PARTS + part) * L::P_TILE) >> 4) + kk * 2, vb = vd + kk * 128;
+                            if (part < PARTS - 1 || kk > 0 || j > 0) mma_at<true>(d, pa, vb, pv);
+                            else mma_at<false>(d, pa, vb, pv);
+                        }
                     umma::commit<1>(p_free(t));
                 }
             }
-            if (ok) umma::commit<1>(v_free(j & 1));
+            if (ok) umma::commit<1>(kv_free(use));
+            if (++use == L::STAGES) use = 0;
         }
     }
     tc_fence_before();
