@@ -58,125 +58,226 @@ struct Append {
     int64_t ks, vs, qs, os;  // row strides
     const float *cos, *sin;
     int64_t table_rows;
-    int q_heads;
+    int q_heads, parts, q_parts;  // parts of a piece: K of each head, V of each head, queries in groups of heads
     void* q_out;
     int* status;
+    int64_t items;
+    int pages_each;  // pages that a sequence's new tokens can fall into, where all have as many
 };
-
-// one rounding: the products are exact in fp64
-__device__ __forceinline__ float rotated(float x, float y, float c, float s) {
-    return static_cast<float>(static_cast<double>(x) * c + static_cast<double>(y) * s);
-}
 
 // the least 2^e >= 2^-126 with m <= 127 2^e; NaN for a maximum that is not finite
 __device__ __forceinline__ float least_scale(uint32_t max_bits) {
     if (max_bits >= 0x7f800000u) return __int_as_float(0x7fc00000);
-    int e = static_cast<int>(max_bits >> 23) - 6 + ((max_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);  // (biased) 1.984375 = 127 / 64
+    const int e = static_cast<int>(max_bits >> 23) - 6 + ((max_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);  // (biased) 1.984375 = 127 / 64
     return __int_as_float(max(e, 1) << 23);
 }
 
-__device__ __forceinline__ float value(const float* p) { return *p; }
-__device__ __forceinline__ float value(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four(const __half* p) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void put_four(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
+__device__ __forceinline__ void put_four(__half* p, float4 x) {
+    const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
 
-// One CTA per (page that a sequence's new tokens fall into, head, K or V).
-template <typename T>
-__global__ void __launch_bounds__(128) append_kernel(const Cache c, const Batch q, const Append a, int pages_each) {
-    dep_sync();
-    __shared__ uint32_t s_max[4];
-    int b, j;
-    int64_t first, count;
-    if (!q.starts) {
-        b = blockIdx.x / pages_each;
-        j = blockIdx.x - b * pages_each;
-        q.rows(b, first, count);
-    } else {  // sequence by sequence; item i of all
-        int i = blockIdx.x;
-        for (b = 0; b < q.batch; b++) {
-            q.rows(b, first, count);
-            const int64_t p0 = q.lens[b] - count;
-            const int n = count > 0 && q.lens[b] > 0 ? static_cast<int>(((q.lens[b] - 1) >> c.page_log) - (max(p0, int64_t(0)) >> c.page_log) + 1) : 0;
-            if (i < n) break;
-            i -= n;
+// Four dims of the lower half of a head and the four that go with them: one position's rows of the tables, in fp64.  Products of fp32 values are exact there, and the sum is
+// rounded once.  (The conversions cost more than the arithmetic: 8 cycles per warp each.  Heads of a token share the tables'.)
+struct Rotation {
+    double cl[4], sl[4], ch[4], sh[4];
+    __device__ __forceinline__ void load(const float* cos, const float* sin, int half) {
+        const float4 a = four(cos), b = four(sin), c = four(cos + half), d = four(sin + half);
+        cl[0] = a.x, cl[1] = a.y, cl[2] = a.z, cl[3] = a.w;
+        sl[0] = b.x, sl[1] = b.y, sl[2] = b.z, sl[3] = b.w;
+        ch[0] = c.x, ch[1] = c.y, ch[2] = c.z, ch[3] = c.w;
+        sh[0] = d.x, sh[1] = d.y, sh[2] = d.z, sh[3] = d.w;
+    }
+    __device__ __forceinline__ void turn(float4& low, float4& high) const {
+        float l[4] = {low.x, low.y, low.z, low.w}, h[4] = {high.x, high.y, high.z, high.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const double x = l[i], y = h[i];
+            l[i] = static_cast<float>(x * cl[i] - y * sl[i]);
+            h[i] = static_cast<float>(y * ch[i] + x * sh[i]);
         }
-        if (b == q.batch) return;
-        j = i;
+        low = make_float4(l[0], l[1], l[2], l[3]);
+        high = make_float4(h[0], h[1], h[2], h[3]);
+    }
+};
+
+__device__ __forceinline__ uint32_t most_of(float4 x) {
+    return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
+}
+// |x inv| <= 127: the lowest byte of x inv + 1.5 2^23, which is rounded to an integer, ties to even
+__device__ __forceinline__ uint32_t codes_of(float4 x, float inv) {
+    const float up = 12582912.f;
+    const uint32_t a = __float_as_uint(fmaf(x.x, inv, up)), b = __float_as_uint(fmaf(x.y, inv, up)), c = __float_as_uint(fmaf(x.z, inv, up)), d = __float_as_uint(fmaf(x.w, inv, up));
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// An item: the new tokens of a sequence that fall into one page, as K or V of one head, or the queries of some heads.  GROUP threads to an item; a thread has four dims of
+// the lower half of a head and the four that go with them in the upper half, of every (GROUP / (D / 8))-th token: values stay in registers from their maximum to their codes.
+template <typename T, int D, int GROUP, int ITERS>
+__global__ void __launch_bounds__(256) append_kernel(const Cache c, const Batch q, const Append a) {
+    dep_sync();
+    constexpr int PACKS = D / 8, AT_ONCE = GROUP / PACKS, HALF = D / 2;
+    __shared__ uint32_t s_max[8];
+    const int me = threadIdx.x % GROUP, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * (256 / GROUP) + threadIdx.x / GROUP;
+    if (item >= a.items) return;  // (GROUP = 256: never)
+    const int64_t piece = item / a.parts;
+    const int part = static_cast<int>(item - piece * a.parts);
+    // ---- which sequence, which of its pages ----
+    int b = 0;
+    int64_t j = 0, first = 0, count = 0;
+    if (!q.starts) {
+        b = static_cast<int>(piece / a.pages_each);
+        j = piece - static_cast<int64_t>(b) * a.pages_each;
+        q.rows(b, first, count);
+    } else {  // a warp looks at 32 sequences at a time (every warp for itself: the same answer)
+        int64_t left = piece;
+        bool found = false;
+        for (int b0 = 0; b0 < q.batch && !found; b0 += 32) {
+            int64_t f = 0, n = 0;
+            int own = 0;
+            if (b0 + lane < q.batch) {
+                q.rows(b0 + lane, f, n);
+                const int64_t len = q.lens[b0 + lane], p0 = max(len - n, int64_t(0));
+                own = n > 0 && len > 0 ? static_cast<int>(((len - 1) >> c.page_log) - (p0 >> c.page_log) + 1) : 0;
+            }
+            int upto = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const uint32_t mask = __ballot_sync(0xffffffffu, left < upto);
+            if (mask) {
+                const int l = __ffs(mask) - 1;
+                b = b0 + l;
+                j = left - __shfl_sync(0xffffffffu, upto - own, l);
+                first = __shfl_sync(0xffffffffu, f, l);
+                count = __shfl_sync(0xffffffffu, n, l);
+                found = true;
+            } else {
+                left -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        if (!found) return;
     }
     const int64_t len = q.lens[b], p0 = len - count;  // the first new token's position, below 0 where it has none
     if (count == 0 || len <= 0) return;
     const int64_t at = (max(p0, int64_t(0)) >> c.page_log) + j;
     const int64_t t0 = max(max(p0, int64_t(0)), at << c.page_log), t1 = min(len, (at + 1) << c.page_log);
     if (t0 >= t1) return;
-    const int page = at < q.width ? q.table[b * q.width + at] : -1;
+    const int page = at < q.width ? q.table[static_cast<int64_t>(b) * q.width + at] : -1;
     const int64_t t_end = a.cos ? min(t1, a.table_rows) : t1;  // tokens behind it have no row in the tables
-    if (page < 0 || page >= c.pages || t_end < t1) {
-        if (a.status && threadIdx.x == 0) *a.status = RMLK_ERR_INVALID_ARG;
-        if (page < 0 || page >= c.pages) return;
-    }
-    const int h = blockIdx.y, half = c.d / 2;
-    const bool is_v = blockIdx.z;
-    const int slot0 = static_cast<int>(t0 & (c.page - 1)), n = static_cast<int>(t_end - t0);
-    if (n <= 0) return;
-    const T* src = static_cast<const T*>(is_v ? a.v : a.k) + (first + t0 - p0) * (is_v ? a.vs : a.ks) + static_cast<int64_t>(h) * c.d;
-    const int64_t stride = is_v ? a.vs : a.ks;
-    const int64_t block = static_cast<int64_t>(page) * c.kv_heads + h;
-    int8_t* dst = (is_v ? c.v : c.k) + block * c.page * c.d;
-    float* scale = (is_v ? c.vs : c.ks) + block;
-    auto get = [&](int r, int i) {
-        const T* x = src + r * stride;
-        const float own = value(x + i);
-        if (is_v || !a.cos) return own;
-        const float other = i < half ? -value(x + i + half) : value(x + i - half);
-        return rotated(own, other, a.cos[(t0 + r) * c.d + i], a.sin[(t0 + r) * c.d + i]);
-    };
-    uint32_t m = 0;
-    for (int i = threadIdx.x; i < n * c.d; i += 128) m = max(m, __float_as_uint(get(i / c.d, i % c.d)) & 0x7fffffffu);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-    const float old = slot0 > 0 ? *scale : 0.f;
-    __syncthreads();
-    m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
-    float s = least_scale(m);
-    if (!(s > old)) s = s != s ? s : old;  // (a NaN of either stays)
-    if (threadIdx.x == 0) *scale = s;
-    if (slot0 > 0 && s > old) {
-        const float ratio = old / s;
-        for (int i = threadIdx.x; i < slot0 * c.d; i += 128) dst[i] = static_cast<int8_t>(rintf(dst[i] * ratio));
-    }
-    const float inv = 1.f / s;
-    for (int i = threadIdx.x; i < n * c.d; i += 128) dst[slot0 * c.d + i] = s == s ? static_cast<int8_t>(rintf(get(i / c.d, i % c.d) * inv)) : 0;
-}
+    const bool lost = page < 0 || page >= c.pages;
+    if ((lost || t_end < t1) && a.status && me == 0) *a.status = RMLK_ERR_INVALID_ARG;
+    const int n = lost ? 0 : static_cast<int>(max(t_end - t0, int64_t(0)));
+    if (n == 0) return;
+    const int64_t row = first + t0 - p0;
+    const int c4 = me % PACKS * 4, r0 = me / PACKS;
 
-// The queries: one CTA per new token.
-template <typename T>
-__global__ void __launch_bounds__(128) rotate_kernel(const Cache c, const Batch q, const Append a) {
-    dep_sync();
-    const int64_t row = blockIdx.x;
-    int b;
-    int64_t first = 0, count = 0;
-    if (!q.starts) {
-        b = static_cast<int>(row / q.each);
-        q.rows(b, first, count);
-    } else {
-        for (b = 0; b < q.batch; b++) {
-            q.rows(b, first, count);
-            if (row >= first && row < first + count) break;
+    if (part >= 2 * c.kv_heads) {  // ---- queries ----
+        const int h0 = part - 2 * c.kv_heads;
+        for (int r = r0; r < n; r += AT_ONCE) {
+            Rotation turn;
+            turn.load(a.cos + (t0 + r) * D + c4, a.sin + (t0 + r) * D + c4, HALF);
+            const T* src = static_cast<const T*>(a.q) + (row + r) * a.qs + c4;
+            T* dst = static_cast<T*>(a.q_out) + (row + r) * a.os + c4;
+#pragma unroll 2
+            for (int h = h0; h < a.q_heads; h += a.q_parts) {
+                float4 low = four(src + static_cast<int64_t>(h) * D), high = four(src + static_cast<int64_t>(h) * D + HALF);
+                turn.turn(low, high);
+                put_four(dst + static_cast<int64_t>(h) * D, low);
+                put_four(dst + static_cast<int64_t>(h) * D + HALF, high);
+            }
         }
-        if (b == q.batch) return;
-    }
-    const int64_t p = q.lens[b] - count + row - first, at = p >> c.page_log;
-    if (p < 0) return;
-    const int page = at < q.width ? q.table[b * q.width + at] : -1;
-    if (page < 0 || page >= c.pages || p >= a.table_rows) {
-        if (a.status && threadIdx.x == 0) *a.status = RMLK_ERR_INVALID_ARG;
         return;
     }
-    const int half = c.d / 2;
-    const T* x = static_cast<const T*>(a.q) + row * a.qs;
-    T* o = static_cast<T*>(a.q_out) + row * a.os;
-    for (int i = threadIdx.x; i < a.q_heads * c.d; i += 128) {
-        const int e = i % c.d;
-        const float other = e < half ? -value(x + i + half) : value(x + i - half);
-        o[i] = static_cast<T>(rotated(value(x + i), other, a.cos[p * c.d + e], a.sin[p * c.d + e]));
+
+    // ---- K or V of one head ----
+    const bool is_v = part >= c.kv_heads;
+    const int h = is_v ? part - c.kv_heads : part, slot0 = static_cast<int>(t0 & (c.page - 1));
+    const int64_t stride = is_v ? a.vs : a.ks, block = static_cast<int64_t>(page) * c.kv_heads + h;
+    const T* src = static_cast<const T*>(is_v ? a.v : a.k) + row * stride + static_cast<int64_t>(h) * D + c4;
+    int8_t* dst = (is_v ? c.v : c.k) + block * c.page * D;
+    float* scale = (is_v ? c.vs : c.ks) + block;
+    const float old = slot0 > 0 ? *scale : 0.f;
+    float4 low[ITERS], high[ITERS];
+#pragma unroll
+    for (int i = 0; i < ITERS; i++) {
+        const int r = r0 + i * AT_ONCE;
+        low[i] = high[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n) {
+            low[i] = four(src + r * stride);
+            high[i] = four(src + r * stride + HALF);
+        }
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < ITERS; i++) {
+        const int r = r0 + i * AT_ONCE;
+        if (!is_v && a.cos && r < n) {
+            Rotation turn;
+            turn.load(a.cos + (t0 + r) * D + c4, a.sin + (t0 + r) * D + c4, HALF);
+            turn.turn(low[i], high[i]);
+        }
+        m = max(m, max(most_of(low[i]), most_of(high[i])));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (GROUP > 32) {
+        if (lane == 0) s_max[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < GROUP / 32; w++) m = max(m, s_max[w]);
+    } else {
+        __syncwarp();  // every lane has read the old scale
+    }
+    float s = least_scale(m);
+    if (!(s > old)) s = s != s ? s : old;  // (a NaN of either stays)
+    if (me == 0) *scale = s;
+    if (slot0 > 0 && s > old) {  // the codes that are there, under the larger scale
+        const float ratio = old / s;
+        for (int i = me; i < slot0 * D / 4; i += GROUP) {
+            const uint32_t w = reinterpret_cast<uint32_t*>(dst)[i];
+            reinterpret_cast<uint32_t*>(dst)[i] = codes_of(make_float4(static_cast<int8_t>(w), static_cast<int8_t>(w >> 8), static_cast<int8_t>(w >> 16), static_cast<int8_t>(w >> 24)), ratio);
+        }
+    }
+    const float inv = s == s ? 1.f / s : 0.f;
+#pragma unroll
+    for (int i = 0; i < ITERS; i++) {
+        const int r = r0 + i * AT_ONCE;
+        if (r < n) {
+            uint32_t* to = reinterpret_cast<uint32_t*>(dst + (slot0 + r) * D + c4);
+            to[0] = s == s ? codes_of(low[i], inv) : 0u;
+            to[HALF / 4] = s == s ? codes_of(high[i], inv) : 0u;
+        }
+    }
+}
+
+template <typename T, int D, int GROUP, int ITERS>
+static int launch_append(cudaStream_t st, const Cache& c, const Batch& s, const Append& a) {
+    const int64_t ctas = ceil_div64(a.items, 256 / GROUP);
+    if (ctas > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_append: too many tokens");
+    RMLK_CUDA(launch_dep(append_kernel<T, D, GROUP, ITERS>, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, st, c, s, a));
+    RMLK_CHECK_LAUNCH("append_kernel");
+    return RMLK_OK;
+}
+
+// A warp to an item where its tokens fit one pass of a warp's lanes (64 x 1 tokens: 9 us with a CTA to each, of which all but a few threads had nothing to do), else a CTA.
+template <typename T, int D>
+static int dispatch_append(cudaStream_t st, const Cache& c, const Batch& s, const Append& a) {
+    if (!s.starts && s.each <= 256 / D) return launch_append<T, D, 32, 1>(st, c, s, a);
+    switch (c.page * D / (8 * 256)) {
+        case 0: case 1: return launch_append<T, D, 256, 1>(st, c, s, a);
+        case 2: return launch_append<T, D, 256, 2>(st, c, s, a);
+        case 4: return launch_append<T, D, 256, 4>(st, c, s, a);
+        default: return launch_append<T, D, 256, 8>(st, c, s, a);
     }
 }
 
@@ -203,19 +304,29 @@ extern "C" int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rml
     if (!aligned_to(k, 4 * e) || !aligned_to(v, 4 * e) || !aligned_to(q, 4 * e) || !aligned_to(q_out, 4 * e) || !aligned_to(cos, 16) || !aligned_to(sin, 16) || k_stride % 4 ||
         v_stride % 4 || (q && (q_stride % 4 || q_out_stride % 4)))
         return fail(RMLK_ERR_INVALID_ARG, "paged_append: rows must lie on boundaries of four values");
-    paged::Append a = {k, v, q, k_stride, v_stride, q_stride, q_out_stride, cos, sin, table_rows, static_cast<int>(q_heads), q_out, status};
-    // pages that the new tokens can fall into: of each sequence one more than their number divided by the page size, rounded up to whole pages
-    const int64_t pages_each = (s.each + c.page - 2) / c.page + 1;
-    const int64_t items = starts ? tokens / c.page + 2 * std::min<int64_t>(batch, tokens) : batch * pages_each;
-    if (items > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_append: too many tokens");
-    const dim3 grid(static_cast<unsigned>(items), c.kv_heads, 2);
-    if (dtype == RMLK_F32) launch_dep(paged::append_kernel<float>, grid, dim3(128), 0, as_stream(stream), c, s, a, static_cast<int>(pages_each));
-    else launch_dep(paged::append_kernel<__half>, grid, dim3(128), 0, as_stream(stream), c, s, a, static_cast<int>(pages_each));
-    RMLK_CHECK_LAUNCH("append_kernel");
-    if (q) {
-        if (dtype == RMLK_F32) launch_dep(paged::rotate_kernel<float>, dim3(static_cast<unsigned>(tokens)), dim3(128), 0, as_stream(stream), c, s, a);
-        else launch_dep(paged::rotate_kernel<__half>, dim3(static_cast<unsigned>(tokens)), dim3(128), 0, as_stream(stream), c, s, a);
-        RMLK_CHECK_LAUNCH("rotate_kernel");
-    }
-    return RMLK_OK;
+    paged::Append a = {};
+    a.k = k;
+    a.v = v;
+    a.q = q;
+    a.ks = k_stride;
+    a.vs = v_stride;
+    a.qs = q_stride;
+    a.os = q_out_stride;
+    a.cos = cos;
+    a.sin = sin;
+    a.table_rows = table_rows;
+    a.q_heads = static_cast<int>(q_heads);
+    a.q_out = q_out;
+    a.status = status;
+    // queries in groups of up to eight heads, which share a token's rows of the tables; where a sequence has few tokens, of up to two
+    const bool few = !starts && s.each <= 256 / c.d;
+    a.q_parts = q ? static_cast<int>(ceil_div64(q_heads, few ? 2 : 8)) : 0;
+    a.parts = 2 * c.kv_heads + a.q_parts;
+    // pages that the new tokens can fall into: of each sequence one more than their number less two, divided by the page size
+    a.pages_each = (s.each + c.page - 2) / c.page + 1;
+    const int64_t pieces = starts ? tokens / c.page + 2 * std::min<int64_t>(batch, tokens) : batch * a.pages_each;
+    a.items = pieces * a.parts;
+    const cudaStream_t st = as_stream(stream);
+    if (dtype == RMLK_F32) return c.d == 64 ? paged::dispatch_append<float, 64>(st, c, s, a) : paged::dispatch_append<float, 128>(st, c, s, a);
+    return c.d == 64 ? paged::dispatch_append<__half, 64>(st, c, s, a) : paged::dispatch_append<__half, 128>(st, c, s, a);
 }
