@@ -1,6 +1,6 @@
 // New keys and values into a paged cache of 8-bit codes, the keys rotated on the way; the queries rotated beside them.
 //
-//   r = x cos[p] + (-x[D/2:], x[:D/2]) sin[p]       (products of fp32 values are exact in fp64; one rounding to fp32)
+//   r = x cos[p] + (-x[D/2:], x[:D/2]) sin[p]       (keys: exact, one rounding to fp32; queries: in fp32)
 //   2^e: the least power of two with max |r| <= 127 2^e over the new tokens of a block (page, head), at least the block's present scale
 //   code = rne(r 2^-e)
 //
@@ -58,7 +58,7 @@ struct Append {
     int64_t ks, vs, qs, os;  // row strides
     const float *cos, *sin;
     int64_t table_rows;
-    int q_heads, parts, q_parts;  // parts of a piece: K of each head, V of each head, queries in groups of heads
+    int q_heads, parts;  // parts of a piece: K of each head, V of each head, queries by four heads
     void* q_out;
     int* status;
     int64_t items;
@@ -84,8 +84,9 @@ __device__ __forceinline__ void put_four(__half* p, float4 x) {
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// Four dims of the lower half of a head and the four that go with them: one position's rows of the tables, in fp64.  Products of fp32 values are exact there, and the sum is
-// rounded once.  (The conversions cost more than the arithmetic: 8 cycles per warp each.  Heads of a token share the tables'.)
+// Keys: four dims of the lower half of a head and the four that go with them, in fp64.  Products of fp32 values are exact there, and the sum is rounded once, so that a key's
+// codes do not depend on how the rotation is computed.  (The conversions cost more than the arithmetic, 8 cycles per warp each: with the queries rotated so too they were the
+// bound, 55 us for 5600 tokens of 32 + 8 heads of 128.)
 struct Rotation {
     double cl[4], sl[4], ch[4], sh[4];
     __device__ __forceinline__ void load(const float* cos, const float* sin, int half) {
@@ -182,20 +183,31 @@ __global__ void __launch_bounds__(256) append_kernel(const Cache c, const Batch 
     const int64_t row = first + t0 - p0;
     const int c4 = me % PACKS * 4, r0 = me / PACKS;
 
-    if (part >= 2 * c.kv_heads) {  // ---- queries ----
-        const int h0 = part - 2 * c.kv_heads;
+    if (part >= 2 * c.kv_heads) {  // ---- queries: in fp32, one product fused with the sum ----
+        constexpr int HEADS = 4;  // loads of so many heads are on their way together
+        const int h0 = (part - 2 * c.kv_heads) * HEADS;
         for (int r = r0; r < n; r += AT_ONCE) {
-            Rotation turn;
-            turn.load(a.cos + (t0 + r) * D + c4, a.sin + (t0 + r) * D + c4, HALF);
+            const float* cos = a.cos + (t0 + r) * D + c4;
+            const float* sin = a.sin + (t0 + r) * D + c4;
+            const float4 cl = four(cos), ch = four(cos + HALF), sl = four(sin), sh = four(sin + HALF);
             const T* src = static_cast<const T*>(a.q) + (row + r) * a.qs + c4;
             T* dst = static_cast<T*>(a.q_out) + (row + r) * a.os + c4;
-#pragma unroll 2
-            for (int h = h0; h < a.q_heads; h += a.q_parts) {
-                float4 low = four(src + static_cast<int64_t>(h) * D), high = four(src + static_cast<int64_t>(h) * D + HALF);
-                turn.turn(low, high);
-                put_four(dst + static_cast<int64_t>(h) * D, low);
-                put_four(dst + static_cast<int64_t>(h) * D + HALF, high);
-            }
+            float4 low[HEADS], high[HEADS];
+#pragma unroll
+            for (int i = 0; i < HEADS; i++)
+                if (h0 + i < a.q_heads) {
+                    low[i] = four(src + static_cast<int64_t>(h0 + i) * D);
+                    high[i] = four(src + static_cast<int64_t>(h0 + i) * D + HALF);
+                }
+#pragma unroll
+            for (int i = 0; i < HEADS; i++)
+                if (h0 + i < a.q_heads) {
+                    const float4 x = low[i], y = high[i];
+                    put_four(dst + static_cast<int64_t>(h0 + i) * D,
+                             make_float4(fmaf(x.x, cl.x, -__fmul_rn(y.x, sl.x)), fmaf(x.y, cl.y, -__fmul_rn(y.y, sl.y)), fmaf(x.z, cl.z, -__fmul_rn(y.z, sl.z)), fmaf(x.w, cl.w, -__fmul_rn(y.w, sl.w))));
+                    put_four(dst + static_cast<int64_t>(h0 + i) * D + HALF,
+                             make_float4(fmaf(y.x, ch.x, __fmul_rn(x.x, sh.x)), fmaf(y.y, ch.y, __fmul_rn(x.y, sh.y)), fmaf(y.z, ch.z, __fmul_rn(x.z, sh.z)), fmaf(y.w, ch.w, __fmul_rn(x.w, sh.w))));
+                }
         }
         return;
     }
@@ -318,10 +330,7 @@ extern "C" int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rml
     a.q_heads = static_cast<int>(q_heads);
     a.q_out = q_out;
     a.status = status;
-    // queries in groups of up to eight heads, which share a token's rows of the tables; where a sequence has few tokens, of up to two
-    const bool few = !starts && s.each <= 256 / c.d;
-    a.q_parts = q ? static_cast<int>(ceil_div64(q_heads, few ? 2 : 8)) : 0;
-    a.parts = 2 * c.kv_heads + a.q_parts;
+    a.parts = 2 * c.kv_heads + (q ? static_cast<int>(ceil_div64(q_heads, 4)) : 0);
     // pages that the new tokens can fall into: of each sequence one more than their number less two, divided by the page size
     a.pages_each = (s.each + c.page - 2) / c.page + 1;
     const int64_t pieces = starts ? tokens / c.page + 2 * std::min<int64_t>(batch, tokens) : batch * a.pages_each;

@@ -25,6 +25,16 @@ def least_scale(amax: float) -> float:
     return 2.0 ** e
 
 
+def same_queries(got, want, q):
+    """Rotated queries against the exact ones.  The sine's product is rounded in fp32, half a step of it, and the sum, half a step of that; |cos|, |sin| <= 1, so the product is at most
+    the largest |q|, the sum twice that: 3 x 2^-24 of it.  want is the fp32 rounding of the exact sum: 2 x 2^-24 more.  f16: both are rounded, 2^-11 of the value each, 2^-25 among
+    the subnormal ones."""
+    f16 = q.dtype == torch.float16
+    got, want, q = got.double().cpu(), want.double().cpu(), q.double().cpu()
+    limit = 5 * 2.0 ** -24 * q.abs().amax(-1, keepdim=True) + (2 * 2.0 ** -11 * want.abs() + 2 * 2.0 ** -25 if f16 else 0)
+    assert bool(((got - want).abs() <= limit).all()), float((got - want).abs().max())
+
+
 def rotated(x, cos, sin):
     """x [heads, D], one position's rows of the tables: exact in 64 bits but for the last rounding of the sum, then one rounding to fp32."""
     half = x.shape[-1] // 2

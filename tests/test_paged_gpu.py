@@ -50,7 +50,8 @@ def test_append_token_by_token(cuda, page, d, kv, dtype):
         status = torch.zeros(1, dtype=torch.int32, device=cuda)
         out = K.paged_append(cache, k, v, lens, table, cos, sin, q=q, status=status)
         want, bad = plain.append(k, v, lens, table, cos, sin, q)
-        assert torch.equal(out.cpu(), want) and not bad and int(status) == 0
+        E.same_queries(out, want, q)
+        assert not bad and int(status) == 0
         plain.same(cache)
 
 
@@ -80,7 +81,7 @@ def test_append_prompts(cuda, page, d, kv, dtype, rotate):
     assert int(status) == 0 and not bad
     plain.same(cache)
     if rotate:
-        assert torch.equal(q_out[: int(starts[-1])].cpu(), want[: int(starts[-1])])
+        E.same_queries(q_out[: int(starts[-1])], want[: int(starts[-1])], q[: int(starts[-1])])
         assert bool((q_out[int(starts[-1]):] == 3).all())
 
 
@@ -146,7 +147,8 @@ def test_append_passes_over_what_has_no_place(cuda):
             K.paged_append(cache, k, v, lens, table, cos, sin, q=q, q_out=out, status=status)
             want, told = plain.append(k, v, lens, table, cos, sin, q)
             assert told == bad and int(status) == int(bad)
-            assert torch.equal(torch.isnan(out).cpu(), torch.isnan(want)) and torch.equal(torch.nan_to_num(out).cpu(), torch.nan_to_num(want))
+            assert torch.equal(torch.isnan(out).cpu(), torch.isnan(want))
+            E.same_queries(torch.nan_to_num(out), torch.nan_to_num(want), q)
             plain.same(cache)
 
 
@@ -403,9 +405,12 @@ def test_graphs_and_streams(cuda):
         for t in (q, k, v):
             t.copy_(torch.randn(t.shape, generator=g))
         graph.replay()
-        x, _ = plain.append(k, v, lens, table, cos, sin, q)
+        want, _ = plain.append(k, v, lens, table, cos, sin, q)
         plain.same(cache)
-        x = torch.nan_to_num(x.to(cuda))
+        written = ~torch.isnan(want).any(2)
+        x = K.paged_append(cache, k, v, lens, table, cos, sin, q=q)
+        E.same_queries(x.cpu()[written], want[written], q.cpu()[written])
+        x = torch.nan_to_num(x.masked_fill(~written.to(cuda)[..., None], 0.0))
         want, bound = E.attention(x, cache, lens, table, 0.125)
         E.close(out, want, bound)
 
@@ -434,7 +439,7 @@ def test_a_decoder_layer(cuda):
         y = K.paged_attention(q, cache, lens, table, d ** -0.5, starts=starts)
         out = K.matmul_i8(*K.quantize_rows(y.view(-1, heads * d)), *w_o)
         plain_q, _ = plain.append(qkv[:, heads: heads + kv], qkv[:, heads + kv:], lens, table, cos, sin, qkv[:, :heads], starts)
-        assert torch.equal(q.cpu(), plain_q)
+        E.same_queries(q, plain_q, qkv[:, :heads])
         plain.same(cache)
         want, bound = E.attention(q, cache, lens, table, d ** -0.5, starts)
         E.close(y, want, bound)
