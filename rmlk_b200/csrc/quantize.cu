@@ -3,57 +3,142 @@
 //   s = max(fl(max |x| / 127), 2^-126),   c = the integer nearest to x / s, ties to even.
 //
 // The codes are those of the real quotient.  fl(x / s) rounded to an integer is not: a quotient of size 100 keeps 17 bits behind the point, so of a
-// million values a few lie so near the middle between two integers that the division rounds onto it.  Here x times 1 / s gives the integer to within
-// one, and the sign of fma(-(c +- 1/2), s, x), which rounds once and so cannot change it, says on which side of the middle x is.
+// million values a few lie so near the middle between two integers that the division rounds onto it.  Here x times 1 / s, off by less than 4e-5, gives the integer, and where it
+// lies within 1e-4 of a middle the sign of fma(-(c +- 1/2), s, x), which rounds once and so cannot change it, says on which side x is.
 //
-// What bounds it: HBM, one read of x (4 or 2 bytes per element) and one byte written.  A row stays in registers between its maximum and its codes.
+// What bounds it: HBM, one read of x (4 or 2 bytes per element) and one byte written.  A row stays in registers between its maximum and its codes: a warp to a row of up to
+// 1024 values (2048 in f16), else a CTA; rows off 16-byte boundaries, and longer than a CTA's registers, are read twice.
+// [4096, 4096] f16: 28 us read twice and value by value.
 #include "common.cuh"
 
 namespace rmlk {
 namespace quant {
 
+struct RowScale {
+    float s, inv, up;  // of values times `up`
+    bool bad;
+    // from the largest magnitude's bits
+    __device__ __forceinline__ float set(uint32_t most) {
+        bad = most >= 0x7f800000u;
+        const float scale = fmaxf(__fdiv_rn(__uint_as_float(most), 127.f), 1.17549435e-38f);
+        up = scale < 7.888609052210118e-31f ? 16777216.f : 1.f;  // below 2^-100 differences would round to zero: all times 2^24
+        s = scale * up;
+        inv = __frcp_rn(s);
+        return bad ? __int_as_float(0x7fc00000) : scale;
+    }
+    __device__ __forceinline__ int code(float x) const {
+        const float v = x * up, sum = fmaf(v, inv, 12582912.f);  // 1.5 2^23: the sum is rounded to an integer
+        float c = sum - 12582912.f;
+        if (fabsf(fmaf(v, inv, -c)) > 0.4999f) {
+            const float above = fmaf(-(c + 0.5f), s, v), below = fmaf(-(c - 0.5f), s, v);
+            const bool odd = static_cast<int>(c) & 1;
+            if (above > 0.f || (above == 0.f && odd)) c += 1.f;
+            else if (below < 0.f || (below == 0.f && odd)) c -= 1.f;
+            return static_cast<int>(c);
+        }
+        return __float_as_int(sum);  // (its lowest byte)
+    }
+};
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+template <int GROUP>
+__device__ __forceinline__ uint32_t group_max(uint32_t m, uint32_t* s_max) {
+    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (GROUP > 32) {
+        if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < GROUP / 32; w++) m = max(m, s_max[w]);
+    }
+    return m;
+}
+
+// Rows on 16-byte boundaries, V values to a 16-byte load; GROUP threads to a row, ITERS loads to a thread.
+template <typename T, int GROUP, int ITERS>
+__global__ void __launch_bounds__(GROUP > 256 ? GROUP : 256) packs_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, int8_t* __restrict__ codes, int64_t ldc,
+                                                                         float* __restrict__ scales) {
+    dep_sync();
+    constexpr int V = 16 / sizeof(T), CTA = GROUP > 256 ? GROUP : 256;
+    __shared__ uint32_t s_max[GROUP / 32];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (CTA / GROUP) + threadIdx.x / GROUP;
+    if (row >= rows) return;  // (a whole warp; where a CTA has one row, never)
+    const int me = threadIdx.x % GROUP;
+    const T* xr = x + row * ldx;
+    Pack<T, V> p[ITERS];
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < ITERS; i++) {
+        const int at = (i * GROUP + me) * V;
+        if (at + V <= cols) {
+            p[i] = load_pack<T, V>(xr + at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) p[i].v[e] = at + e < cols ? xr[at + e] : static_cast<T>(0.f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITERS; i++)
+#pragma unroll
+        for (int e = 0; e < V; e++) most = max(most, magnitude(static_cast<float>(p[i].v[e])));
+    most = group_max<GROUP>(most, s_max);
+    RowScale r;
+    const float scale = r.set(most);
+    if (me == 0) scales[row] = scale;
+#pragma unroll
+    for (int i = 0; i < ITERS; i++) {
+        const int at = (i * GROUP + me) * V;
+        if (at >= cols) continue;
+        Pack<int8_t, V> c;
+#pragma unroll
+        for (int e = 0; e < V; e++) c.v[e] = r.bad ? 0 : static_cast<int8_t>(r.code(static_cast<float>(p[i].v[e])));
+        int8_t* to = codes + row * ldc + at;
+        if (at + V <= cols) {
+            store_pack<int8_t, V>(to, c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                if (at + e < cols) to[e] = c.v[e];
+        }
+    }
+}
+
+// Any rows: a CTA each, read twice.
 template <typename T>
 __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t cols, int8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scales) {
     dep_sync();
-    __shared__ float s_max[8];
-    __shared__ int s_bad[8];
+    __shared__ uint32_t s_max[8];
     const int64_t row = blockIdx.x;
     const T* xr = x + row * ldx;
-    float m = 0.f;
-    bool bad = false;
-    for (int64_t i = threadIdx.x; i < cols; i += 256) {
-        const float v = fabsf(static_cast<float>(xr[i]));
-        bad = bad || !(v < INFINITY);
-        m = fmaxf(m, v);
-    }
-    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-    const int any = __any_sync(0xffffffffu, bad);
-    if ((threadIdx.x & 31) == 0) {
-        s_max[threadIdx.x >> 5] = __uint_as_float(most);
-        s_bad[threadIdx.x >> 5] = any;
-    }
-    __syncthreads();
-    m = 0.f;
-    bad = false;
-#pragma unroll
-    for (int w = 0; w < 8; w++) {
-        m = fmaxf(m, s_max[w]);
-        bad = bad || s_bad[w];
-    }
-    float s = fmaxf(__fdiv_rn(m, 127.f), 1.17549435e-38f);
-    if (threadIdx.x == 0) scales[row] = bad ? __int_as_float(0x7fc00000) : s;
-    const float up24 = s < 7.888609052210118e-31f ? 16777216.f : 1.f;  // below 2^-100 differences would round to zero: all times 2^24
-    s *= up24;
-    const float inv = __frcp_rn(s);
-    for (int64_t i = threadIdx.x; i < cols; i += 256) {
-        const float v = static_cast<float>(xr[i]) * up24;
-        float c = rintf(v * inv);
-        const float up = fmaf(-(c + 0.5f), s, v), down = fmaf(-(c - 0.5f), s, v);
-        const bool odd = static_cast<int>(c) & 1;
-        if (up > 0.f || (up == 0.f && odd)) c += 1.f;
-        else if (down < 0.f || (down == 0.f && odd)) c -= 1.f;
-        codes[row * ldc + i] = bad ? 0 : static_cast<int8_t>(c);
-    }
+    uint32_t most = 0;
+    for (int64_t i = threadIdx.x; i < cols; i += 256) most = max(most, magnitude(static_cast<float>(xr[i])));
+    most = group_max<256>(most, s_max);
+    RowScale r;
+    const float scale = r.set(most);
+    if (threadIdx.x == 0) scales[row] = scale;
+    for (int64_t i = threadIdx.x; i < cols; i += 256) codes[row * ldc + i] = r.bad ? 0 : static_cast<int8_t>(r.code(static_cast<float>(xr[i])));
+}
+
+template <typename T, int GROUP, int ITERS>
+static void packs(cudaStream_t st, const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scales) {
+    constexpr int CTA = GROUP > 256 ? GROUP : 256;
+    launch_dep(packs_kernel<T, GROUP, ITERS>, dim3(static_cast<unsigned>(ceil_div64(rows, CTA / GROUP))), dim3(CTA), 0, st, x, ldx, rows, static_cast<int>(cols), codes, ldc, scales);
+}
+
+template <typename T>
+static void quantize(cudaStream_t st, const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes, int64_t ldc, float* scales) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t loads = ceil_div64(cols, V);
+    const bool whole = aligned_to(x, 16) && ldx % V == 0 && aligned_to(codes, V) && ldc % V == 0 && loads <= 512 * 8;
+    if (!whole) launch_dep(rows_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, st, x, ldx, cols, codes, ldc, scales);
+    else if (loads <= 32) packs<T, 32, 1>(st, x, ldx, rows, cols, codes, ldc, scales);
+    else if (loads <= 64) packs<T, 32, 2>(st, x, ldx, rows, cols, codes, ldc, scales);
+    else if (loads <= 256 && rows > 2 * sm_count()) packs<T, 32, 8>(st, x, ldx, rows, cols, codes, ldc, scales);  // (with few rows, more threads to each)
+    else if (loads <= 256) packs<T, 256, 1>(st, x, ldx, rows, cols, codes, ldc, scales);
+    else if (loads <= 512) packs<T, 256, 2>(st, x, ldx, rows, cols, codes, ldc, scales);
+    else if (loads <= 1024) packs<T, 256, 4>(st, x, ldx, rows, cols, codes, ldc, scales);
+    else if (loads <= 2048) packs<T, 512, 4>(st, x, ldx, rows, cols, codes, ldc, scales);
+    else packs<T, 512, 8>(st, x, ldx, rows, cols, codes, ldc, scales);
 }
 
 }  // namespace quant
@@ -69,12 +154,9 @@ extern "C" int rmlk_b200_quantize_rows(rmlk_stream_t stream, int dtype, int64_t 
     if (ldx < cols || ldc < cols) return fail(RMLK_ERR_INVALID_ARG, "quantize_rows: rows overlap");
     const size_t e = dtype_size(dtype);
     if (!aligned_to(x, e) || !aligned_to(scales, 4)) return fail(RMLK_ERR_INVALID_ARG, "quantize_rows: misaligned pointer");
-    if (dtype == RMLK_F32)
-        launch_dep(quant::rows_kernel<float>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, as_stream(stream), static_cast<const float*>(x), ldx, cols,
-                   static_cast<int8_t*>(codes), ldc, scales);
-    else
-        launch_dep(quant::rows_kernel<__half>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, as_stream(stream), static_cast<const __half*>(x), ldx, cols,
-                   static_cast<int8_t*>(codes), ldc, scales);
-    RMLK_CHECK_LAUNCH("quantize rows_kernel");
+    const cudaStream_t st = as_stream(stream);
+    if (dtype == RMLK_F32) quant::quantize(st, static_cast<const float*>(x), ldx, rows, cols, static_cast<int8_t*>(codes), ldc, scales);
+    else quant::quantize(st, static_cast<const __half*>(x), ldx, rows, cols, static_cast<int8_t*>(codes), ldc, scales);
+    RMLK_CHECK_LAUNCH("quantize_rows");
     return RMLK_OK;
 }
