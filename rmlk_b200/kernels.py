@@ -591,23 +591,27 @@ def quantize_rows(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales:
     largest magnitude over 127, a code the nearest integer to the real quotient.  Rows of the codes start on 16-byte boundaries, as matmul_i8
     wants them.  A row with an infinity or a NaN gets the scale NaN."""
     dev = _device_of("quantize_rows", x)
-    shape = x.shape
-    if len(shape) != 2 or x.dtype not in _FLOATS:
+    shape, code = x.shape, _FLOATS.get(x.dtype)
+    if len(shape) != 2 or code is None:
         raise _told("quantize_rows", dev, ("x", x, _FLOATS, (None, None), True))
     m, k = shape
     ldx = _rows_apart(x)
+    fits = ldx >= k
     if codes is None:
         ldc = (k + 15) // 16 * 16
         codes = x.new_empty((m, ldc), dtype=_I8)
         if ldc != k:
             codes = codes[:, :k]
     else:
-        ldc = _rows_apart(codes) if codes.dim() == 2 else 0
+        ldc = _rows_apart(codes) if codes.dim() == 2 else -1
+        fits = fits and ldc >= k and codes.shape == shape and codes.dtype is _I8 and codes.get_device() == dev
     if scales is None:
-        scales = x.new_empty(m, dtype=_F32)
-    if (ldx < k or ldc < k or codes.shape != shape or codes.dtype is not _I8 or codes.get_device() != dev or scales.shape != shape[:1] or not _dense(scales, _F32, dev)):
+        scales = x.new_empty(m) if code == dt.F32 else x.new_empty(m, dtype=_F32)
+    else:
+        fits = fits and scales.shape == shape[:1] and _dense(scales, _F32, dev)
+    if not fits:
         raise _told("quantize_rows", dev, ("x", x, _FLOATS, (m, k), True), ("codes", codes, _I8, (m, k), True), ("scales", scales, _F32, (m,), False))
-    _check(lib().rmlk_b200_quantize_rows(_stream_of(dev), _FLOATS[x.dtype], m, k, x.data_ptr(), ldx, codes.data_ptr(), ldc, scales.data_ptr()))
+    _check(lib().rmlk_b200_quantize_rows(_stream_of(dev), code, m, k, x.data_ptr(), ldx, codes.data_ptr(), ldc, scales.data_ptr()))
     return codes, scales
 
 
@@ -625,23 +629,25 @@ def matmul_i8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales
     """(x @ w.T) * x_scales[:, None] * w_scales for int8 codes x [m, k], w [n, k] (rows on 16-byte boundaries; k <= 131071): [m, n] of
     `dtype` (f32 or f16).  The sums are exact 32-bit integers."""
     dev = _device_of("matmul_i8", x)
-    xs, ws = x.shape, w.shape
-    if len(xs) != 2 or len(ws) != 2 or dtype not in _FLOATS:
+    xs, ws, code = x.shape, w.shape, _FLOATS.get(dtype)
+    if len(xs) != 2 or len(ws) != 2 or code is None:
         raise _told("matmul_i8", dev, ("x", x, _I8, (None, None), True), ("w", w, _I8, (None, None), True))
     m, k = xs
     n = ws[0]
+    ldx, ldw = _rows_apart(x), _rows_apart(w)
+    fits = (ws[1] == k and ldx >= k and ldw >= k and x.dtype is _I8 and w.dtype is _I8 and w.get_device() == dev and x_scales.shape == (m,) and w_scales.shape == (n,)
+            and _dense(x_scales, _F32, dev) and _dense(w_scales, _F32, dev) and (status is None or _dense(status, _I32, dev)))
     if out is None:
-        out = x.new_empty((m, n), dtype=dtype)
+        if fits:
+            out = x_scales.new_empty((m, n)) if code == dt.F32 else x.new_empty((m, n), dtype=dtype)
         ldo = n
     else:
         ldo = _rows_apart(out) if out.dim() == 2 else -1
-    ldx, ldw = _rows_apart(x), _rows_apart(w)
-    if (ws[1] != k or ldx < k or ldw < k or ldo < n or out.shape != (m, n) or out.dtype is not dtype or out.get_device() != dev or x.dtype is not _I8 or w.dtype is not _I8
-            or w.get_device() != dev or x_scales.shape != (m,) or w_scales.shape != (n,) or not _dense(x_scales, _F32, dev) or not _dense(w_scales, _F32, dev)
-            or (status is not None and not _dense(status, _I32, dev))):
+        fits = fits and ldo >= n and out.shape == (m, n) and out.dtype is dtype and out.get_device() == dev
+    if not fits:
         raise _told("matmul_i8", dev, ("x", x, _I8, (None, None), True), ("w", w, _I8, (None, k), True), ("out", out, dtype, (m, n), True), ("x_scales", x_scales, _F32, (m,), False),
                     ("w_scales", w_scales, _F32, (n,), False), ("status", status, _I32, (1,), False))
-    _check(lib().rmlk_b200_matmul_i8(_stream_of(dev), _FLOATS[dtype], m, n, k, x.data_ptr(), ldx, x_scales.data_ptr(), w.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(), ldo,
+    _check(lib().rmlk_b200_matmul_i8(_stream_of(dev), code, m, n, k, x.data_ptr(), ldx, x_scales.data_ptr(), w.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(), ldo,
                                      None if status is None else status.data_ptr()))
     return out
 
@@ -705,7 +711,7 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lens: torc
         fits = _dense(cos, _F32, dev) and _dense(sin, _F32, dev) and cos.shape == (rows, shape[3]) == sin.shape
     if fits and q is not None:
         if q_out is None:
-            q_out = q.new_empty(q.shape)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         heads = q.shape[1] if q.dim() == 3 else 0
         fits = q.dtype is dtype and q.shape == (tokens, heads, shape[3]) == q_out.shape and q_out.dtype is dtype and q.get_device() == dev and q_out.get_device() == dev
         if fits:
@@ -740,10 +746,12 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lens: torch.Tensor, tabl
     fits = len(qs) == 3 and dtype in _FLOATS and qs[2] == shape[3] and q.get_device() == dev
     ldq = ldo = 0
     if fits:
-        if out is None:
-            out = q.new_empty(qs)
         ldq = _rows_apart(q)
-        ldo = _rows_apart(out) if out.dim() == 3 else 0
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            ldo = qs[1] * qs[2]
+        else:
+            ldo = _rows_apart(out) if out.dim() == 3 else 0
         if workspace is None:
             workspace = paged_attention_workspace(q, cache, at[0], starts is not None)
         fits = ldq and ldo and out.shape == qs and out.dtype is dtype and out.get_device() == dev and workspace.is_contiguous() and workspace.get_device() == dev
