@@ -35,11 +35,11 @@ static int launch_prompt(cudaStream_t st, const Cache& c, const Batch& s, const 
     cudaError_t cfg_err = cudaSuccess;
     if (dev >= 0 && dev < 64) std::call_once(configured[dev], [&] { cfg_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL); });
     RMLK_CUDA(cfg_err);
-    constexpr int64_t ROWS = L::TILES * 128;
+    constexpr int64_t ROWS = L::ROWS;
     const int64_t tokens = s.tokens, batch = s.batch;
     const int64_t items = s.starts ? tokens * a.group / ROWS + std::min(batch, tokens) : batch * ceil_div64(s.each * a.group, ROWS);  // ragged: as many as there can be
-    if (items > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");
-    RMLK_CUDA(launch_dep(kernel, dim3(static_cast<unsigned>(items), c.kv_heads), dim3(L::THREADS), L::TOTAL, st, c, s, a));
+    if (items * c.kv_heads > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");
+    RMLK_CUDA(launch_dep(kernel, dim3(static_cast<unsigned>(items * c.kv_heads)), dim3(L::THREADS), L::TOTAL, st, c, s, a));
     RMLK_CHECK_LAUNCH("paged_attention prompt_kernel");
     return RMLK_OK;
 }
@@ -67,6 +67,7 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
     const int rc = paged::take("paged_attention", cache, tokens, batch, starts, lens, table, table_width, c, s);
     if (rc != RMLK_OK) return rc;
     if (q_heads < 1 || q_heads % c.kv_heads || q_heads / c.kv_heads > 64) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: q_heads must be a multiple of kv_heads, up to 64 for each");
+    if (tokens * (q_heads / c.kv_heads) >= (1ll << 31)) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");
     if (!(scale - scale == 0.f)) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the scale must be finite");
     if (tokens == 0 || batch == 0) return RMLK_OK;
     if (!q || !out) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: NULL pointer");

@@ -105,9 +105,11 @@ __device__ __forceinline__ float quad_sum(float x) {
     x += __shfl_xor_sync(0xffffffffu, x, 1);
     return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
-// a / b for 0 <= a, 0 < b: nearly always in 32 bits, where a division is a fifth of the instructions
+// a / b for 0 <= a, 0 < b: nearly always in 32 bits.  A 64-bit division is 2 KB of instructions: inlined wherever one may be needed, they made kernels of 100 KB, which do not
+// stay in the instruction cache.
+__device__ __noinline__ int64_t divide_64(int64_t a, int64_t b) { return a / b; }
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-    return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+    return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : divide_64(a, b);
 }
 
 // named barriers between two warps: one hands over and goes on, the other waits
