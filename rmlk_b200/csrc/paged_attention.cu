@@ -1,5 +1,6 @@
 // Attention over a paged cache of 8-bit codes (paged.cuh): softmax(scale q k^T) v, k and v = code times the scale of their page and head.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "paged_few.cuh"
@@ -49,12 +50,21 @@ static int launch_prompt(cudaStream_t st, const Cache& c, const Batch& s, const 
 
 using namespace rmlk;
 
-// Rows of a KV head (new tokens x query heads that share it) up to which few_kernel takes a call.
-constexpr int64_t FEW_ROWS = 64;
-static bool takes_few(int64_t tokens, int64_t batch, int64_t group, bool ragged) { return !ragged && batch > 0 && tokens / batch * group <= FEW_ROWS; }
+// Which kernel takes a call: few_kernel shares the keys out over all SMs and reads them once for each 16 query rows; prompt_kernel has a CTA to 128 rows, which reads all their
+// keys, and two CTAs to an SM.  With P = batch x kv_heads, few_kernel's time is that of P ceil(rows / 16) tiles spread over the GPU, prompt_kernel's that of one CTA as long
+// as every CTA has an SM, of 1.4 for every two CTAs per SM behind that; one CTA takes as long as 3.4 tiles per SM.  Measured with 8 KV heads over 8000 keys, us (few, prompt):
+//   f16 128: 1 x 64 rows 26, 175;  8 x 64 110, 186;  8 x 128 206, 189;  64 x 32 398, 504;  64 x 64 777, 506
+//   f32 64:  1 x 64 rows 21, 233;  8 x 128 146, 239;  8 x 256 280, 239;  64 x 32 281, 550;  64 x 64 546, 554
+// The new tokens of ragged sequences lie at places that only the device knows: they go to prompt_kernel.
+static bool takes_few(int64_t tokens, int64_t batch, int64_t kv_heads, int64_t group, bool ragged) {
+    if (ragged || batch < 1) return false;
+    const double sms = sm_count(), rows = static_cast<double>(tokens / batch) * group, problems = static_cast<double>(batch) * kv_heads;
+    const double ctas = problems * std::ceil(rows / 128.0), alone = ctas <= sms ? 1.0 : 1.4 * std::ceil(ctas / (2.0 * sms));
+    return problems * std::ceil(rows / 16.0) <= 3.4 * sms * alone;
+}
 
 extern "C" size_t rmlk_b200_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int ragged) {
-    if (kv_heads < 1 || q_heads < kv_heads || !takes_few(tokens, batch, q_heads / kv_heads, ragged != 0)) return 0;
+    if (kv_heads < 1 || q_heads < kv_heads || !takes_few(tokens, batch, kv_heads, q_heads / kv_heads, ragged != 0)) return 0;
     return paged::few_workspace(head_dim);
 }
 
@@ -76,7 +86,7 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
     if (!aligned_to(q, 16) || !aligned_to(out, 16) || q_stride % per || out_stride % per) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: rows must lie on 16-byte boundaries");
     paged::Attend a = {q, out, q_stride, out_stride, static_cast<int>(q_heads), static_cast<int>(q_heads / c.kv_heads), scale, status};
     const cudaStream_t st = as_stream(stream);
-    if (takes_few(tokens, batch, a.group, starts != nullptr)) {
+    if (takes_few(tokens, batch, c.kv_heads, a.group, starts != nullptr)) {
         if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
             return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
         const bool one = s.each * a.group <= 8;

@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                 uint32_t p[NR][NC][L::DIGITS];
 #pragma unroll
                 for (int n = 0; n < NC; n++) {
-                    const float v = scales[stage * NC + n].y, k = passes > 1 ? (n == pass ? MOST : 0.f) : v == ref ? MOST : v * per;
+                    // (a page whose scale is not finite: its weights are 0, or the row is NaN already)
+                    const float v = scales[stage * NC + n].y, k = passes > 1 ? (n == pass ? MOST : 0.f) : v == ref ? MOST : v < INFINITY ? v * per : 0.f;
 #pragma unroll
                     for (int r = 0; r < NR; r++) {
                         // the lower bits of 2^23 + a number below 2^23 are that number

@@ -1,14 +1,15 @@
 // Attention of many query rows per KV head over the paged 8-bit cache: prompts, parts of them behind a cached beginning.
 //
-// A CTA keeps 128 query rows of one KV head (the rows of the query heads that share it lie behind one another) and walks over the keys that they see in blocks of 128
-// (fp32: 64).  Both contractions run on tcgen05.mma kind::f16: codes are exact in f16, f16 queries too; fp32 queries and, for fp32 results, weights are two f16 numbers each
-// (the second the rounding error of the first), whose products go to the same accumulator.
-//   warps 0-3   softmax, one thread to a row: scores out of TMEM, weights back into TMEM, where the values' MMAs take them as their first operand.  One thread issues the MMAs: the
-//               values of block j and, right behind, the scores of block j + 1.
-//   warps 4-7   codes of K and V from the pages into f16 tiles; those of the next block are asked for as soon as a block's are put down
-// A CTA's chain - scores, softmax, values - has no overlap of its own; two CTAs share an SM and overlap theirs.  (One CTA of two tiles with scores a block ahead, weights in shared
-// memory and blocks of 64: its MMAs, each 128 x 64 x 16, read their first operand from shared memory at the same rate and were the bound, 445 us for what takes @@ now.)
-// What bounds it: the MMAs and the exponentials (16 per clock and SM) are each about half of a block's time, and what two CTAs do not overlap.
+// A CTA keeps 128 query rows of one KV head (the rows of the query heads that share it lie behind one another) and walks over the keys that they see in blocks of
+// 64.  Both contractions run on tcgen05.mma kind::f16: codes are exact in f16, f16 queries too; fp32 queries and, for fp32 results, weights are two f16 numbers each (the
+// second the rounding error of the first), whose products go to the same accumulator.
+//   warps 0-3   softmax, one thread to a row: scores out of TMEM, weights back into TMEM in their place, where the values' MMAs take them as their first operand
+//   warps 4-6   codes of K and V from the pages into f16 tiles, two of each
+//   warp 7      one thread issues the MMAs: values of block j, scores of block j + 2 in the place of the weights
+// so that a softmax finds its scores ready.  Two CTAs share an SM.
+// What was tried: one CTA of two tiles per SM with the weights in shared memory, 445 us for 4 x 1024 tokens of 32 heads of 128 behind 5000 keys (its one MMA thread was the bound); blocks of 128
+// keys whose scores come only when the values of the block before are on their way, 433 us (half of a CTA's time is MMAs, during which its softmax waits); this one @@.
+// What bounds it: the MMAs of the scores (128 x 64 x 16 each, which read their first operand from shared memory at the rate of the second), and the softmax warps' chain of latencies.
 // The output sums stay in TMEM.  They are brought under a new maximum only when a row's has grown by more than 2^8 (weights are up to 2^14 then), which after the first
 // blocks hardly happens.  For fp32 results they are added to fp32 sums every four blocks: the accumulator truncates, and 256 keys are what its error allows.
 // Scales of K go into the scores' factor, scales of V into the weights, relative to the largest that the rows see.  Where scales of V span more than 2^10, or
@@ -49,15 +50,15 @@ struct Prompt {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int D = D_, HALVES = D / 64;  // tiles of 64 dims: 128-byte rows of f16
     static constexpr int ROWS = 128, PARTS = F32 ? 2 : 1;  // f16 numbers of a query or weight
-    static constexpr int KT = F32 ? 64 : 128, GROUPS = KT / 16;  // keys of a block; 16 of them have a page
-    static constexpr int THREADS = 256;
+    static constexpr int KT = 64, GROUPS = KT / 16;  // keys of a block; 16 of them have a page
+    static constexpr int THREADS = 256, MAKERS = 96;
     static constexpr uint32_t Q_HALF = ROWS * 128, Q_TILE = Q_HALF * HALVES, KV_HALF = KT * 128, KV_TILE = KV_HALF * HALVES;
-    static constexpr uint32_t Q = 0, K = PARTS * Q_TILE, V = K + KV_TILE, ROW_SCALE = V + KV_TILE, RED = ROW_SCALE + ROWS * 4, BARS = RED + 64, TOTAL = BARS + 64 + 1024;
-    // TMEM columns: scores, weights (two keys to a column), sums, (fp32) kept sums.  f16 with 128 values: weights take the place of scores that have been read.
-    static constexpr uint32_t P_AT = F32 ? 64 : D == 64 ? 128 : 0, O_AT = F32 ? 128 : D == 64 ? 192 : 128, KEPT = D, COLS = F32 && D == 128 ? 512 : 256;
+    static constexpr uint32_t Q = 0, K = PARTS * Q_TILE, V = K + 2 * KV_TILE, ROW_SCALE = V + 2 * KV_TILE, RED = ROW_SCALE + ROWS * 4, BARS = RED + 64, TOTAL = BARS + 128 + 1024;
+    // TMEM columns: two places for scores (64 columns) and the weights made of them (two keys to a column; fp32: the second numbers behind the first), sums, (fp32) kept sums
+    static constexpr uint32_t O_AT = 128, KEPT = D, COLS = F32 && D == 128 ? 512 : 256;
     static constexpr int PER_SM = COLS == 512 ? 1 : 2;
     static constexpr int FLUSH = 4;  // (fp32) blocks per accumulation
-    static_assert(TOTAL <= 113 * 1024, "shared memory budget exceeded");
+    static_assert(TOTAL <= (PER_SM == 2 ? 113 : 227) * 1024, "shared memory budget exceeded");
 };
 
 // One query row by one warp, a key after the other, in fp32: any scales, NaN for what is not finite and for a key without a page.
@@ -162,11 +163,15 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
     uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
     float* s_row = reinterpret_cast<float*>(sm + L::ROW_SCALE);
     volatile uint32_t* s_red = reinterpret_cast<volatile uint32_t*>(sm + L::RED);
-    // Barriers: keys in place, values in place, and one that completes with the scores of block j: with them, since MMAs finish in the order in which they are issued, the values of
-    // block j - 1 have been added, the keys of block j and the values and weights of block j - 1 are done with.
-    const uint32_t k_full = base + L::BARS, v_full = k_full + 8, done = k_full + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::BARS + 24);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::BARS + 32);
+    // barriers: keys and values in place and done with (two places each), scores there (two places), weights there, values of a block added
+    const uint32_t bars = base + L::BARS, p_full = bars + 80, o_done = bars + 88;
+    auto k_full = [&](int i) { return bars + 8u * i; };
+    auto k_free = [&](int i) { return bars + 8u * (2 + i); };
+    auto v_full = [&](int i) { return bars + 8u * (4 + i); };
+    auto v_free = [&](int i) { return bars + 8u * (6 + i); };
+    auto s_full = [&](int i) { return bars + 8u * (8 + i); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::BARS + 96);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::BARS + 104);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // ---- which rows: sequence by sequence, the tiles that see most first ----
@@ -240,9 +245,15 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             s_red[2 * warp + 1] = l;
         }
         if (tid == 0) {
-            mbar_init(k_full, 128);
-            mbar_init(v_full, 128);
-            mbar_init(done, 1);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(k_full(i), L::MAKERS);
+                mbar_init(k_free(i), 1);
+                mbar_init(v_full(i), L::MAKERS);
+                mbar_init(v_free(i), 1);
+                mbar_init(s_full(i), 1);
+            }
+            mbar_init(p_full, 128);
+            mbar_init(o_done, 1);
             *abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -273,39 +284,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
     int* status = a.status;
 
     // ---- queries ----
-    // Codes of K and V: 16-byte pieces of a key, a thread always the same piece of keys own_key + i STEP.
-    constexpr int PIECES = D / 16, N = KT * PIECES / 128, STEP = 128 / PIECES;
-    const int me = tid & 127, own_key = me / PIECES, piece = me % PIECES;
-    const int64_t head = static_cast<int64_t>(h) * c.page * D + piece * 16, page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
-    int page[N];
-    uint4 kx[N], vx[N];
-    auto look_up = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int key = j * KT + own_key + i * STEP;
-            page[i] = key < seen ? table[key >> c.page_log] : -1;
-        }
-    };
-    auto load = [&](const int8_t* codes, int j, uint4 (&x)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            x[i] = make_uint4(0u, 0u, 0u, 0u);  // (keys that no row sees)
-            if (page[i] >= 0)
-                x[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(page[i]) * page_bytes + head + ((j * KT + own_key + i * STEP) & (c.page - 1)) * D);
-        }
-    };
-    auto put = [&](uint32_t tile, const uint4 (&x)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int r = own_key + i * STEP, u = 2 * (piece & 3);
-            uint8_t* to = sm + tile + (piece >> 2) * L::KV_HALF;
-            *reinterpret_cast<uint4*>(to + swizzled(r, u)) = eight_f16(x[i].x, x[i].y);
-            *reinterpret_cast<uint4*>(to + swizzled(r, u + 1)) = eight_f16(x[i].z, x[i].w);
-        }
-        fence_proxy_async();
-    };
-
-    // ---- queries; the first keys and values ----
+    // ---- queries ----
     if (warp < 4) {
         constexpr int PER = D / 4, AT_ONCE = 32 / PER, BATCH = 8;  // lanes to a row (four values each), rows of a warp at a time, loads on their way
         using Four = typename std::conditional<L::F32, float4, uint2>::type;
@@ -348,16 +327,6 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             }
         }
         fence_proxy_async();
-    } else {
-        look_up(0);
-        load(c.k, 0, kx);
-        load(c.v, 0, vx);
-        look_up(1);
-        put(L::K, kx);
-        put(L::V, vx);
-        load(c.k, 1, kx);
-        load(c.v, 1, vx);
-        look_up(2);
     }
     tc_fence_before();
     __syncthreads();
@@ -367,35 +336,11 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
     if (warp < 4) {
         // ---------------- softmax ----------------
         const int r = tid;
-        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, s_at = tmem + lanes, p_at = tmem + lanes + L::P_AT, o_at = tmem + lanes + L::O_AT;
+        const uint32_t at = tmem + (static_cast<uint32_t>(warp * 32) << 16), o_at = at + L::O_AT;
         const int sees = r < rows ? sees_of(row0 + r) : 0, least = sees_of(row0);  // least: what every row sees
         const float q_scale = fabsf(a.scale) * 1.44269504f * (L::F32 ? s_row[r] : 1.f);
         const float v_inv = 1.f / v_top;
-        // lower halves of the operands' descriptors: address / 16, and for the values the distance between blocks of 64 dims
-        const uint32_t q_desc = (base + L::Q) >> 4 | 1u << 16, k_desc = (base + L::K) >> 4 | 1u << 16, v_desc = (base + L::V) >> 4 | (L::KV_HALF >> 4) << 16;
-        constexpr uint32_t qk = (1u << 4) | ((KT >> 3) << 17) | ((128 >> 4) << 24), pv = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);  // (values: keys along the rows)
-        auto issue_scores = [&]() {
-#pragma unroll
-            for (int part = PARTS - 1; part >= 0; part--)  // the small products first
-#pragma unroll
-                for (int half = 0; half < HALVES; half++)
-#pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        mma_ss(tmem, q_desc + ((part * L::Q_TILE + half * L::Q_HALF) >> 4) + kk * 2, k_desc + ((half * L::KV_HALF) >> 4) + kk * 2, qk,
-                               part < PARTS - 1 || half > 0 || kk > 0);
-        };
-        auto issue_values = [&](bool add) {
-#pragma unroll
-            for (int part = PARTS - 1; part >= 0; part--)
-#pragma unroll
-                for (int kk = 0; kk < KT / 16; kk++) mma_ts(tmem + L::O_AT, tmem + L::P_AT + part * (KT / 2) + kk * 8, v_desc + kk * 128, pv, part < PARTS - 1 || kk > 0 ? 1u : add);
-        };
-        if (tid == 0) {
-            issue_scores();
-            umma::commit<1>(done);
-        }
         float top = -INFINITY, sum = 0.f;
-        uint32_t phase = 0;
         bool ok = true, fresh = true;  // fresh: nothing kept yet (fp32)
         int in_run = 0;                // (fp32) blocks since the sums were last added up
         // scales of 16 keys each: lanes look up pages two blocks ahead, scales one
@@ -427,29 +372,26 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             page_of(j + 2);
             const bool hidden = (j + 1) * KT > least;
             const int see = sees - j * KT;
-            ok = __all_sync(0xffffffffu, mbar_wait(done, phase, abort_flag, status));
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full(j & 1), (j >> 1) & 1, abort_flag, status));
             if (!ok) break;
-            phase ^= 1;
             tc_fence_after();
-            // ---- the largest score ----
+            const uint32_t s_at = at + (j & 1) * KT;
+            float x[KT];
+            tmem_ld_x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(x));
+            tmem_ld_x32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+            tmem_wait_ld();
+            if (hidden) {
+#pragma unroll
+                for (int i = 0; i < KT; i++)
+                    if (i >= see) x[i] = -INFINITY;
+            }
             float most = -INFINITY;
 #pragma unroll
-            for (int c0 = 0; c0 < KT; c0 += 32) {
-                float s[32];
-                tmem_ld_x32(s_at + c0, *reinterpret_cast<uint32_t(*)[32]>(s));
-                tmem_wait_ld();
-                if (hidden) {
+            for (int n = 0; n < GROUPS; n++) {
+                float m = x[16 * n];
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (c0 + i >= see) s[i] = -INFINITY;
-                }
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    float m = s[16 * n];
-#pragma unroll
-                    for (int i = 1; i < 16; i++) m = fmaxf(m, s[16 * n + i]);
-                    most = fmaxf(most, m * f_of(c0 / 16 + n));
-                }
+                for (int i = 1; i < 16; i++) m = fmaxf(m, x[16 * n + i]);
+                most = fmaxf(most, m * f_of(n));
             }
             // The maximum that the sums are under moves when it has fallen behind by more than 2^8.
             const bool move = most > top + 8.f || (top == -INFINITY && most > top);
@@ -459,58 +401,56 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             top = new_top;
             sum *= corr;
             const float shift = (top == -INFINITY ? 0.f : top) - 6.f;  // weights are 2^6 exp2(s - top)
-            // ---- weights, 32 keys at a time ----
             float2 part = make_float2(0.f, 0.f);
             const float2 shift2 = make_float2(-shift, -shift);
 #pragma unroll
-            for (int ch = 0; ch < KT / 32; ch++) {
-                float x[32];
-                tmem_ld_x32(s_at + 32 * ch, *reinterpret_cast<uint32_t(*)[32]>(x));
-                tmem_wait_ld();
-                if (hidden) {
+            for (int n = 0; n < GROUPS; n++) {
+                const float f = f_of(n);
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (32 * ch + i >= see) x[i] = -INFINITY;
-                }
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    const float f = f_of(2 * ch + n);
-#pragma unroll
-                    for (int i = 16 * n; i < 16 * n + 16; i += 2) {
-                        float2 y = fma2(make_float2(x[i], x[i + 1]), make_float2(f, f), shift2);
-                        y.x = ex2(y.x);
-                        y.y = ex2(y.y);
-                        part = add2(part, y);
-                        x[i] = y.x;
-                        x[i + 1] = y.y;
-                    }
-                }
-                if (!even) {
-#pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        const float v = __shfl_sync(0xffffffffu, vs, 2 * ch + n);
-#pragma unroll
-                        for (int i = 16 * n; i < 16 * n + 16; i++) x[i] *= v;
-                    }
-                }
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    w[i] = pack_f16(x[2 * i], x[2 * i + 1]);
-                    if constexpr (L::F32) {
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                        x[2 * i] -= back.x;
-                        x[2 * i + 1] -= back.y;
-                    }
-                }
-                tc::tmem_st_x16(p_at + 16 * ch, w);
-                if constexpr (L::F32) {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) w[i] = pack_f16(x[2 * i], x[2 * i + 1]);
-                    tc::tmem_st_x16(p_at + KT / 2 + 16 * ch, w);
+                for (int i = 16 * n; i < 16 * n + 16; i += 2) {
+                    float2 y = fma2(make_float2(x[i], x[i + 1]), make_float2(f, f), shift2);
+                    y.x = ex2(y.x);
+                    y.y = ex2(y.y);
+                    part = add2(part, y);
+                    x[i] = y.x;
+                    x[i + 1] = y.y;
                 }
             }
             sum += part.x + part.y;
+            if (!even) {
+#pragma unroll
+                for (int n = 0; n < GROUPS; n++) {
+                    const float v = __shfl_sync(0xffffffffu, vs, n);
+#pragma unroll
+                    for (int i = 16 * n; i < 16 * n + 16; i++) x[i] *= v;
+                }
+            }
+#pragma unroll
+            for (int ch = 0; ch < 2; ch++) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float(&y)[2] = *reinterpret_cast<float(*)[2]>(x + 32 * ch + 2 * i);
+                    w[i] = pack_f16(y[0], y[1]);
+                    if constexpr (L::F32) {
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                        y[0] -= back.x;
+                        y[1] -= back.y;
+                    }
+                }
+                tc::tmem_st_x16(s_at + 16 * ch, w);
+                if constexpr (L::F32) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) w[i] = pack_f16(x[32 * ch + 2 * i], x[32 * ch + 2 * i + 1]);
+                    tc::tmem_st_x16(s_at + 32 + 16 * ch, w);
+                }
+            }
+            // The values of the block before have been added: the sums can be touched.  (And the MMA thread has seen the weights before these: p_full is never two ahead of it.)
+            if (j > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, abort_flag, status));
+                if (!ok) break;
+                tc_fence_after();
+            }
             // ---- the sums under the new maximum; (fp32) added to those that are kept ----
             if constexpr (L::F32) {
                 if (j > 0 && (any || ++in_run == L::FLUSH)) {
@@ -544,20 +484,10 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             }
             tmem_wait_st();
             tc_fence_before();
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // all weights are there
-            if (tid == 0) {
-                tc_fence_after();
-                ok = mbar_wait(v_full, j & 1, abort_flag, status);
-                if (ok) issue_values(j > 0);
-                if (j + 1 < blocks) {
-                    ok = ok && mbar_wait(k_full, j & 1, abort_flag, status);
-                    if (ok) issue_scores();
-                }
-                if (ok) umma::commit<1>(done);
-            }
+            mbar_arrive(p_full);
         }
         // ---- results ----
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(done, phase, abort_flag, status));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (blocks - 1) & 1, abort_flag, status));
         tc_fence_after();
         const float inv = 1.f / sum * v_top;
         const int row = row0 + r, token = token_of(row);
@@ -592,22 +522,103 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             }
         }
         tc_fence_before();
-    } else {
-        // ---------------- codes to f16 tiles, from block 1 on ----------------
-        mbar_arrive(v_full);  // block 0: in place before the barrier above
+    } else if (warp < 7) {
+        // ---------------- codes to f16 tiles: 16-byte pieces of a key, a thread always the same piece, of keys own_key + i STEP ----------------
+        constexpr int PIECES = D / 16, STEP = L::MAKERS / PIECES, N = (KT + STEP - 1) / STEP;
+        const int me = tid - 128, own_key = me / PIECES, piece = me % PIECES;
+        const int64_t head = static_cast<int64_t>(h) * c.page * D + piece * 16, page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
+        int page[N];
+        uint4 kx[N], vx[N];
+        auto look_up = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int at = own_key + i * STEP, key = j * KT + at;
+                page[i] = at < KT && key < seen ? table[key >> c.page_log] : -1;
+            }
+        };
+        auto load = [&](const int8_t* codes, int j, uint4 (&x)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                x[i] = make_uint4(0u, 0u, 0u, 0u);  // (keys that no row sees)
+                if (page[i] >= 0)
+                    x[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(page[i]) * page_bytes + head + ((j * KT + own_key + i * STEP) & (c.page - 1)) * D);
+            }
+        };
+        auto put = [&](uint32_t tile, const uint4 (&x)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int r = own_key + i * STEP, u = 2 * (piece & 3);
+                if (r < KT) {
+                    uint8_t* to = sm + tile + (piece >> 2) * L::KV_HALF;
+                    *reinterpret_cast<uint4*>(to + swizzled(r, u)) = eight_f16(x[i].x, x[i].y);
+                    *reinterpret_cast<uint4*>(to + swizzled(r, u + 1)) = eight_f16(x[i].z, x[i].w);
+                }
+            }
+            fence_proxy_async();
+        };
+        look_up(0);
+        load(c.k, 0, kx);
+        load(c.v, 0, vx);
+        look_up(1);
         bool ok = true;
-        for (int j = 1; j < blocks; j++) {
-            ok = mbar_wait(done, (j - 1) & 1, abort_flag, status);  // scores of block j - 1: its keys are done with
+#pragma unroll 1
+        for (int j = 0; j < blocks; j++) {
+            const int i = j & 1;
+            const uint32_t parity = ((j >> 1) & 1) ^ 1;  // (the first use of a place goes through)
+            ok = mbar_wait(k_free(i), parity, abort_flag, status);
             if (!ok) break;
-            put(L::K, kx);
-            mbar_arrive(k_full);
+            put(L::K + i * L::KV_TILE, kx);
+            mbar_arrive(k_full(i));
             load(c.k, j + 1, kx);
-            ok = mbar_wait(done, j & 1, abort_flag, status);  // scores of block j: values of block j - 1 are
+            ok = mbar_wait(v_free(i), parity, abort_flag, status);
             if (!ok) break;
-            put(L::V, vx);
-            mbar_arrive(v_full);
+            put(L::V + i * L::KV_TILE, vx);
+            mbar_arrive(v_full(i));
             load(c.v, j + 1, vx);
             look_up(j + 2);
+        }
+    } else if (lane == 0) {
+        // ---------------- MMAs ----------------
+        // lower halves of the operands' descriptors: address / 16, and for the values the distance between blocks of 64 dims
+        const uint32_t q_desc = (base + L::Q) >> 4 | 1u << 16, k_desc = (base + L::K) >> 4 | 1u << 16, v_desc = (base + L::V) >> 4 | (L::KV_HALF >> 4) << 16;
+        constexpr uint32_t qk = (1u << 4) | ((KT >> 3) << 17) | ((128 >> 4) << 24), pv = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);  // (values: keys along the rows)
+        bool ok = true;
+        auto scores = [&](int j) {
+            const int i = j & 1;
+            ok = ok && mbar_wait(k_full(i), (j >> 1) & 1, abort_flag, status);
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t kd = k_desc + i * (L::KV_TILE >> 4), d = tmem + i * KT;
+#pragma unroll
+            for (int part = PARTS - 1; part >= 0; part--)  // the small products first
+#pragma unroll
+                for (int half = 0; half < HALVES; half++)
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++)
+                        mma_ss(d, q_desc + ((part * L::Q_TILE + half * L::Q_HALF) >> 4) + kk * 2, kd + ((half * L::KV_HALF) >> 4) + kk * 2, qk, part < PARTS - 1 || half > 0 || kk > 0);
+            umma::commit<1>(s_full(i));
+            umma::commit<1>(k_free(i));
+        };
+#pragma unroll 1
+        for (int j = -2; j < blocks && ok; j++) {
+            if (j >= 0) {
+                const int i = j & 1;
+                ok = mbar_wait(v_full(i), (j >> 1) & 1, abort_flag, status) && mbar_wait(p_full, j & 1, abort_flag, status);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int part = PARTS - 1; part >= 0; part--)
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++)
+                        mma_ts(tmem + L::O_AT, tmem + i * KT + part * 32 + kk * 8, v_desc + i * (L::KV_TILE >> 4) + kk * 128, pv, part < PARTS - 1 || kk > 0 ? 1u : j > 0);
+                umma::commit<1>(o_done);
+                umma::commit<1>(v_free(i));
+            }
+            if (j + 2 < blocks) {
+                // in the place of the weights that the MMAs just issued read.  (Their softmax has the scores of block j + 1 meanwhile.)
+                if (j >= 0) ok = mbar_wait(o_done, j & 1, abort_flag, status);
+                scores(j + 2);
+            }
         }
     }
     tc_fence_before();
