@@ -1,15 +1,15 @@
 // Attention of many query rows per KV head over the paged 8-bit cache: prompts, parts of them behind a cached beginning.
 //
-// A CTA keeps 128 query rows of one KV head (the rows of the query heads that share it lie behind one another) and walks over the keys that they see in blocks of
-// 64.  Both contractions run on tcgen05.mma kind::f16: codes are exact in f16, f16 queries too; fp32 queries and, for fp32 results, weights are two f16 numbers each (the
-// second the rounding error of the first), whose products go to the same accumulator.
-//   warps 0-3   softmax, one thread to a row: scores out of TMEM, weights back into TMEM in their place, where the values' MMAs take them as their first operand
-//   warps 4-6   codes of K and V from the pages into f16 tiles, two of each
-//   warp 7      one thread issues the MMAs: values of block j, scores of block j + 2 in the place of the weights
-// so that a softmax finds its scores ready.  Two CTAs share an SM.
-// What was tried: one CTA of two tiles per SM with the weights in shared memory, 445 us for 4 x 1024 tokens of 32 heads of 128 behind 5000 keys (its one MMA thread was the bound); blocks of 128
-// keys whose scores come only when the values of the block before are on their way, 433 us (half of a CTA's time is MMAs, during which its softmax waits); this one @@.
-// What bounds it: the MMAs of the scores (128 x 64 x 16 each, which read their first operand from shared memory at the rate of the second), and the softmax warps' chain of latencies.
+// A CTA keeps two tiles (fp32 with 128 values: one) of 128 query rows of one KV head - the rows of the query heads that share it lie behind one another - and walks over the
+// keys that they see in blocks of 64.  Both contractions run on tcgen05.mma kind::f16: codes are exact in f16, f16 queries too; fp32 queries and, for fp32 results, weights are two
+// f16 numbers each (the second the rounding error of the first), whose products go to the same accumulator.
+//   warps 0-3, 4-7   softmax of a tile, one thread to a row: scores out of TMEM, weights back into TMEM in their place, where the values' MMAs take them as their first operand
+//   warps 8-11       codes of K and V from the pages into f16 tiles, three of each: the codes are turned once for both tiles
+//   warps 12, 13     one thread of each issues the MMAs of the scores, up to two blocks ahead of the softmax, and those of the values
+// What was tried, 4 x 1024 tokens of 32 heads of 128 behind 5000 keys: one thread for all MMAs and the weights through shared memory 445 us (the thread needs some 70 cycles per MMA: it
+// was the bound); two CTAs of one tile per SM, blocks of 128 keys with the scores behind the values 433 us (half of a CTA's time is MMAs, during which its softmax waits), blocks
+// of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); this one @@.
+// What bounds it: @@
 // The output sums stay in TMEM.  They are brought under a new maximum only when a row's has grown by more than 2^8 (weights are up to 2^14 then), which after the first
 // blocks hardly happens.  For fp32 results they are added to fp32 sums every four blocks: the accumulator truncates, and 256 keys are what its error allows.
 // Scales of K go into the scores' factor, scales of V into the weights, relative to the largest that the rows see.  Where scales of V span more than 2^10, or
@@ -49,16 +49,19 @@ template <typename T, int D_>
 struct Prompt {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int D = D_, HALVES = D / 64;  // tiles of 64 dims: 128-byte rows of f16
-    static constexpr int ROWS = 128, PARTS = F32 ? 2 : 1;  // f16 numbers of a query or weight
-    static constexpr int KT = 64, GROUPS = KT / 16;  // keys of a block; 16 of them have a page
-    static constexpr int THREADS = 256, MAKERS = 96;
-    static constexpr uint32_t Q_HALF = ROWS * 128, Q_TILE = Q_HALF * HALVES, KV_HALF = KT * 128, KV_TILE = KV_HALF * HALVES;
-    static constexpr uint32_t Q = 0, K = PARTS * Q_TILE, V = K + 2 * KV_TILE, ROW_SCALE = V + 2 * KV_TILE, RED = ROW_SCALE + ROWS * 4, BARS = RED + 64, TOTAL = BARS + 128 + 1024;
-    // TMEM columns: two places for scores (64 columns) and the weights made of them (two keys to a column; fp32: the second numbers behind the first), sums, (fp32) kept sums
-    static constexpr uint32_t O_AT = 128, KEPT = D, COLS = F32 && D == 128 ? 512 : 256;
-    static constexpr int PER_SM = COLS == 512 ? 1 : 2;
+    static constexpr int TILES = F32 && D == 128 ? 1 : 2, ROWS = 128 * TILES;  // (fp32 sums twice, in TMEM: room for one tile of 128 values)
+    static constexpr int PARTS = F32 ? 2 : 1;              // f16 numbers of a query or weight
+    static constexpr int KT = 64, GROUPS = KT / 16;        // keys of a block; 16 of them have a page
+    static constexpr int MAKERS = 128, THREADS = ROWS + MAKERS + 64;
+    static constexpr int NBUF = 3;                         // blocks of keys, and of values, in shared memory
+    static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = Q_HALF * HALVES, KV_HALF = KT * 128, KV_TILE = KV_HALF * HALVES;
+    static constexpr uint32_t Q = 0, K = TILES * PARTS * Q_TILE, V = K + NBUF * KV_TILE, ROW_SCALE = V + NBUF * KV_TILE, RED = ROW_SCALE + ROWS * 4, BARS = RED + 128,
+                              TOTAL = BARS + 256 + 1024;
+    // TMEM columns: for each tile two places for scores (64 columns) and the weights made of them (two keys to a column; fp32: the second numbers behind the first), sums and (fp32)
+    // kept sums
+    static constexpr uint32_t O_AT = 256, O_PITCH = 128, KEPT = D;
     static constexpr int FLUSH = 4;  // (fp32) blocks per accumulation
-    static_assert(TOTAL <= (PER_SM == 2 ? 113 : 227) * 1024, "shared memory budget exceeded");
+    static_assert(TOTAL <= 227 * 1024, "shared memory budget exceeded");
 };
 
 // One query row by one warp, a key after the other, in fp32: any scales, NaN for what is not finite and for a key without a page.
@@ -154,24 +157,27 @@ __device__ __forceinline__ uint4 eight_f16(uint32_t w0, uint32_t w1) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) prompt_kernel(const Cache c, const Batch q, const Attend a) {
+__global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const Cache c, const Batch q, const Attend a) {
     using L = Prompt<T, D>;
-    constexpr int HALVES = L::HALVES, PARTS = L::PARTS, KT = L::KT, ROWS = L::ROWS, GROUPS = L::GROUPS;
+    constexpr int TILES = L::TILES, HALVES = L::HALVES, PARTS = L::PARTS, KT = L::KT, ROWS = L::ROWS, GROUPS = L::GROUPS, NBUF = L::NBUF;
     dep_sync();
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* sm = smem_raw + (base - smem_u32(smem_raw));
     float* s_row = reinterpret_cast<float*>(sm + L::ROW_SCALE);
     volatile uint32_t* s_red = reinterpret_cast<volatile uint32_t*>(sm + L::RED);
-    // barriers: keys and values in place and done with (two places each), scores there (two places), weights there, values of a block added
-    const uint32_t bars = base + L::BARS, p_full = bars + 80, o_done = bars + 88;
+    // barriers: keys and values in place and done with; of each tile: scores there and their place free again, weights there, values of a block added
+    const uint32_t bars = base + L::BARS;
     auto k_full = [&](int i) { return bars + 8u * i; };
-    auto k_free = [&](int i) { return bars + 8u * (2 + i); };
-    auto v_full = [&](int i) { return bars + 8u * (4 + i); };
-    auto v_free = [&](int i) { return bars + 8u * (6 + i); };
-    auto s_full = [&](int i) { return bars + 8u * (8 + i); };
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::BARS + 96);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::BARS + 104);
+    auto k_free = [&](int i) { return bars + 8u * (NBUF + i); };
+    auto v_full = [&](int i) { return bars + 8u * (2 * NBUF + i); };
+    auto v_free = [&](int i) { return bars + 8u * (3 * NBUF + i); };
+    auto s_full = [&](int t, int i) { return bars + 8u * (4 * NBUF + 2 * t + i); };
+    auto s_free = [&](int t, int i) { return bars + 8u * (4 * NBUF + 4 + 2 * t + i); };
+    auto p_full = [&](int t) { return bars + 8u * (4 * NBUF + 8 + t); };
+    auto o_done = [&](int t) { return bars + 8u * (4 * NBUF + 10 + t); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::BARS + 8 * (4 * NBUF + 12));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::BARS + 8 * (4 * NBUF + 13));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // ---- which rows: sequence by sequence, the tiles that see most first ----
@@ -245,15 +251,20 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             s_red[2 * warp + 1] = l;
         }
         if (tid == 0) {
-            for (int i = 0; i < 2; i++) {
+            for (int i = 0; i < NBUF; i++) {
                 mbar_init(k_full(i), L::MAKERS);
                 mbar_init(k_free(i), 1);
                 mbar_init(v_full(i), L::MAKERS);
                 mbar_init(v_free(i), 1);
-                mbar_init(s_full(i), 1);
             }
-            mbar_init(p_full, 128);
-            mbar_init(o_done, 1);
+            for (int t = 0; t < 2; t++) {
+                for (int i = 0; i < 2; i++) {
+                    mbar_init(s_full(t, i), 1);
+                    mbar_init(s_free(t, i), 1);
+                }
+                mbar_init(p_full(t), 128);
+                mbar_init(o_done(t), 1);
+            }
             *abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -276,16 +287,18 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
     if (v_top == 0.f) v_top = 1.f;
 
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(L::COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const int blocks = (seen + KT - 1) / KT;
+    // blocks of each tile: the second one's rows see at least as much as the first one's
+    const int blocks = (seen + KT - 1) / KT, blocks0 = rows > 128 ? (max(sees_of(row0 + 127), 0) + KT - 1) / KT : blocks, blocks1 = rows > 128 ? blocks : 0;
     const bool negative = a.scale < 0.f;  // scores' factors are not below zero: the sign goes to the queries
     int* status = a.status;
 
     // ---- queries ----
     // ---- queries ----
-    if (warp < 4) {
+    if (warp < 4 * TILES) {
+        const int t = warp >> 2;
         constexpr int PER = D / 4, AT_ONCE = 32 / PER, BATCH = 8;  // lanes to a row (four values each), rows of a warp at a time, loads on their way
         using Four = typename std::conditional<L::F32, float4, uint2>::type;
         const int c4 = lane % PER;
@@ -294,7 +307,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             Four raw[BATCH];
 #pragma unroll
             for (int i = 0; i < BATCH; i++) {
-                const int at = r0 + i * 4 * AT_ONCE;
+                const int at = t * 128 + r0 + i * 4 * AT_ONCE;
                 raw[i] = Four{};
                 if (at < rows) {
                     const int row = row0 + at, token = token_of(row);
@@ -304,7 +317,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
 #pragma unroll
             for (int i = 0; i < BATCH; i++) {
                 const int r = r0 + i * 4 * AT_ONCE;
-                uint8_t* tile = sm + L::Q + (c4 >> 4) * L::Q_HALF;
+                uint8_t* tile = sm + L::Q + t * PARTS * L::Q_TILE + (c4 >> 4) * L::Q_HALF;
                 const uint32_t to = swizzled(r, (c4 & 15) >> 1) + (c4 & 1) * 8;
                 if constexpr (L::F32) {
                     float4 x = raw[i];
@@ -313,7 +326,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
                     for (int o = PER / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
                     const int e = scale_exponent(most);
                     const float up = negative ? -exp2_int(e) : exp2_int(e);
-                    if (c4 == 0) s_row[r] = exp2_int(-e);
+                    if (c4 == 0) s_row[t * 128 + r] = exp2_int(-e);
                     x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
                     const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(x.z, x.w);
                     const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
@@ -333,11 +346,11 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp < 4) {
+    if (warp < 4 * TILES) {
         // ---------------- softmax ----------------
-        const int r = tid;
-        const uint32_t at = tmem + (static_cast<uint32_t>(warp * 32) << 16), o_at = at + L::O_AT;
-        const int sees = r < rows ? sees_of(row0 + r) : 0, least = sees_of(row0);  // least: what every row sees
+        const int t = warp >> 2, r = tid, own_blocks = t == 0 ? blocks0 : blocks1;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), at = lanes + t * 128, o_at = lanes + L::O_AT + t * L::O_PITCH;
+        const int sees = r < rows ? sees_of(row0 + r) : 0, least = sees_of(row0 + t * 128);  // least: what every row of the tile sees
         const float q_scale = fabsf(a.scale) * 1.44269504f * (L::F32 ? s_row[r] : 1.f);
         const float v_inv = 1.f / v_top;
         float top = -INFINITY, sum = 0.f;
@@ -363,7 +376,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
         page_of(0);
         scales_of();
         page_of(1);
-        for (int j = 0; j < blocks; j++) {
+        for (int j = 0; j < own_blocks; j++) {
             // lane n has the scales of 16 keys; f_of: what a row's scores are multiplied by (not zero: hidden scores stay -inf)
             const float ks = ks_next, vs = vs_next * v_inv;
             auto f_of = [&](int n) { return fmaxf(__shfl_sync(0xffffffffu, ks, n) * q_scale, 1e-38f); };
@@ -372,7 +385,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             page_of(j + 2);
             const bool hidden = (j + 1) * KT > least;
             const int see = sees - j * KT;
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full(j & 1), (j >> 1) & 1, abort_flag, status));
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, j & 1), (j >> 1) & 1, abort_flag, status));
             if (!ok) break;
             tc_fence_after();
             const uint32_t s_at = at + (j & 1) * KT;
@@ -447,7 +460,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             }
             // The values of the block before have been added: the sums can be touched.  (And the MMA thread has seen the weights before these: p_full is never two ahead of it.)
             if (j > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(o_done, (j - 1) & 1, abort_flag, status));
+                ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (j - 1) & 1, abort_flag, status));
                 if (!ok) break;
                 tc_fence_after();
             }
@@ -484,17 +497,17 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(p_full);
+            mbar_arrive(p_full(t));
         }
         // ---- results ----
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (blocks - 1) & 1, abort_flag, status));
+        if (ok && own_blocks > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (own_blocks - 1) & 1, abort_flag, status));
         tc_fence_after();
         const float inv = 1.f / sum * v_top;
         const int row = row0 + r, token = token_of(row);
         T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D;
 #pragma unroll 1
         for (int i = 0; i < D; i += 32) {
-            uint32_t o[32];
+            uint32_t o[32];  // (of a tile without keys: nothing that is looked at)
             tmem_ld_x32(o_at + i, o);
             if constexpr (L::F32) {
                 uint32_t m[32];
@@ -522,18 +535,18 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
             }
         }
         tc_fence_before();
-    } else if (warp < 7) {
+    } else if (warp < 4 * TILES + 4) {
         // ---------------- codes to f16 tiles: 16-byte pieces of a key, a thread always the same piece, of keys own_key + i STEP ----------------
-        constexpr int PIECES = D / 16, STEP = L::MAKERS / PIECES, N = (KT + STEP - 1) / STEP;
-        const int me = tid - 128, own_key = me / PIECES, piece = me % PIECES;
+        constexpr int PIECES = D / 16, STEP = L::MAKERS / PIECES, N = KT / STEP;
+        const int me = tid - ROWS, own_key = me / PIECES, piece = me % PIECES;
         const int64_t head = static_cast<int64_t>(h) * c.page * D + piece * 16, page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
         int page[N];
         uint4 kx[N], vx[N];
         auto look_up = [&](int j) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int at = own_key + i * STEP, key = j * KT + at;
-                page[i] = at < KT && key < seen ? table[key >> c.page_log] : -1;
+                const int key = j * KT + own_key + i * STEP;
+                page[i] = key < seen ? table[key >> c.page_log] : -1;
             }
         };
         auto load = [&](const int8_t* codes, int j, uint4 (&x)[N]) {
@@ -548,11 +561,9 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const int r = own_key + i * STEP, u = 2 * (piece & 3);
-                if (r < KT) {
-                    uint8_t* to = sm + tile + (piece >> 2) * L::KV_HALF;
-                    *reinterpret_cast<uint4*>(to + swizzled(r, u)) = eight_f16(x[i].x, x[i].y);
-                    *reinterpret_cast<uint4*>(to + swizzled(r, u + 1)) = eight_f16(x[i].z, x[i].w);
-                }
+                uint8_t* to = sm + tile + (piece >> 2) * L::KV_HALF;
+                *reinterpret_cast<uint4*>(to + swizzled(r, u)) = eight_f16(x[i].x, x[i].y);
+                *reinterpret_cast<uint4*>(to + swizzled(r, u + 1)) = eight_f16(x[i].z, x[i].w);
             }
             fence_proxy_async();
         };
@@ -561,63 +572,91 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
         load(c.v, 0, vx);
         look_up(1);
         bool ok = true;
+        int i = 0;
+        uint32_t phase = 1;  // (the first use of a place goes through)
 #pragma unroll 1
         for (int j = 0; j < blocks; j++) {
-            const int i = j & 1;
-            const uint32_t parity = ((j >> 1) & 1) ^ 1;  // (the first use of a place goes through)
-            ok = mbar_wait(k_free(i), parity, abort_flag, status);
+            ok = mbar_wait(k_free(i), phase, abort_flag, status);
             if (!ok) break;
             put(L::K + i * L::KV_TILE, kx);
             mbar_arrive(k_full(i));
             load(c.k, j + 1, kx);
-            ok = mbar_wait(v_free(i), parity, abort_flag, status);
+            ok = mbar_wait(v_free(i), phase, abort_flag, status);
             if (!ok) break;
             put(L::V + i * L::KV_TILE, vx);
             mbar_arrive(v_full(i));
             load(c.v, j + 1, vx);
             look_up(j + 2);
+            if (++i == NBUF) {
+                i = 0;
+                phase ^= 1;
+            }
+        }
+    } else if (warp == 4 * TILES + 4) {
+        // ---------------- MMAs of the scores: lower halves of descriptors are address / 16, and for the values the distance between blocks of 64 dims ----------------
+        if (lane == 0) {
+            constexpr uint32_t qk = (1u << 4) | ((KT >> 3) << 17) | ((128 >> 4) << 24);
+            const uint32_t q_desc = (base + L::Q) >> 4 | 1u << 16, k_desc = (base + L::K) >> 4 | 1u << 16;
+            bool ok = true;
+            int i = 0;
+            uint32_t phase = 0;
+#pragma unroll 1
+            for (int j = 0; j < blocks && ok; j++) {
+                ok = mbar_wait(k_full(i), phase, abort_flag, status);
+                const uint32_t kd = k_desc + i * (L::KV_TILE >> 4), d = tmem + (j & 1) * KT;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) {
+                    if (!ok || j >= (t == 0 ? blocks0 : blocks1)) continue;
+                    // the weights of block j - 2, which lie there, have been read
+                    ok = mbar_wait(s_free(t, j & 1), ((j >> 1) & 1) ^ 1, abort_flag, status);
+                    if (!ok) continue;
+                    tc_fence_after();
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; part--)  // the small products first
+#pragma unroll
+                        for (int half = 0; half < HALVES; half++)
+#pragma unroll
+                            for (int kk = 0; kk < 4; kk++)
+                                mma_ss(d + t * 128, q_desc + (((t * PARTS + part) * L::Q_TILE + half * L::Q_HALF) >> 4) + kk * 2, kd + ((half * L::KV_HALF) >> 4) + kk * 2, qk,
+                                       part < PARTS - 1 || half > 0 || kk > 0);
+                    umma::commit<1>(s_full(t, j & 1));
+                }
+                if (ok) umma::commit<1>(k_free(i));
+                if (++i == NBUF) {
+                    i = 0;
+                    phase ^= 1;
+                }
+            }
         }
     } else if (lane == 0) {
-        // ---------------- MMAs ----------------
-        // lower halves of the operands' descriptors: address / 16, and for the values the distance between blocks of 64 dims
-        const uint32_t q_desc = (base + L::Q) >> 4 | 1u << 16, k_desc = (base + L::K) >> 4 | 1u << 16, v_desc = (base + L::V) >> 4 | (L::KV_HALF >> 4) << 16;
-        constexpr uint32_t qk = (1u << 4) | ((KT >> 3) << 17) | ((128 >> 4) << 24), pv = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);  // (values: keys along the rows)
+        // ---------------- MMAs of the values ----------------
+        constexpr uint32_t pv = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);  // keys along the rows
+        const uint32_t v_desc = (base + L::V) >> 4 | (L::KV_HALF >> 4) << 16;
         bool ok = true;
-        auto scores = [&](int j) {
-            const int i = j & 1;
-            ok = ok && mbar_wait(k_full(i), (j >> 1) & 1, abort_flag, status);
-            if (!ok) return;
-            tc_fence_after();
-            const uint32_t kd = k_desc + i * (L::KV_TILE >> 4), d = tmem + i * KT;
-#pragma unroll
-            for (int part = PARTS - 1; part >= 0; part--)  // the small products first
-#pragma unroll
-                for (int half = 0; half < HALVES; half++)
-#pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        mma_ss(d, q_desc + ((part * L::Q_TILE + half * L::Q_HALF) >> 4) + kk * 2, kd + ((half * L::KV_HALF) >> 4) + kk * 2, qk, part < PARTS - 1 || half > 0 || kk > 0);
-            umma::commit<1>(s_full(i));
-            umma::commit<1>(k_free(i));
-        };
+        int i = 0;
+        uint32_t phase = 0;
 #pragma unroll 1
-        for (int j = -2; j < blocks && ok; j++) {
-            if (j >= 0) {
-                const int i = j & 1;
-                ok = mbar_wait(v_full(i), (j >> 1) & 1, abort_flag, status) && mbar_wait(p_full, j & 1, abort_flag, status);
-                if (!ok) break;
+        for (int j = 0; j < blocks && ok; j++) {
+            ok = mbar_wait(v_full(i), phase, abort_flag, status);
+            const uint32_t vd = v_desc + i * (L::KV_TILE >> 4);
+#pragma unroll
+            for (int t = 0; t < TILES; t++) {
+                if (!ok || j >= (t == 0 ? blocks0 : blocks1)) continue;
+                ok = mbar_wait(p_full(t), j & 1, abort_flag, status);
+                if (!ok) continue;
                 tc_fence_after();
 #pragma unroll
                 for (int part = PARTS - 1; part >= 0; part--)
 #pragma unroll
                     for (int kk = 0; kk < 4; kk++)
-                        mma_ts(tmem + L::O_AT, tmem + i * KT + part * 32 + kk * 8, v_desc + i * (L::KV_TILE >> 4) + kk * 128, pv, part < PARTS - 1 || kk > 0 ? 1u : j > 0);
-                umma::commit<1>(o_done);
-                umma::commit<1>(v_free(i));
+                        mma_ts(tmem + L::O_AT + t * L::O_PITCH, tmem + t * 128 + (j & 1) * KT + part * 32 + kk * 8, vd + kk * 128, pv, part < PARTS - 1 || kk > 0 ? 1u : j > 0);
+                umma::commit<1>(o_done(t));
+                umma::commit<1>(s_free(t, j & 1));
             }
-            if (j + 2 < blocks) {
-                // in the place of the weights that the MMAs just issued read.  (Their softmax has the scores of block j + 1 meanwhile.)
-                if (j >= 0) ok = mbar_wait(o_done, j & 1, abort_flag, status);
-                scores(j + 2);
+            if (ok) umma::commit<1>(v_free(i));
+            if (++i == NBUF) {
+                i = 0;
+                phase ^= 1;
             }
         }
     }
@@ -625,7 +664,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, Prompt<T, D>::PER_SM) p
     __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::COLS) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
 }
 
