@@ -228,29 +228,40 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     const int seen = max(sees_of(row0 + rows - 1), 0);  // keys that the last row sees
     const int32_t* table = q.table + static_cast<int64_t>(b) * q.width;
 
-    // ---- the pages that they see: all there, scales finite and not below zero, those of V of one size? ----
-    float v_top = 0.f, v_low = INFINITY;
-    bool plain = true;
-    const int pages = (seen + c.page - 1) >> c.page_log;
-    for (int i = tid; i < pages; i += L::THREADS) {
-        const int p = i < q.width ? table[i] : -1;
-        if (p < 0 || p >= c.pages) {
-            plain = false;
-        } else {
-            const int64_t block = static_cast<int64_t>(p) * c.kv_heads + h;
-            const float k = c.ks[block], v = c.vs[block];
-            plain = plain && k >= 0.f && k < INFINITY && v >= 0.f && v < INFINITY;
-            v_top = fmaxf(v_top, v);
-            if (v > 7.52316385e-37f) v_low = fminf(v_low, v);  // 2^-120: a block of zeros has the scale 2^-126
+    // blocks of each tile: the second one's rows see at least as much as the first one's
+    const int blocks = (seen + KT - 1) / KT, blocks0 = rows > 128 ? (max(sees_of(row0 + 127), 0) + KT - 1) / KT : blocks, blocks1 = rows > 128 ? blocks : 0;
+    const bool negative = a.scale < 0.f;  // scores' factors are not below zero: the sign goes to the queries
+    int* status = a.status;
+    constexpr int OTHERS = L::MAKERS + 64, FIRST = ROWS / 32;  // threads and first warp that are not the softmax's
+
+    // ---- while the softmax's warps bring the queries, the others look at the pages: all there, scales finite and not below zero, those of V of one size? ----
+    if (warp >= FIRST) {
+        float v_top = 0.f, v_low = INFINITY;
+        bool plain = true;
+        const int pages = (seen + c.page - 1) >> c.page_log;
+        for (int i = tid - ROWS; i < pages; i += OTHERS) {
+            const int p = i < q.width ? table[i] : -1;
+            if (p < 0 || p >= c.pages) {
+                plain = false;
+            } else {
+                const int64_t block = static_cast<int64_t>(p) * c.kv_heads + h;
+                const float k = c.ks[block], v = c.vs[block];
+                plain = plain && k >= 0.f && k < INFINITY && v >= 0.f && v < INFINITY;
+                v_top = fmaxf(v_top, v);
+                if (v > 7.52316385e-37f) v_low = fminf(v_low, v);  // 2^-120: a block of zeros has the scale 2^-126
+            }
         }
-    }
-    {
         const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(v_top)), l = __reduce_min_sync(0xffffffffu, __float_as_uint(v_low));
+        plain = __all_sync(0xffffffffu, plain);
         if (lane == 0) {
-            s_red[2 * warp] = t;
-            s_red[2 * warp + 1] = l;
+            s_red[2 * (warp - FIRST)] = t;
+            s_red[2 * (warp - FIRST) + 1] = plain ? l : 0u;  // (0: no lower end, never of one size)
         }
-        if (tid == 0) {
+        if (warp == FIRST + 4) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        if (warp == FIRST + 5 && lane == 0) {
             for (int i = 0; i < NBUF; i++) {
                 mbar_init(k_full(i), L::MAKERS);
                 mbar_init(k_free(i), 1);
@@ -268,38 +279,12 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             *abort_flag = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        plain = __syncthreads_and(plain);
-        uint32_t top = 0, low = 0x7f800000u;
-        for (int w = 0; w < L::THREADS / 32; w++) {
-            top = max(top, s_red[2 * w]);
-            low = min(low, s_red[2 * w + 1]);
-        }
-        v_top = __uint_as_float(top);
-        v_low = __uint_as_float(low);
+        asm volatile("bar.sync 2, %0;" ::"n"(OTHERS) : "memory");
     }
-    if (!plain || !(v_low * 1024.f >= v_top) || seen == 0) {
-        for (int r = warp; r < rows; r += L::THREADS / 32) {
-            const int row = row0 + r, token = token_of(row);
-            row_in_fp32<T, D>(c, q, a, b, first + token, h * a.group + row - token * a.group, sees_of(row));
-        }
-        return;
-    }
-    if (v_top == 0.f) v_top = 1.f;
-
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    // blocks of each tile: the second one's rows see at least as much as the first one's
-    const int blocks = (seen + KT - 1) / KT, blocks0 = rows > 128 ? (max(sees_of(row0 + 127), 0) + KT - 1) / KT : blocks, blocks1 = rows > 128 ? blocks : 0;
-    const bool negative = a.scale < 0.f;  // scores' factors are not below zero: the sign goes to the queries
-    int* status = a.status;
-
     // ---- queries ----
-    // ---- queries ----
-    if (warp < 4 * TILES) {
+    if (warp < FIRST) {
         const int t = warp >> 2;
-        constexpr int PER = D / 4, AT_ONCE = 32 / PER, BATCH = 8;  // lanes to a row (four values each), rows of a warp at a time, loads on their way
+        constexpr int PER = D / 4, AT_ONCE = 32 / PER, BATCH = 16;  // lanes to a row (four values each), rows of a warp at a time, loads on their way
         using Four = typename std::conditional<L::F32, float4, uint2>::type;
         const int c4 = lane % PER;
 #pragma unroll 1
@@ -341,12 +326,36 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         }
         fence_proxy_async();
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    // the queries are there, TMEM and what was seen of the pages; the warps that bring the codes need no queries and go on
+    const bool maker = warp >= FIRST && warp < FIRST + 4;
+    if (maker) {
+        asm volatile("bar.arrive 1, %0;" ::"n"(L::THREADS) : "memory");
+    } else {
+        tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(L::THREADS) : "memory");
+        tc_fence_after();
+    }
+    float v_top;
+    {
+        uint32_t top = 0, low = 0x7f800000u;
+        for (int w = 0; w < OTHERS / 32; w++) {
+            top = max(top, s_red[2 * w]);
+            low = min(low, s_red[2 * w + 1]);
+        }
+        v_top = __uint_as_float(top);
+        if (!(__uint_as_float(low) * 1024.f >= v_top) || low == 0 || seen == 0) {
+            for (int r = warp; r < rows; r += L::THREADS / 32) {
+                const int row = row0 + r, token = token_of(row);
+                row_in_fp32<T, D>(c, q, a, b, first + token, h * a.group + row - token * a.group, sees_of(row));
+            }
+            if (warp == FIRST + 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "n"(512) : "memory");
+            return;
+        }
+        if (v_top == 0.f) v_top = 1.f;
+    }
+    const uint32_t tmem = maker ? 0u : *tmem_slot;
 
-    if (warp < 4 * TILES) {
+    if (warp < FIRST) {
         // ---------------- softmax ----------------
         const int t = warp >> 2, r = tid, own_blocks = t == 0 ? blocks0 : blocks1;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), at = lanes + t * 128, o_at = lanes + L::O_AT + t * L::O_PITCH;
@@ -535,7 +544,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             }
         }
         tc_fence_before();
-    } else if (warp < 4 * TILES + 4) {
+    } else if (maker) {
         // ---------------- codes to f16 tiles: 16-byte pieces of a key, a thread always the same piece, of keys own_key + i STEP ----------------
         constexpr int PIECES = D / 16, STEP = L::MAKERS / PIECES, N = KT / STEP;
         const int me = tid - ROWS, own_key = me / PIECES, piece = me % PIECES;
@@ -592,7 +601,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 phase ^= 1;
             }
         }
-    } else if (warp == 4 * TILES + 4) {
+    } else if (warp == FIRST + 4) {
         // ---------------- MMAs of the scores: lower halves of descriptors are address / 16, and for the values the distance between blocks of 64 dims ----------------
         if (lane == 0) {
             constexpr uint32_t qk = (1u << 4) | ((KT >> 3) << 17) | ((128 >> 4) << 24);
@@ -662,7 +671,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == FIRST + 4) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
