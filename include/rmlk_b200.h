@@ -498,7 +498,8 @@ RMLK_API int rmlk_b200_quantize_rows(rmlk_stream_t stream, int dtype, int64_t ro
 
 /* out[m,n] = (sum_k x[m,k] w[n,k]) * x_scales[m] * w_scales[n]: int8 operands (any codes, -128 too), both with k running along the rows,
  * ldx / ldw bytes apart (multiples of 16, on 16-byte boundaries; what lies behind k in a row is not read as part of it); the sum is exact
- * (int32: k <= 131071), converted to fp32 and scaled there.  out: f32 or f16, rows ldo elements apart, on 16-byte boundaries in its first row.
+ * (int32: k <= 131071), converted to fp32 and scaled there.  out: f32 or f16, rows ldo elements apart, wherever their type may lie (rows on 16-byte
+ * boundaries are written fastest).
  * `status`: device word that receives RMLK_ERR_TIMEOUT should a bounded wait of the tensor-core kernel expire, or NULL. */
 RMLK_API int rmlk_b200_matmul_i8(rmlk_stream_t stream, int out_dtype, int64_t m, int64_t n, int64_t k, const void* x, int64_t ldx,
                         const float* x_scales, const void* w, int64_t ldw, const float* w_scales, void* out, int64_t ldo, int* status);
@@ -536,17 +537,20 @@ RMLK_API int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rmlk_
 
 /* Attention of the new tokens over such a cache (their own keys and values in it already): row i of sequence b, at position
  * p = lens[b] - new[b] + i, sees positions 0 .. p;
- *   out[row, h] = softmax_t(scale q[row, h] . k[t, h / (q_heads / kv_heads)]) v[t, ..]
+ *   out[row, h] = softmax_t(scale q[row, h] . k[t, h / (q_heads / kv_heads)]) v[t, ..]      (scale: any finite number)
  * q, out: [tokens, q_heads, head_dim] f32 or f16, heads dense, rows q_stride / out_stride elements apart; q_heads a multiple of
- * kv_heads, up to 64 for each.  A row that sees nothing is 0; one that sees a token whose page is not in [0, pages) or lies behind table_width is
- * NaN, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG (RMLK_ERR_TIMEOUT: a bounded wait expired).
- * `workspace`: rmlk_b200_paged_attention_workspace_bytes() bytes on a 16-byte boundary, zero-filled before its first use; its counters are
- * zero again after each call.  Calls that may overlap on the GPU take one each. */
+ * kv_heads, up to 64 for each; rows on 16-byte boundaries.  A row that sees nothing is 0; one that sees a block whose scale is NaN is NaN; one that sees
+ * a token whose page is not in [0, pages) or lies behind table_width is NaN, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG
+ * (RMLK_ERR_TIMEOUT: a bounded wait expired).
+ * Few rows over many keys share the keys out over the whole GPU, where every sequence has as many (starts NULL); with starts each sequence is walked
+ * along by itself.  So single tokens beside whole prompts are best given to a call of their own.
+ * `workspace`: rmlk_b200_paged_attention_workspace_bytes() bytes (0: none is needed) on a 16-byte boundary, zero-filled before its first use; its
+ * counters are zero again after each call.  Calls that may overlap on the GPU take one each. */
 RMLK_API int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const rmlk_paged_cache* cache, int64_t tokens, int64_t batch,
                               int64_t q_heads, const int32_t* starts, const int32_t* lens, const int32_t* table, int64_t table_width,
                               const void* q, int64_t q_stride, float scale, void* out, int64_t out_stride, void* workspace,
                               size_t workspace_bytes, int* status);
-/* ragged: 1 where starts will be given, 0 where not */
+/* Enough for either type; ragged: 1 where starts will be given, 0 where not. */
 RMLK_API size_t rmlk_b200_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                  int ragged);
 

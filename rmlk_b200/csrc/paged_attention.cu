@@ -50,21 +50,26 @@ static int launch_prompt(cudaStream_t st, const Cache& c, const Batch& s, const 
 
 using namespace rmlk;
 
-// Which kernel takes a call: few_kernel shares the keys out over all SMs and reads them once for each 16 query rows; prompt_kernel has a CTA to 128 rows, which reads all their
-// keys, and two CTAs to an SM.  With P = batch x kv_heads, few_kernel's time is that of P ceil(rows / 16) tiles spread over the GPU, prompt_kernel's that of one CTA as long
-// as every CTA has an SM, of 1.4 for every two CTAs per SM behind that; one CTA takes as long as 3.4 tiles per SM.  Measured with 8 KV heads over 8000 keys, us (few, prompt):
-//   f16 128: 1 x 64 rows 26, 175;  8 x 64 110, 186;  8 x 128 206, 189;  64 x 32 398, 504;  64 x 64 777, 506
-//   f32 64:  1 x 64 rows 21, 233;  8 x 128 146, 239;  8 x 256 280, 239;  64 x 32 281, 550;  64 x 64 546, 554
+// Which kernel takes a call: few_kernel shares the keys out over all SMs and reads them once for each 16 query rows; prompt_kernel has a CTA per SM to 128 or 256 rows, which
+// walks over all their keys.  With P = batch x kv_heads, few_kernel takes the time of P ceil(rows / 16) tiles spread evenly over the GPU, prompt_kernel that of its CTAs, as many at
+// a time as there are SMs.  A CTA takes as long as `cost` tiles of few_kernel on an SM.  Measured with 8 KV heads over 8000 keys, us (few, prompt), B x rows of a KV head:
+//   f16 128: 8 x 64 112, 156;  8 x 128 210, 159;  1 x 512 112, 180;  8 x 256 421, 187;  64 x 32 407, 604;  64 x 64 793, 603
+//   f32 128: 8 x 64 139, 200;  8 x 128 260, 203;  8 x 256 505, 204;  64 x 32 505, 755;  64 x 64 992, 760
+//   f16 64:  8 x 128 128, 136;  8 x 256 246, 175;  64 x 64 478, 511;  64 x 128 944, 512
+//   f32 64:  8 x 128 150, 187;  8 x 256 287, 259;  64 x 64 564, 764;  64 x 128 1115, 772
 // The new tokens of ragged sequences lie at places that only the device knows: they go to prompt_kernel.
-static bool takes_few(int64_t tokens, int64_t batch, int64_t kv_heads, int64_t group, bool ragged) {
+static bool takes_few(bool f32, int64_t tokens, int64_t batch, int64_t kv_heads, int64_t group, int64_t head_dim, bool ragged) {
     if (ragged || batch < 1) return false;
     const double sms = sm_count(), rows = static_cast<double>(tokens / batch) * group, problems = static_cast<double>(batch) * kv_heads;
-    const double ctas = problems * std::ceil(rows / 128.0), alone = ctas <= sms ? 1.0 : 1.4 * std::ceil(ctas / (2.0 * sms));
-    return problems * std::ceil(rows / 16.0) <= 3.4 * sms * alone;
+    const bool pairs = !(f32 && head_dim == 128);  // a CTA of prompt_kernel has two tiles of 128 rows where there are as many
+    const double cost = pairs && rows > 128 ? (head_dim == 64 ? 5.5 : 3.1) : (head_dim == 64 ? 4.2 : 2.6);
+    return problems * std::ceil(rows / 16.0) <= cost * sms * std::ceil(problems * std::ceil(rows / (pairs ? 256.0 : 128.0)) / sms);
 }
 
 extern "C" size_t rmlk_b200_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int ragged) {
-    if (kv_heads < 1 || q_heads < kv_heads || !takes_few(tokens, batch, kv_heads, q_heads / kv_heads, ragged != 0)) return 0;
+    if (kv_heads < 1 || q_heads < kv_heads) return 0;
+    const int64_t group = q_heads / kv_heads;
+    if (!takes_few(true, tokens, batch, kv_heads, group, head_dim, ragged != 0) && !takes_few(false, tokens, batch, kv_heads, group, head_dim, ragged != 0)) return 0;
     return paged::few_workspace(head_dim);
 }
 
@@ -86,7 +91,7 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
     if (!aligned_to(q, 16) || !aligned_to(out, 16) || q_stride % per || out_stride % per) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: rows must lie on 16-byte boundaries");
     paged::Attend a = {q, out, q_stride, out_stride, static_cast<int>(q_heads), static_cast<int>(q_heads / c.kv_heads), scale, status};
     const cudaStream_t st = as_stream(stream);
-    if (takes_few(tokens, batch, c.kv_heads, a.group, starts != nullptr)) {
+    if (takes_few(dtype == RMLK_F32, tokens, batch, c.kv_heads, a.group, c.d, starts != nullptr)) {
         if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
             return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
         const bool one = s.each * a.group <= 8;

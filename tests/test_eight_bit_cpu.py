@@ -32,9 +32,9 @@ def _append(cache=None, dtype=F32, tokens=3, batch=3, starts=None, lens=A, table
                                             lo, None)
 
 
-def _attend(cache=None, dtype=F32, tokens=3, batch=3, qh=4, starts=None, lens=A, table=A, width=2, q=A, lq=256, out=A, lo=256, work=A, size=1 << 30, **c):
+def _attend(cache=None, dtype=F32, tokens=3, batch=3, qh=4, starts=None, lens=A, table=A, width=2, q=A, lq=256, out=A, lo=256, work=A, size=1 << 30, scale=0.125, **c):
     cache = _cache(**c) if cache is None else cache
-    return _lib()[0].rmlk_b200_paged_attention(None, dtype, ctypes.addressof(cache) if cache else None, tokens, batch, qh, starts, lens, table, width, q, lq, 0.125, out, lo, work, size,
+    return _lib()[0].rmlk_b200_paged_attention(None, dtype, ctypes.addressof(cache) if cache else None, tokens, batch, qh, starts, lens, table, width, q, lq, scale, out, lo, work, size,
                                                None)
 
 
@@ -47,7 +47,9 @@ def _attend(cache=None, dtype=F32, tokens=3, batch=3, qh=4, starts=None, lens=A,
                dict(k=A + 8), dict(v=A + 4), dict(cos=None), dict(sin=None), dict(cos=None, sin=None), dict(rows=-1), dict(qh=0), dict(qo=0), dict(lq=255), dict(lo=255), dict(q=A + 4),
                dict(qo=A + 8), dict(lens=A + 2), dict(table=A + 1), dict(starts=A + 2), dict(cos=A + 4)]),
     (_attend, [dict(cache=0), dict(page=8), dict(page=256), dict(d=96), dict(pages=-1), dict(kv=0), dict(qh=3), dict(qh=0), dict(qh=130, lq=130 * 64, lo=130 * 64), dict(tokens=4), dict(tokens=-3),
-               dict(width=-1), dict(lens=0), dict(table=0), dict(q=0), dict(out=0), dict(lq=255), dict(lo=252), dict(lq=258), dict(lo=257), dict(q=A + 8), dict(out=A + 4), dict(lens=A + 1)]),
+               dict(width=-1), dict(lens=0), dict(table=0), dict(q=0), dict(out=0), dict(lq=255), dict(lo=252), dict(lq=258), dict(lo=257), dict(q=A + 8), dict(out=A + 4), dict(lens=A + 1),
+               dict(pages=0), dict(scale=float("inf")), dict(scale=float("nan")), dict(work=0), dict(work=A + 8), dict(size=0), dict(size=1 << 15), dict(starts=A + 2),
+               dict(tokens=1 << 30, batch=1 << 30, qh=8, lq=512, lo=512)]),
 ])
 def test_refused(call, bad):
     for case in bad:
@@ -82,4 +84,9 @@ def test_bindings_refuse_before_the_call():
 
 def test_workspace_sizes():
     L = _lib()[0]
-    assert all(L.rmlk_b200_paged_attention_workspace_bytes(64, 64, 32, 8, d, ragged) >= 0 for d in (64, 128) for ragged in (0, 1))
+    size = L.rmlk_b200_paged_attention_workspace_bytes
+    for d in (64, 128):
+        assert size(64, 64, 32, 8, d, 0) > 0 == size(64, 64, 32, 8, d, 1)
+        assert size(1, 1, 8, 8, d, 0) == size(64, 64, 32, 8, d, 0)  # one will do for all calls of a head_dim
+        assert size(1 << 16, 8, 32, 8, d, 0) == 0  # whole prompts need none
+        assert size(0, 0, 32, 8, d, 0) == size(5, 0, 32, 8, d, 0) == size(4, 4, 8, 0, d, 0) == size(4, 4, 4, 8, d, 0) == 0
