@@ -508,8 +508,9 @@ RMLK_API int rmlk_b200_matmul_i8(rmlk_stream_t stream, int out_dtype, int64_t m,
  * [pages, kv_heads] fp32, one for the block of a page and head: a value is its code times the scale.  page_size 16, 32, 64 or 128;
  * head_dim 64 or 128; everything on 16-byte boundaries.
  * Sequence b of a batch holds lens[b] tokens (int32, device); token t lies in slot t % page_size of page table[b * table_width + t / page_size]
- * (int32, device).  Entries behind the last token's page are not read.  The new tokens of a call are the LAST ones of each sequence - lens counts them:
- * rows starts[b] .. starts[b+1] of its tensors (int32 [batch + 1], device, rising from 0), or tokens / batch rows each where starts is NULL.
+ * (int32, device; table_width * page_size up to 2^30).  Entries behind the last token's page are not read.  The new tokens of a call are the LAST
+ * ones of each sequence - lens counts them: rows starts[b] .. starts[b+1] of its tensors (int32 [batch + 1], device, rising from 0), or
+ * tokens / batch rows each where starts is NULL.  Pages that hold the same beginning of several sequences may be named by all of them.
  * A sequence of length 0 is one that the call passes over.  Rows behind starts[batch] are neither read nor written. */
 typedef struct rmlk_paged_cache {
     int64_t pages, kv_heads, page_size, head_dim;
@@ -529,7 +530,8 @@ typedef struct rmlk_paged_cache {
  * Codes are value / 2^e rounded to nearest even.  A block that receives an infinity or a NaN gets the scale NaN - what attends to it is NaN -
  * until it is begun anew in its first slot.  Positions below 0 (lens[b] less than the new tokens) are passed over.
  * A token whose page is not in [0, pages), which lies behind table_width pages or table_rows positions is not stored, its query is not
- * written, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG.  No page may receive tokens of two sequences in one call. */
+ * written, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG.  q_out may be q.
+ * No page may receive tokens twice in one call: from two sequences, or from one whose table names it twice among its new tokens' pages. */
 RMLK_API int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rmlk_paged_cache* cache, int64_t tokens, int64_t batch,
                            const int32_t* starts, const int32_t* lens, const int32_t* table, int64_t table_width, const void* k,
                            int64_t k_stride, const void* v, int64_t v_stride, const float* cos, const float* sin, int64_t table_rows,

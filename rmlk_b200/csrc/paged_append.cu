@@ -23,7 +23,8 @@ int take(const char* what, const rmlk_paged_cache* cache, int64_t tokens, int64_
     if (d != 64 && d != 128) return bad("head_dim must be 64 or 128");
     if (cache->pages < 0 || cache->pages >= (1ll << 31) || cache->kv_heads < 1 || cache->kv_heads > 65535 || cache->pages * cache->kv_heads >= (1ll << 31))
         return bad("bad cache extent");
-    if (tokens < 0 || tokens >= (1ll << 31) || batch < 0 || batch >= (1ll << 24) || table_width < 0 || table_width >= (1ll << 31) / page) return bad("bad extent");
+    if (tokens < 0 || tokens >= (1ll << 31) || batch < 0 || batch >= (1ll << 24) || table_width < 0 || table_width > (1ll << 30) / page)  // (keys and steps past them stay in 31 bits)
+        return bad("bad extent");
     if (static_cast<double>(batch) * static_cast<double>(table_width + 1) * static_cast<double>(cache->kv_heads) > 1e13) return bad("bad extent");  // (unit counts times CTAs stay in 63 bits)
     if (tokens > 0 && batch > 0 && !starts && tokens % batch) return bad("without starts, tokens must be a multiple of batch");
     if (tokens > 0 && batch > 0) {

@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
         s.tile = static_cast<int>(item) - s.h * tiles;
         s.first_key = unit0 * L::UNIT + warp * KS;
         const int64_t left = min(keys, (unit0 + s.taken) * L::UNIT) - s.first_key;
-        s.left = static_cast<int>(min(max(left, int64_t(0)), int64_t(0x7fffff00)));  // (2^31 keys are none of a cache's)
+        s.left = static_cast<int>(max(left, int64_t(0)));
         s.steps = (s.left + L::UNIT - 1) / L::UNIT;
     };
     auto move_on = [&](Segment& s) {

@@ -219,9 +219,9 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     const int rows = static_cast<int>(min(count * a.group - static_cast<int64_t>(item) * ROWS, static_cast<int64_t>(ROWS)));  // valid rows from row0 on
     const int row0 = item * ROWS;
     const int64_t table_keys = q.width << c.page_log;
-    // (the table has room for fewer than 2^31 keys; what lies far below the first is as good as -1)
+    // (the table has room for at most 2^30 keys; what lies far below the first is as good as -1)
     const int64_t len = q.lens[b];
-    const int keys = static_cast<int>(min(len, table_keys + 1)), before = static_cast<int>(max(len - count, -(int64_t(1) << 31) + (1 << 26)));
+    const int keys = static_cast<int>(min(len, table_keys + 1)), before = static_cast<int>(min(max(len - count, -(int64_t(1) << 31) + (1 << 26)), int64_t(1) << 30));
     // rows of the sequence and head are counted from its first new token on
     auto token_of = [&](int row) { return static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(a.group)); };
     auto sees_of = [&](int row) { return min(before + token_of(row) + 1, keys); };

@@ -697,7 +697,8 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lens: torc
     starts[b]:starts[b+1] (int32 [batch + 1]), or tokens / batch rows where starts is None.  With tables cos, sin [positions, head_dim] fp32 the
     keys are rotated as `rope` does, and the queries q [tokens, q_heads, head_dim] too: they are returned (rows that no sequence has are left
     unwritten).  Scales of blocks are powers of two; a block that fills over several calls keeps or raises its scale.  status [1] int32 becomes 1
-    where a token has no page or no row in the tables; it is not stored.  No page may receive tokens of two sequences in one call."""
+    where a token has no page or no row in the tables; it is not stored.  q_out may be q.  No page may receive tokens twice
+    in one call: from two sequences, or from one whose table names it twice among its new tokens' pages."""
     dev = _device_of("paged_append", cache.k)
     c, shape, at = _paged("paged_append", dev, cache, lens, table, starts, status)
     dtype, want = k.dtype, (k.shape[0] if k.dim() else 0, shape[1], shape[3])
