@@ -544,8 +544,8 @@ RMLK_API int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rmlk_
  * kv_heads, up to 64 for each; rows on 16-byte boundaries.  A row that sees nothing is 0; one that sees a block whose scale is NaN is NaN; one that sees
  * a token whose page is not in [0, pages) or lies behind table_width is NaN, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG
  * (RMLK_ERR_TIMEOUT: a bounded wait expired).
- * Few rows over many keys share the keys out over the whole GPU, where every sequence has as many (starts NULL); with starts each sequence is walked
- * along by itself.  So single tokens beside whole prompts are best given to a call of their own.
+ * Few rows over many keys share the keys out over the whole GPU, where every sequence has as many (starts NULL); with starts at most eight SMs walk along
+ * one sequence and head.  So single tokens beside whole prompts are best given to a call of their own.
  * `workspace`: rmlk_b200_paged_attention_workspace_bytes() bytes (0: none is needed) on a 16-byte boundary, zero-filled before its first use; its
  * counters are zero again after each call.  Calls that may overlap on the GPU take one each. */
 RMLK_API int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const rmlk_paged_cache* cache, int64_t tokens, int64_t batch,

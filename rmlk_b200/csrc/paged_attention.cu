@@ -26,23 +26,61 @@ static int launch_few(cudaStream_t st, const Cache& c, const Batch& s, const Att
     return RMLK_OK;
 }
 
-template <typename T, int D>
-static int launch_prompt(cudaStream_t st, const Cache& c, const Batch& s, const Attend& a) {
+// CTAs of prompt_kernel where all sequences have as many tokens
+static int64_t prompt_ctas(int64_t tokens, int64_t batch, int64_t kv_heads, int64_t group, int64_t rows) { return kv_heads * batch * ceil_div64(ceil_div64(tokens, batch) * group, rows); }
+// CTAs of a cluster that share the keys of each of them: as many as leave all clusters room at once, with 256 keys each or more.  Clusters of 4 fill 7/8 of the SMs, those
+// of 8 some 3/4 (16 of them, f16, 512 rows over 8000 keys: 78 us, with clusters of 4 61).
+// One prompt of 16 tokens, 4 query heads of 128 to each of 8 KV heads, f16: over 8000 keys 28 us, 132 without sharing; over 2000 15 and 38.
+static int prompt_splits(int64_t ctas, int64_t most_keys) {
+    const int64_t sms = sm_count();
+    int splits = 1;
+    while (splits < 8 && ctas * 2 * splits <= (splits == 1 ? sms : splits == 2 ? sms * 7 / 8 : sms * 3 / 4) && most_keys >= 512 * splits) splits *= 2;
+    return splits;
+}
+
+template <typename T, int D, bool SHARED>
+static int launch_prompt(cudaStream_t st, const Cache& c, const Batch& s, const Attend& a, int64_t ctas, int splits) {
     using L = Prompt<T, D>;
-    auto kernel = prompt_kernel<T, D>;
+    auto kernel = prompt_kernel<T, D, SHARED>;
     static std::once_flag configured[64];  // the dynamic shared memory limit is raised once per device
     int dev = 0;
     cudaGetDevice(&dev);
     cudaError_t cfg_err = cudaSuccess;
     if (dev >= 0 && dev < 64) std::call_once(configured[dev], [&] { cfg_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL); });
     RMLK_CUDA(cfg_err);
-    constexpr int64_t ROWS = L::ROWS;
-    const int64_t tokens = s.tokens, batch = s.batch;
-    const int64_t items = s.starts ? tokens * a.group / ROWS + std::min(batch, tokens) : batch * ceil_div64(s.each * a.group, ROWS);  // ragged: as many as there can be
-    if (items * c.kv_heads > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");
-    RMLK_CUDA(launch_dep(kernel, dim3(static_cast<unsigned>(items * c.kv_heads)), dim3(L::THREADS), L::TOTAL, st, c, s, a));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas * splits));
+    cfg.blockDim = dim3(L::THREADS);
+    cfg.dynamicSmemBytes = L::TOTAL;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    unsigned na = 0;
+    if (SHARED) {
+        at[na].id = cudaLaunchAttributeClusterDimension;
+        at[na].val.clusterDim.x = splits;
+        at[na].val.clusterDim.y = at[na].val.clusterDim.z = 1;
+        na++;
+    }
+    if (dep_launch_enabled()) {
+        at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = na;
+    RMLK_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, s, a, splits));
     RMLK_CHECK_LAUNCH("paged_attention prompt_kernel");
     return RMLK_OK;
+}
+
+template <typename T, int D>
+static int prompts(cudaStream_t st, const Cache& c, const Batch& s, const Attend& a) {
+    constexpr int64_t ROWS = Prompt<T, D>::ROWS;
+    const int64_t even = prompt_ctas(s.tokens, s.batch, c.kv_heads, a.group, ROWS);
+    const int64_t ctas = s.starts ? c.kv_heads * (s.tokens * a.group / ROWS + std::min<int64_t>(s.batch, s.tokens)) : even;  // (ragged: as many as there can be)
+    const int splits = prompt_splits(even, s.width << c.page_log);
+    if (ctas * splits > 0x7fffffffll) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: too many tokens");
+    return splits > 1 ? launch_prompt<T, D, true>(st, c, s, a, ctas, splits) : launch_prompt<T, D, false>(st, c, s, a, ctas, 1);
 }
 
 }  // namespace paged
@@ -50,26 +88,29 @@ static int launch_prompt(cudaStream_t st, const Cache& c, const Batch& s, const 
 
 using namespace rmlk;
 
-// Which kernel takes a call: few_kernel shares the keys out over all SMs and reads them once for each 16 query rows; prompt_kernel has a CTA per SM to 128 or 256 rows, which
-// walks over all their keys.  With P = batch x kv_heads, few_kernel takes the time of P ceil(rows / 16) tiles spread evenly over the GPU, prompt_kernel that of its CTAs, as many at
-// a time as there are SMs.  A CTA takes as long as `cost` tiles of few_kernel on an SM.  Measured with 8 KV heads over 8000 keys, us (few, prompt), B x rows of a KV head:
-//   f16 128: 8 x 64 112, 156;  8 x 128 210, 159;  1 x 512 112, 180;  8 x 256 421, 187;  64 x 32 407, 604;  64 x 64 793, 603
-//   f32 128: 8 x 64 139, 200;  8 x 128 260, 203;  8 x 256 505, 204;  64 x 32 505, 755;  64 x 64 992, 760
-//   f16 64:  8 x 128 128, 136;  8 x 256 246, 175;  64 x 64 478, 511;  64 x 128 944, 512
-//   f32 64:  8 x 128 150, 187;  8 x 256 287, 259;  64 x 64 564, 764;  64 x 128 1115, 772
+// Which kernel takes a call: few_kernel shares the keys out over all SMs and reads them once for each 16 query rows; prompt_kernel has a CTA or a cluster of them to 128 or 256
+// rows, which walks over all their keys.  With P = batch x kv_heads, few_kernel takes the time of P ceil(rows / 16) tiles spread evenly over the GPU, prompt_kernel that of
+// its CTAs, as many at a time as there are SMs.  A CTA with all keys takes as long as `cost` tiles of few_kernel on an SM.  Measured with 8 KV heads over 8000 keys, us (few,
+// prompt), B x rows of a KV head:
+//   f16 128: 1 x 64 26, 28;  1 x 256 63, 40;  1 x 512 111, 61;  8 x 64 112, 156;  8 x 128 210, 159;  8 x 256 404, 186;  64 x 32 407, 604;  64 x 64 793, 603
+//   f32 128: 1 x 64 30, 37;  1 x 256 77, 64;  8 x 64 139, 200;  8 x 128 260, 203;  8 x 256 508, 203;  64 x 32 505, 755;  64 x 64 992, 760
+//   f16 64:  1 x 64 19, 25;  1 x 256 41, 34;  8 x 128 128, 136;  8 x 256 246, 174;  64 x 64 478, 511;  64 x 128 944, 512
+//   f32 64:  1 x 64 21, 32;  1 x 256 48, 42;  8 x 128 150, 187;  8 x 256 287, 246;  64 x 64 564, 764;  64 x 128 1115, 772
 // The new tokens of ragged sequences lie at places that only the device knows: they go to prompt_kernel.
-static bool takes_few(bool f32, int64_t tokens, int64_t batch, int64_t kv_heads, int64_t group, int64_t head_dim, bool ragged) {
+static bool takes_few(bool f32, int64_t tokens, int64_t batch, int64_t kv_heads, int64_t group, int64_t head_dim, int64_t most_keys, bool ragged) {
     if (ragged || batch < 1) return false;
     const double sms = sm_count(), rows = static_cast<double>(tokens / batch) * group, problems = static_cast<double>(batch) * kv_heads;
     const bool pairs = !(f32 && head_dim == 128);  // a CTA of prompt_kernel has two tiles of 128 rows where there are as many
-    const double cost = pairs && rows > 128 ? (head_dim == 64 ? 5.5 : 3.1) : (head_dim == 64 ? 4.2 : 2.6);
-    return problems * std::ceil(rows / 16.0) <= cost * sms * std::ceil(problems * std::ceil(rows / (pairs ? 256.0 : 128.0)) / sms);
+    const double cost = pairs && rows > 128 ? (head_dim == 64 ? 5.5 : 3.1) : (head_dim == 64 ? 4.2 : 2.6), ctas = problems * std::ceil(rows / (pairs ? 256.0 : 128.0));
+    const int splits = ctas > sms ? 1 : paged::prompt_splits(static_cast<int64_t>(ctas), most_keys);
+    return problems * std::ceil(rows / 16.0) <= cost * sms * std::ceil(ctas / sms) / splits;
 }
 
 extern "C" size_t rmlk_b200_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int ragged) {
     if (kv_heads < 1 || q_heads < kv_heads) return 0;
     const int64_t group = q_heads / kv_heads;
-    if (!takes_few(true, tokens, batch, kv_heads, group, head_dim, ragged != 0) && !takes_few(false, tokens, batch, kv_heads, group, head_dim, ragged != 0)) return 0;
+    // (with few keys few_kernel has the most calls: enough for a table of any width)
+    if (!takes_few(true, tokens, batch, kv_heads, group, head_dim, 0, ragged != 0) && !takes_few(false, tokens, batch, kv_heads, group, head_dim, 0, ragged != 0)) return 0;
     return paged::few_workspace(head_dim);
 }
 
@@ -91,7 +132,7 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
     if (!aligned_to(q, 16) || !aligned_to(out, 16) || q_stride % per || out_stride % per) return fail(RMLK_ERR_INVALID_ARG, "paged_attention: rows must lie on 16-byte boundaries");
     paged::Attend a = {q, out, q_stride, out_stride, static_cast<int>(q_heads), static_cast<int>(q_heads / c.kv_heads), scale, status};
     const cudaStream_t st = as_stream(stream);
-    if (takes_few(dtype == RMLK_F32, tokens, batch, c.kv_heads, a.group, c.d, starts != nullptr)) {
+    if (takes_few(dtype == RMLK_F32, tokens, batch, c.kv_heads, a.group, c.d, s.width << c.page_log, starts != nullptr)) {
         if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
             return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
         const bool one = s.each * a.group <= 8;
@@ -102,6 +143,6 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
         if (c.d == 64) return one ? paged::launch_few<__half, 64, 1>(st, c, s, a, workspace) : paged::launch_few<__half, 64, 2>(st, c, s, a, workspace);
         return one ? paged::launch_few<__half, 128, 1>(st, c, s, a, workspace) : paged::launch_few<__half, 128, 2>(st, c, s, a, workspace);
     }
-    if (dtype == RMLK_F32) return c.d == 64 ? paged::launch_prompt<float, 64>(st, c, s, a) : paged::launch_prompt<float, 128>(st, c, s, a);
-    return c.d == 64 ? paged::launch_prompt<__half, 64>(st, c, s, a) : paged::launch_prompt<__half, 128>(st, c, s, a);
+    if (dtype == RMLK_F32) return c.d == 64 ? paged::prompts<float, 64>(st, c, s, a) : paged::prompts<float, 128>(st, c, s, a);
+    return c.d == 64 ? paged::prompts<__half, 64>(st, c, s, a) : paged::prompts<__half, 128>(st, c, s, a);
 }

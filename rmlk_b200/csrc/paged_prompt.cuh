@@ -6,10 +6,15 @@
 //   warps 0-3, 4-7   softmax of a tile, one thread to a row: scores out of TMEM, weights back into TMEM in their place, where the values' MMAs take them as their first operand
 //   warps 8-11       codes of K and V from the pages into f16 tiles, three of each: the codes are turned once for both tiles
 //   warps 12, 13     one thread of each issues the MMAs of the scores, up to two blocks ahead of the softmax, and those of the values
-// What was tried, 4 x 1024 tokens of 32 heads of 128 behind 5000 keys: one thread for all MMAs and the weights through shared memory 445 us (the thread needs some 70 cycles per MMA: it
-// was the bound); two CTAs of one tile per SM, blocks of 128 keys with the scores behind the values 433 us (half of a CTA's time is MMAs, during which its softmax waits), blocks
-// of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); this one @@.
-// What bounds it: @@
+// Where there are fewer such CTAs than SMs, a cluster of 2, 4 or 8 shares the keys: each leaves its sums in its shared memory, in the place of its operands, and joins some of the rows
+// over distributed shared memory.
+// What was tried, f16, 4 prompts of up to 1024 tokens, 32 heads of 128, behind 5000 keys: one thread for all MMAs and the weights through shared memory 445 us (the thread needs some 70
+// cycles per MMA: it was the bound); two CTAs of one tile per SM, blocks of 128 keys with the scores behind the values 433 us (half of a CTA's time is MMAs, during which its softmax
+// waits), blocks of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); as it is 330 us, 0.70 PFLOP/s.
+// What bounds it there: instructions (half of all issue slots: a score is scaled, compared, exponentiated and packed, a code turned) beside the tensor pipe (half of its time), which
+// wait for one another at the ends of a block; 256 CTAs on 148 SMs leave a tenth of the time to the last ones.
+// 16 prompts of up to 512 tokens, fp32, 32 heads of 64: 90 us.  A CTA has 4 blocks on average, so starting (queries turned into f16 pairs) and storing are half of it; with the pages
+// looked at before the queries, not beside them, 95 us.
 // The output sums stay in TMEM.  They are brought under a new maximum only when a row's has grown by more than 2^8 (weights are up to 2^14 then), which after the first
 // blocks hardly happens.  For fp32 results they are added to fp32 sums every four blocks: the accumulator truncates, and 256 keys are what its error allows.
 // Scales of K go into the scores' factor, scales of V into the weights, relative to the largest that the rows see.  Where scales of V span more than 2^10, or
@@ -23,7 +28,9 @@
 namespace rmlk {
 namespace paged {
 
+using umma::cluster_sync_all;
 using umma::fence_proxy_async;
+using umma::mapa_shared;
 using umma::mbar_arrive;
 using umma::mbar_init;
 using umma::mbar_wait;
@@ -55,13 +62,14 @@ struct Prompt {
     static constexpr int MAKERS = 128, THREADS = ROWS + MAKERS + 64;
     static constexpr int NBUF = 3;                         // blocks of keys, and of values, in shared memory
     static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = Q_HALF * HALVES, KV_HALF = KT * 128, KV_TILE = KV_HALF * HALVES;
-    static constexpr uint32_t Q = 0, K = TILES * PARTS * Q_TILE, V = K + NBUF * KV_TILE, ROW_SCALE = V + NBUF * KV_TILE, RED = ROW_SCALE + ROWS * 4, BARS = RED + 128,
+    static constexpr uint32_t Q = 0, K = TILES * PARTS * Q_TILE, V = K + NBUF * KV_TILE, ROW_SCALE = V + NBUF * KV_TILE, RED = ROW_SCALE + ROWS * 8, BARS = RED + 128,
                               TOTAL = BARS + 256 + 1024;
     // TMEM columns: for each tile two places for scores (64 columns) and the weights made of them (two keys to a column; fp32: the second numbers behind the first), sums and (fp32)
     // kept sums
     static constexpr uint32_t O_AT = 256, O_PITCH = 128, KEPT = D;
     static constexpr int FLUSH = 4;  // (fp32) blocks per accumulation
     static_assert(TOTAL <= 227 * 1024, "shared memory budget exceeded");
+    static_assert(ROWS * D * 4 <= ROW_SCALE, "a CTA's sums take the place of its operands");
 };
 
 // One query row by one warp, a key after the other, in fp32: any scales, NaN for what is not finite and for a key without a page.
@@ -127,6 +135,8 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 
 // D[tmem] (+)= A x B, kind::f16, issued by one thread.  Descriptors: their lower halves (addresses) vary, their upper halves are the same for all tiles here.
 constexpr uint32_t DESC_UPPER = (1024 >> 4) | (1u << 14) | (2u << 29);  // 1 KB between groups of 8 rows, version 1, 128-byte swizzle
+// (shared addresses of a cluster's CTAs hold their rank in the upper bits)
+__device__ __forceinline__ uint32_t desc_lower(uint32_t address, uint32_t distance) { return (address & 0x3ffffu) >> 4 | distance << 16; }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
@@ -156,8 +166,9 @@ __device__ __forceinline__ uint4 eight_f16(uint32_t w0, uint32_t w1) {
     return make_uint4(two(w0, 0x4140), two(w0, 0x4342), two(w1, 0x4140), two(w1, 0x4342));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const Cache c, const Batch q, const Attend a) {
+// SHARED: a cluster of `cluster` CTAs shares the keys of each tile pair
+template <typename T, int D, bool SHARED>
+__global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const Cache c, const Batch q, const Attend a, const int cluster) {
     using L = Prompt<T, D>;
     constexpr int TILES = L::TILES, HALVES = L::HALVES, PARTS = L::PARTS, KT = L::KT, ROWS = L::ROWS, GROUPS = L::GROUPS, NBUF = L::NBUF;
     dep_sync();
@@ -181,8 +192,18 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // ---- which rows: sequence by sequence, the tiles that see most first ----
-    const int h = static_cast<int>(blockIdx.x % c.kv_heads);
-    int b = 0, item = static_cast<int>(blockIdx.x / c.kv_heads);
+    const int splits = SHARED ? cluster : 1;
+    const int problem = static_cast<int>(blockIdx.x) / splits, share = static_cast<int>(blockIdx.x) - problem * splits;  // the CTAs of a cluster share the keys
+    const int h = problem % c.kv_heads;
+    int b = 0, item = problem / c.kv_heads;
+    // (CTAs of a cluster see the same and leave here together; should what they read change meanwhile, the others find this one's memory still there)
+    auto leave = [&]() {
+        if constexpr (SHARED) {
+            __syncwarp();
+            cluster_sync_all();
+            cluster_sync_all();
+        }
+    };
     int64_t first = 0, count = 0;
     if (!q.starts) {
         const int per = (q.each * a.group + ROWS - 1) / ROWS;
@@ -214,7 +235,10 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 item -= __shfl_sync(0xffffffffu, upto, 31);
             }
         }
-        if (!found) return;
+        if (!found) {
+            leave();
+            return;
+        }
     }
     const int rows = static_cast<int>(min(count * a.group - static_cast<int64_t>(item) * ROWS, static_cast<int64_t>(ROWS)));  // valid rows from row0 on
     const int row0 = item * ROWS;
@@ -228,8 +252,10 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     const int seen = max(sees_of(row0 + rows - 1), 0);  // keys that the last row sees
     const int32_t* table = q.table + static_cast<int64_t>(b) * q.width;
 
-    // blocks of each tile: the second one's rows see at least as much as the first one's
-    const int blocks = (seen + KT - 1) / KT, blocks0 = rows > 128 ? (max(sees_of(row0 + 127), 0) + KT - 1) / KT : blocks, blocks1 = rows > 128 ? blocks : 0;
+    // this CTA's blocks, from key0 on, and those of each tile: the second one's rows see at least as much as the first one's
+    const int all_blocks = (seen + KT - 1) / KT, each_blocks = (all_blocks + splits - 1) / splits, block0 = min(share * each_blocks, all_blocks), key0 = block0 * KT;
+    const int blocks = min(each_blocks, all_blocks - block0);
+    const int blocks0 = rows > 128 ? min(max((sees_of(row0 + 127) + KT - 1) / KT - block0, 0), blocks) : blocks, blocks1 = rows > 128 ? blocks : 0;
     const bool negative = a.scale < 0.f;  // scores' factors are not below zero: the sign goes to the queries
     int* status = a.status;
     constexpr int OTHERS = L::MAKERS + 64, FIRST = ROWS / 32;  // threads and first warp that are not the softmax's
@@ -344,11 +370,12 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         }
         v_top = __uint_as_float(top);
         if (!(__uint_as_float(low) * 1024.f >= v_top) || low == 0 || seen == 0) {
-            for (int r = warp; r < rows; r += L::THREADS / 32) {
+            for (int r = warp + share * (L::THREADS / 32); r < rows; r += splits * (L::THREADS / 32)) {
                 const int row = row0 + r, token = token_of(row);
                 row_in_fp32<T, D>(c, q, a, b, first + token, h * a.group + row - token * a.group, sees_of(row));
             }
             if (warp == FIRST + 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "n"(512) : "memory");
+            leave();
             return;
         }
         if (v_top == 0.f) v_top = 1.f;
@@ -369,7 +396,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         int page_next = 0;
         float ks_next = 0.f, vs_next = 0.f;
         auto page_of = [&](int j) {
-            const int key = j * KT + lane * 16;
+            const int key = key0 + j * KT + lane * 16;
             page_next = -1;
             if (lane < GROUPS && key < seen) page_next = table[key >> c.page_log];
         };
@@ -392,8 +419,8 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             const bool even = __all_sync(0xffffffffu, vs == 1.f);  // all scales of V are the largest
             scales_of();
             page_of(j + 2);
-            const bool hidden = (j + 1) * KT > least;
-            const int see = sees - j * KT;
+            const bool hidden = key0 + (j + 1) * KT > least;
+            const int see = sees - key0 - j * KT;
             ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, j & 1), (j >> 1) & 1, abort_flag, status));
             if (!ok) break;
             tc_fence_after();
@@ -511,7 +538,9 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         // ---- results ----
         if (ok && own_blocks > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(t), (own_blocks - 1) & 1, abort_flag, status));
         tc_fence_after();
-        const float inv = 1.f / sum * v_top;
+        // (the sums of a share go to where the operands of both tiles were)
+        if constexpr (SHARED) asm volatile("bar.sync 3, %0;" ::"n"(ROWS) : "memory");
+        const float inv = SHARED ? v_top : 1.f / sum * v_top;
         const int row = row0 + r, token = token_of(row);
         T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D;
 #pragma unroll 1
@@ -527,7 +556,13 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             } else {
                 tmem_wait_ld();
             }
-            if (r < rows) {
+            if constexpr (SHARED) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 x = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                    *reinterpret_cast<float4*>(sm + r * (D * 4) + ((((i + e) >> 2) ^ (r & 7)) << 4)) = own_blocks > 0 ? x : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            } else if (r < rows) {
 #pragma unroll
                 for (int e = 0; e < 32; e++) o[e] = __float_as_uint(!ok ? __int_as_float(0x7fc00000) : sees <= 0 ? 0.f : __uint_as_float(o[e]) * inv);
 #pragma unroll
@@ -543,6 +578,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 }
             }
         }
+        if constexpr (SHARED) reinterpret_cast<float2*>(sm + L::ROW_SCALE)[r] = make_float2(top, ok ? sum : __int_as_float(0x7fc00000));
         tc_fence_before();
     } else if (maker) {
         // ---------------- codes to f16 tiles: 16-byte pieces of a key, a thread always the same piece, of keys own_key + i STEP ----------------
@@ -554,7 +590,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         auto look_up = [&](int j) {
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const int key = j * KT + own_key + i * STEP;
+                const int key = key0 + j * KT + own_key + i * STEP;
                 page[i] = key < seen ? table[key >> c.page_log] : -1;
             }
         };
@@ -563,7 +599,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             for (int i = 0; i < N; i++) {
                 x[i] = make_uint4(0u, 0u, 0u, 0u);  // (keys that no row sees)
                 if (page[i] >= 0)
-                    x[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(page[i]) * page_bytes + head + ((j * KT + own_key + i * STEP) & (c.page - 1)) * D);
+                    x[i] = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(page[i]) * page_bytes + head + ((key0 + j * KT + own_key + i * STEP) & (c.page - 1)) * D);
             }
         };
         auto put = [&](uint32_t tile, const uint4 (&x)[N]) {
@@ -605,7 +641,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         // ---------------- MMAs of the scores: lower halves of descriptors are address / 16, and for the values the distance between blocks of 64 dims ----------------
         if (lane == 0) {
             constexpr uint32_t qk = (1u << 4) | ((KT >> 3) << 17) | ((128 >> 4) << 24);
-            const uint32_t q_desc = (base + L::Q) >> 4 | 1u << 16, k_desc = (base + L::K) >> 4 | 1u << 16;
+            const uint32_t q_desc = desc_lower(base + L::Q, 1), k_desc = desc_lower(base + L::K, 1);
             bool ok = true;
             int i = 0;
             uint32_t phase = 0;
@@ -640,7 +676,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     } else if (lane == 0) {
         // ---------------- MMAs of the values ----------------
         constexpr uint32_t pv = (1u << 4) | (1u << 16) | ((D >> 3) << 17) | ((128 >> 4) << 24);  // keys along the rows
-        const uint32_t v_desc = (base + L::V) >> 4 | (L::KV_HALF >> 4) << 16;
+        const uint32_t v_desc = desc_lower(base + L::V, L::KV_HALF >> 4);
         bool ok = true;
         int i = 0;
         uint32_t phase = 0;
@@ -668,6 +704,42 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 phase ^= 1;
             }
         }
+    }
+    if constexpr (SHARED) {
+        // ---- the shares' sums, maxima and weights' sums joined, in the keys' order: each CTA of the cluster takes every splits-th row ----
+        __syncwarp();
+        cluster_sync_all();
+        constexpr int UNITS = D / 4, MOST = 8;
+        for (int i = tid; i < ROWS / splits * UNITS; i += L::THREADS) {
+            const int r = i / UNITS * splits + share, u = i % UNITS;
+            if (r >= rows) break;
+            const uint32_t of_row = base + L::ROW_SCALE + r * 8, of_sums = base + r * (D * 4) + ((u ^ (r & 7)) << 4);
+            float2 part[MOST];  // a share's maximum and its weights' sum
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int p = 0; p < MOST; p++)
+                if (p < splits) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(part[p].x), "=f"(part[p].y) : "r"(mapa_shared(of_row, p)));
+#pragma unroll
+            for (int p = 0; p < MOST; p++)
+                if (p < splits) top = fmaxf(top, part[p].x);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int p = 0; p < MOST; p++)
+                if (p < splits) {
+                    const float f = part[p].x == -INFINITY ? 1.f : ex2(part[p].x - top);  // (no keys: sums of zero, or NaN, which has to stay)
+                    float4 x;
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(mapa_shared(of_sums, p)));
+                    sum = fmaf(part[p].y, f, sum);
+                    o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z), fmaf(x.w, f, o.w));
+                }
+            const int row = row0 + r, token = token_of(row);
+            const float inv = 1.f / sum;
+            o = sees_of(row) <= 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D + 4 * u;
+            if constexpr (L::F32) *reinterpret_cast<float4*>(dst) = o;
+            else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(o.x, o.y), pack_f16(o.z, o.w));
+        }
+        cluster_sync_all();  // (what is read lies in all of them)
     }
     tc_fence_before();
     __syncthreads();

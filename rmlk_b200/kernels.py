@@ -741,8 +741,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lens: torch.Tensor, tabl
     of which sees the sequence up to itself: one token per sequence, a few, or whole prompts (lens, table, starts as for paged_append, by which
     their keys and values are in the cache already) -> [tokens, q_heads, head_dim].  A row that sees nothing is 0; one that sees a token without a
     valid page is NaN and status [1] int32 becomes 1.  workspace: see paged_attention_workspace; without one the call makes its own.
-    Without starts a few rows per sequence share all SMs between them; with starts each sequence is walked along by itself: single tokens beside
-    whole prompts are best given to a call of their own."""
+    Without starts a few rows per sequence share all SMs between them; with starts at most eight SMs walk along one sequence and head: single tokens
+    beside whole prompts are best given to a call of their own."""
     dev = _device_of("paged_attention", cache.k)
     c, shape, at = _paged("paged_attention", dev, cache, lens, table, starts, status)
     dtype, qs = q.dtype, q.shape

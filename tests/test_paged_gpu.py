@@ -231,6 +231,63 @@ def K_uniform(q, cache, lens, table, d, starts, new, total):
     yield K.paged_attention(x, cache, n, t, 1 / math.sqrt(d)), E.attention(x, cache, n, t, 1 / math.sqrt(d))
 
 
+@pytest.mark.parametrize("new,total", [([40], [5000]), ([300], [300]), ([1, 20], [3000, 513]), ([9, 0, 3], [2000, 0, 1]), ([130, 257], [1500, 4000]), ([33], [20])])
+@pytest.mark.parametrize("page,d,group,kv,dtype", [(16, 64, 4, 1, torch.float32), (64, 128, 1, 2, torch.float32), (32, 64, 8, 1, torch.float16), (128, 128, 6, 1, torch.float16)])
+def test_few_prompts_share_their_keys(cuda, new, total, page, d, group, kv, dtype):
+    """So few that clusters of CTAs share the keys of each: shares that see nothing of the keys or only for some rows, sequences of a share or less."""
+    g = _gen(page, d, len(new), total[0])
+    cache, table, lens = E.make(kv, page, d, total, cuda, g, width=5000 // page + 1)
+    starts = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device=cuda)
+    q = torch.randn(sum(new) + 1, kv * group, d, generator=g).to(dtype).to(cuda)
+    out = torch.full_like(q, 9.0)
+    _attend(q, cache, lens, table, 1 / math.sqrt(d), starts, out=out)
+    assert bool((out[-1] == 9).all())
+    _attend(4 * q, cache, lens, table, -0.3, starts)
+    table[:, 0] = table[0, 0].clone()  # the same beginning for all
+    _attend(q, cache, lens, table, 1 / math.sqrt(d), starts)
+
+
+def test_shared_keys_of_any_scale(cuda):
+    """Poisoned blocks, scales of V of any size, queries that are not finite: where clusters share the keys, too."""
+    from rmlk_b200 import kernels as K
+    for d, dtype in ((64, torch.float32), (128, torch.float16)):
+        g = _gen(21, d)
+        cache, table, n = E.make(2, 64, d, [3000, 900], cuda, g)
+        starts = torch.tensor([0, 100, 140], dtype=torch.int32, device=cuda)
+        q = torch.randn(140, 8, d, generator=g).to(dtype).to(cuda)
+        q[7, 3, 5], q[120, 0, 0] = math.nan, math.inf
+        out = K.paged_attention(q, cache, n, table, d ** -0.5, starts=starts)
+        want, bound = E.attention(q.nan_to_num(0.0, 0.0), cache, n, table, d ** -0.5, starts)
+        want[7, 3], want[120, 0] = math.nan, math.nan
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        E.close(out, want, bound)
+        q = torch.randn(140, 8, d, generator=g).to(dtype).to(cuda)
+        for spread in ((-60, 40), (-9, 0)):
+            cache.v_scales.copy_(torch.exp2(torch.randint(*spread, cache.v_scales.shape, generator=g).float()))
+            if spread[0] > -20 or dtype == torch.float32:
+                _attend(q, cache, n, table, d ** -0.5, starts)
+        cache.v_scales.fill_(0.125)
+        cache.k_scales[table[0, 46], 1] = math.nan  # tokens 2944 .. 2999, of which the first 44 are seen by all rows
+        out = K.paged_attention(q, cache, n, table, d ** -0.5, starts=starts)
+        cache.k_scales[table[0, 46], 1] = 0.125
+        want, bound = E.attention(q, cache, n, table, d ** -0.5, starts)
+        want[44:100, 4:] = math.nan
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        E.close(out, want, bound)
+
+
+def test_queries_are_rotated_in_place(cuda):
+    from rmlk_b200 import kernels as K
+    g = _gen(22)
+    cos, sin = _tables(100, 64, cuda)
+    for dtype, new in ((torch.float32, 1), (torch.float16, 40)):
+        cache, table, lens = E.make(2, 16, 64, [90, 50, 41], cuda, g)
+        q, k, v = (torch.randn(3 * new, h, 64, generator=g).to(dtype).to(cuda) for h in (6, 2, 2))
+        want = K.paged_append(cache, k, v, lens, table, cos, sin, q=q)
+        got = K.paged_append(cache, k, v, lens, table, cos, sin, q=q, q_out=q)
+        assert got is q and torch.equal(q, want)
+
+
 def test_rows_that_lie_apart(cuda):
     from rmlk_b200 import kernels as K
     g = _gen(6)
