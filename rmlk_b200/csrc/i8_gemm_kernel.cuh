@@ -138,6 +138,13 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
     const uint32_t tmem = *tmem_slot;
 
     int sums[SPLIT ? MT / (L::EPI_WARPS / 4) : 1];  // (SPLIT) this warp's sums: MT / 2 tokens of 32 channels
+    // (SPLIT) what an epilogue thread writes: tokens at0, at0 + ROWS, ... of the `here` ones of this CTA, m0 + (those << log_splits), of channel n
+    constexpr int ROWS = L::EPI_WARPS * 32 / BN, MOST = SPLIT ? MT / 2 / ROWS : 1;
+    const Tile own = tile_at(SPLIT ? first : 0, p);
+    const int per = MT >> log_splits, channel = (static_cast<int>(threadIdx.x) - 64) & (BN - 1), at0 = (static_cast<int>(threadIdx.x) - 64) / BN;
+    const int64_t n = static_cast<int64_t>(own.n_tile) * BN + channel, m0 = static_cast<int64_t>(own.m_tile) * MT + rank;
+    const int here = static_cast<int>(min(static_cast<int64_t>(per), (p.M - m0 + splits - 1) >> log_splits));
+    float sx[MOST], sw = 0.f;
     if (warp == 0) {
         // ---------------- loads ----------------
         if (lane == 0) {
@@ -200,6 +207,11 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
         const uint32_t lane_field = static_cast<uint32_t>(sub * 32) << 16;
         const uint32_t pair_empty = CG == 2 ? mapa_shared(acc_empty(0), 0) : acc_empty(0);
         dep_wait();  // scales and outputs may belong to kernels before this one
+        if constexpr (SPLIT) {  // (asked for one by one at the end, the scales of 64 tokens took 4 us)
+            if (n < p.N) sw = __ldg(p.sw + n);
+#pragma unroll
+            for (int i = 0; i < MOST; i++) sx[i] = at0 + i * ROWS < here ? __ldg(p.sx + m0 + ((at0 + i * ROWS) << log_splits)) : 0.f;
+        }
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -253,27 +265,27 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
 #pragma unroll
             for (int j = 0; j < HM; j++) {
                 const int token = part * HM + j;
-                if (token >= tokens) break;
                 const uint32_t addr = mapa_shared(at + (token >> log_splits) * (BN * 4), token & (splits - 1));
-                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(sums[j]) : "memory");
+                if (token < tokens) asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(sums[j]) : "memory");
             }
         }
     }
     if constexpr (SPLIT) {
         __syncwarp();
         cluster_sync_all();
-        if (warp >= 2 && !*abort_flag) {
-            const int per = MT >> log_splits;
-            const int* s = reinterpret_cast<const int*>(base_ptr + L::SUMS);
-            const Tile t = tile_at(first, p);
-            const int e = threadIdx.x - 64, channel = e % BN;
-            const int64_t n = static_cast<int64_t>(t.n_tile) * BN + channel;
-            for (int at = e / BN; at < per; at += L::EPI_WARPS * 32 / BN) {
-                const int64_t m = static_cast<int64_t>(t.m_tile) * MT + (at << log_splits) + rank;
-                if (m >= p.M || n >= p.N) break;
-                int sum = 0;
-                for (int r = 0; r < splits; r++) sum += s[(r * per + at) * BN + channel];
-                static_cast<Out*>(p.out)[m * p.ldo + n] = static_cast<Out>(scaled(sum, __ldg(p.sx + m), __ldg(p.sw + n)));
+        if (warp >= 2 && !*abort_flag && n < p.N) {
+            const int* s = reinterpret_cast<const int*>(base_ptr + L::SUMS) + channel;
+            int sum[MOST] = {};
+#pragma unroll 1
+            for (int r = 0; r < splits; r++) {
+#pragma unroll
+                for (int i = 0; i < MOST; i++)
+                    if (at0 + i * ROWS < here) sum[i] += s[(r * per + at0 + i * ROWS) * BN];
+            }
+            Out* o = static_cast<Out*>(p.out) + n;
+#pragma unroll
+            for (int i = 0; i < MOST; i++) {
+                if (at0 + i * ROWS < here) o[(m0 + ((at0 + i * ROWS) << log_splits)) * p.ldo] = static_cast<Out>(scaled(sum[i], sx[i], sw));
             }
         }
     }

@@ -14,8 +14,11 @@
 namespace rmlk {
 namespace quant {
 
+struct RowScale;
+__device__ __noinline__ uint32_t exact_codes(RowScale r, float x0, float x1, float x2, float x3);
+
 struct RowScale {
-    float s, inv, up;  // of values times `up`
+    float s, up, by;  // the scale, times `up`; a value times `by` is the quotient
     bool bad;
     // from the largest magnitude's bits
     __device__ __forceinline__ float set(uint32_t most) {
@@ -23,22 +26,43 @@ struct RowScale {
         const float scale = fmaxf(__fdiv_rn(__uint_as_float(most), 127.f), 1.17549435e-38f);
         up = scale < 7.888609052210118e-31f ? 16777216.f : 1.f;  // below 2^-100 differences would round to zero: all times 2^24
         s = scale * up;
-        inv = __frcp_rn(s);
+        by = __frcp_rn(s) * up;
         return bad ? __int_as_float(0x7fc00000) : scale;
     }
+    // the quotient rounded to an integer in the lowest bits, nearly always the right one
+    __device__ __forceinline__ float rounded(float x) const { return fmaf(x, by, 12582912.f); }  // 1.5 2^23
+    __device__ __forceinline__ bool near_middle(float x, float sum) const { return fabsf(fmaf(x, by, -(sum - 12582912.f))) > 0.4999f; }
+    __device__ __forceinline__ int exact(float x) const {
+        const float v = x * up;
+        float c = rounded(x) - 12582912.f;
+        const float above = fmaf(-(c + 0.5f), s, v), below = fmaf(-(c - 0.5f), s, v);
+        const bool odd = static_cast<int>(c) & 1;
+        if (above > 0.f || (above == 0.f && odd)) c += 1.f;
+        else if (below < 0.f || (below == 0.f && odd)) c -= 1.f;
+        return static_cast<int>(c);
+    }
     __device__ __forceinline__ int code(float x) const {
-        const float v = x * up, sum = fmaf(v, inv, 12582912.f);  // 1.5 2^23: the sum is rounded to an integer
-        float c = sum - 12582912.f;
-        if (fabsf(fmaf(v, inv, -c)) > 0.4999f) {
-            const float above = fmaf(-(c + 0.5f), s, v), below = fmaf(-(c - 0.5f), s, v);
-            const bool odd = static_cast<int>(c) & 1;
-            if (above > 0.f || (above == 0.f && odd)) c += 1.f;
-            else if (below < 0.f || (below == 0.f && odd)) c -= 1.f;
-            return static_cast<int>(c);
+        const float sum = rounded(x);
+        return bad ? 0 : near_middle(x, sum) ? exact(x) : __float_as_int(sum);  // (its lowest byte)
+    }
+    // four codes as the bytes of a word
+    __device__ __forceinline__ uint32_t codes(const float (&x)[4]) const {
+        float sum[4];
+        bool near = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            sum[i] = rounded(x[i]);
+            near = near || near_middle(x[i], sum[i]);
         }
-        return __float_as_int(sum);  // (its lowest byte)
+        if (near) return exact_codes(*this, x[0], x[1], x[2], x[3]);  // (one word in a thousand)
+        const uint32_t w = __byte_perm(__byte_perm(__float_as_uint(sum[0]), __float_as_uint(sum[1]), 0x0040), __byte_perm(__float_as_uint(sum[2]), __float_as_uint(sum[3]), 0x0040), 0x5410);
+        return bad ? 0u : w;
     }
 };
+
+__device__ __noinline__ uint32_t exact_codes(RowScale r, float x0, float x1, float x2, float x3) {
+    return __byte_perm(__byte_perm(r.code(x0), r.code(x1), 0x0040), __byte_perm(r.code(x2), r.code(x3), 0x0040), 0x5410);
+}
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
@@ -66,7 +90,6 @@ __global__ void __launch_bounds__(GROUP > 256 ? GROUP : 256) packs_kernel(const 
     const int me = threadIdx.x % GROUP;
     const T* xr = x + row * ldx;
     Pack<T, V> p[ITERS];
-    uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < ITERS; i++) {
         const int at = (i * GROUP + me) * V;
@@ -77,10 +100,20 @@ __global__ void __launch_bounds__(GROUP > 256 ? GROUP : 256) packs_kernel(const 
             for (int e = 0; e < V; e++) p[i].v[e] = at + e < cols ? xr[at + e] : static_cast<T>(0.f);
         }
     }
+    uint32_t most = 0;
+    if constexpr (sizeof(T) == 2) {  // magnitudes of f16 are in the order of their bits: two at a time
+        uint32_t m2 = 0;
 #pragma unroll
-    for (int i = 0; i < ITERS; i++)
+        for (int i = 0; i < ITERS; i++)
 #pragma unroll
-        for (int e = 0; e < V; e++) most = max(most, magnitude(static_cast<float>(p[i].v[e])));
+            for (int e = 0; e < V; e += 2) m2 = __vmaxu2(m2, reinterpret_cast<const uint32_t&>(p[i].v[e]) & 0x7fff7fffu);
+        most = magnitude(__half2float(__ushort_as_half(static_cast<unsigned short>(max(m2 & 0xffffu, m2 >> 16)))));
+    } else {
+#pragma unroll
+        for (int i = 0; i < ITERS; i++)
+#pragma unroll
+            for (int e = 0; e < V; e++) most = max(most, magnitude(static_cast<float>(p[i].v[e])));
+    }
     most = group_max<GROUP>(most, s_max);
     RowScale r;
     const float scale = r.set(most);
@@ -91,7 +124,10 @@ __global__ void __launch_bounds__(GROUP > 256 ? GROUP : 256) packs_kernel(const 
         if (at >= cols) continue;
         Pack<int8_t, V> c;
 #pragma unroll
-        for (int e = 0; e < V; e++) c.v[e] = r.bad ? 0 : static_cast<int8_t>(r.code(static_cast<float>(p[i].v[e])));
+        for (int e = 0; e < V; e += 4) {
+            const float x[4] = {static_cast<float>(p[i].v[e]), static_cast<float>(p[i].v[e + 1]), static_cast<float>(p[i].v[e + 2]), static_cast<float>(p[i].v[e + 3])};
+            reinterpret_cast<uint32_t&>(c.v[e]) = r.codes(x);
+        }
         int8_t* to = codes + row * ldc + at;
         if (at + V <= cols) {
             store_pack<int8_t, V>(to, c);
@@ -116,7 +152,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const T* __restrict__ x, int6
     RowScale r;
     const float scale = r.set(most);
     if (threadIdx.x == 0) scales[row] = scale;
-    for (int64_t i = threadIdx.x; i < cols; i += 256) codes[row * ldc + i] = r.bad ? 0 : static_cast<int8_t>(r.code(static_cast<float>(xr[i])));
+    for (int64_t i = threadIdx.x; i < cols; i += 256) codes[row * ldc + i] = static_cast<int8_t>(r.code(static_cast<float>(xr[i])));
 }
 
 template <typename T, int GROUP, int ITERS>
@@ -133,7 +169,7 @@ static void quantize(cudaStream_t st, const T* x, int64_t ldx, int64_t rows, int
     if (!whole) launch_dep(rows_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, st, x, ldx, cols, codes, ldc, scales);
     else if (loads <= 32) packs<T, 32, 1>(st, x, ldx, rows, cols, codes, ldc, scales);
     else if (loads <= 64) packs<T, 32, 2>(st, x, ldx, rows, cols, codes, ldc, scales);
-    else if (loads <= 256 && rows > 2 * sm_count()) packs<T, 32, 8>(st, x, ldx, rows, cols, codes, ldc, scales);  // (with few rows, more threads to each)
+    else if (V == 4 && loads <= 256 && rows > 2 * sm_count()) packs<T, 32, 8>(st, x, ldx, rows, cols, codes, ldc, scales);  // (with few rows, more threads to each)
     else if (loads <= 256) packs<T, 256, 1>(st, x, ldx, rows, cols, codes, ldc, scales);
     else if (loads <= 512) packs<T, 256, 2>(st, x, ldx, rows, cols, codes, ldc, scales);
     else if (loads <= 1024) packs<T, 256, 4>(st, x, ldx, rows, cols, codes, ldc, scales);
