@@ -8,11 +8,11 @@
 //   warps 12, 13     one thread of each issues the MMAs of the scores, up to two blocks ahead of the softmax, and those of the values
 // Where there are fewer such CTAs than SMs, a cluster of 2, 4 or 8 shares the keys: each leaves its sums in its shared memory, in the place of its operands, and joins some of the rows
 // over distributed shared memory.
-// What was tried, f16, 4 prompts of up to 1024 tokens, 32 heads of 128, behind 5000 keys: one thread for all MMAs and the weights through shared memory 445 us (the thread needs some 70
+// What was tried, f16, 4 prompts of up to 1024 tokens, 32 heads of 128, behind up to 5000 keys: one thread for all MMAs and the weights through shared memory 445 us (the thread needs some 70
 // cycles per MMA: it was the bound); two CTAs of one tile per SM, blocks of 128 keys with the scores behind the values 433 us (half of a CTA's time is MMAs, during which its softmax
 // waits), blocks of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); as it is 330 us, 0.70 PFLOP/s.
-// What bounds it there: instructions (half of all issue slots: a score is scaled, compared, exponentiated and packed, a code turned) beside the tensor pipe (half of its time), which
-// wait for one another at the ends of a block; 256 CTAs on 148 SMs leave a tenth of the time to the last ones.
+// What bounds it there: instructions (49 % of all issue slots: a score is scaled, compared, exponentiated and packed, a code turned) beside the tensor pipe (36 % of its cycles), which
+// wait for one another at the ends of a block.
 // 16 prompts of up to 512 tokens, fp32, 32 heads of 64: 90 us.  A CTA has 4 blocks on average, so starting (queries turned into f16 pairs) and storing are half of it; with the pages
 // looked at before the queries, not beside them, 95 us.
 // The output sums stay in TMEM.  They are brought under a new maximum only when a row's has grown by more than 2^8 (weights are up to 2^14 then), which after the first

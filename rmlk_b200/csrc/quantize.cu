@@ -7,8 +7,8 @@
 // lies within 1e-4 of a middle the sign of fma(-(c +- 1/2), s, x), which rounds once and so cannot change it, says on which side x is.
 //
 // What bounds it: HBM, one read of x (4 or 2 bytes per element) and one byte written.  A row stays in registers between its maximum and its codes: a warp to a row of up to
-// 1024 values (2048 in f16), else a CTA; rows off 16-byte boundaries, and longer than a CTA's registers, are read twice.
-// [4096, 4096] f16: 28 us read twice and value by value.
+// 256 values (512 in f16; 1024 in f32 where rows are many), else a CTA; rows off 16-byte boundaries, and longer than a CTA's registers, are read twice.
+// [4096, 14336] f16: 37 us, 4.7 TB/s; with a branch for each value instead of each four 64.  [4096, 4096] f16: 13 us, read twice 28.  [16384, 4096] f32: 55 us, 6.1 TB/s.
 #include "common.cuh"
 
 namespace rmlk {
@@ -169,7 +169,7 @@ static void quantize(cudaStream_t st, const T* x, int64_t ldx, int64_t rows, int
     if (!whole) launch_dep(rows_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, st, x, ldx, cols, codes, ldc, scales);
     else if (loads <= 32) packs<T, 32, 1>(st, x, ldx, rows, cols, codes, ldc, scales);
     else if (loads <= 64) packs<T, 32, 2>(st, x, ldx, rows, cols, codes, ldc, scales);
-    else if (V == 4 && loads <= 256 && rows > 2 * sm_count()) packs<T, 32, 8>(st, x, ldx, rows, cols, codes, ldc, scales);  // (with few rows, more threads to each)
+    else if (V == 4 && loads <= 256 && rows > 2 * sm_count()) packs<T, 32, 8>(st, x, ldx, rows, cols, codes, ldc, scales);  // ([4096, 1024] 5.4 us, with CTAs 6.5; f16, [4096, 2048]: 14.3, with CTAs 8.2)
     else if (loads <= 256) packs<T, 256, 1>(st, x, ldx, rows, cols, codes, ldc, scales);
     else if (loads <= 512) packs<T, 256, 2>(st, x, ldx, rows, cols, codes, ldc, scales);
     else if (loads <= 1024) packs<T, 256, 4>(st, x, ldx, rows, cols, codes, ldc, scales);
