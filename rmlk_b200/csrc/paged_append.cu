@@ -8,8 +8,8 @@
 // that after any number of steps a code is off by less than one step of the final scale (1/2 + 1/4 + ...); ratios of any size would add half a step
 // each time.  It costs up to one bit of the eight (a scale of max / 127 is up to twice as fine).
 //
-// What bounds it: HBM, q, k, v and the tables' rows read and q and the codes written once.  5600 tokens of 32 + 8 + 8 heads of 128, f16: 38 us, 3.5 TB/s; the values wait in
-// registers for their block's maximum (80 registers: 34 % of the warps), and the keys' conversions to fp64 and back take their time beside the loads.
+// What bounds it: HBM, q, k, v and the tables' rows read and q and the codes written once.  5600 tokens of 32 + 8 + 8 heads of 128, f16: 35 us, 3.8 TB/s; the values wait in
+// registers for their block's maximum (64 of them with a few spilled, 38 us with the 80 that it would take), and the keys' conversions to fp64 and back take their time.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -126,7 +126,7 @@ __device__ __forceinline__ uint32_t codes_of(float4 x, float inv) {
 // An item: the new tokens of a sequence that fall into one page, as K or V of one head, or the queries of some heads.  GROUP threads to an item; a thread has four dims of
 // the lower half of a head and the four that go with them in the upper half, of every (GROUP / (D / 8))-th token: values stay in registers from their maximum to their codes.
 template <typename T, int D, int GROUP, int ITERS>
-__global__ void __launch_bounds__(256) append_kernel(const Cache c, const Batch q, const Append a) {
+__global__ void __launch_bounds__(256, ITERS <= 2 ? 4 : 2) append_kernel(const Cache c, const Batch q, const Append a) {
     dep_sync();
     constexpr int PACKS = D / 8, AT_ONCE = GROUP / PACKS, HALF = D / 2;
     __shared__ uint32_t s_max[8];
