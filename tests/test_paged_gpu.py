@@ -472,6 +472,38 @@ def test_graphs_and_streams(cuda):
         E.close(out, want, bound)
 
 
+def test_calls_side_by_side(cuda):
+    """Single tokens, a few prompts (clusters) and many, captured each on a stream of its own and replayed at the same time over one cache, with a workspace each."""
+    from rmlk_b200 import kernels as K
+    g = _gen(23)
+    calls = []
+    lens = [700, 90, 2000, 1, 300, 512]
+    cache, table, n = E.make(2, 32, 64, lens, cuda, g)
+    for new in ([1] * 6, [40, 7, 64, 1, 90, 33], [700, 90, 1500, 1, 300, 512]):
+        starts = torch.tensor([sum(new[:b]) for b in range(7)], dtype=torch.int32, device=cuda) if max(new) > 1 else None
+        q = torch.randn(sum(new), 8, 64, generator=g).to(torch.float16).to(cuda)
+        calls.append((q, cache, n, table, 0.125, starts, torch.empty_like(q), K.paged_attention_workspace(q, cache, 6, starts is not None)))
+    alone = [K.paged_attention(*c).clone() for c in calls]
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream() for _ in calls], []
+    for s, c in zip(streams, calls):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            K.paged_attention(*c)
+            K.paged_attention(*c)
+        graphs.append(graph)
+    for c in calls:
+        c[6].zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for c, want in zip(calls, alone):
+        assert torch.equal(c[6], want)
+
+
 def test_a_decoder_layer(cuda):
     """A prompt and a few steps as a program runs them: quantised projections, append, attention, output projection; against the same
     in 64 bits on the codes and scales that the operators left."""
