@@ -135,7 +135,10 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
     if (takes_few(dtype == RMLK_F32, tokens, batch, c.kv_heads, a.group, c.d, s.width << c.page_log, starts != nullptr)) {
         if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
             return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
-        const bool one = s.each * a.group <= 8;
+        // tiles of 8 or 16 rows; one of 16 takes 1.4 times as long.  24 x 4 tokens, 6 heads of 128 to each of 4, 1500 keys, f16: three of 8 27 us, two of 16 29; 16 rows: 22, 18; 40 rows
+        // (2 requests, 8 KV heads, 20000 keys): 61, 60
+        const int rows = s.each * a.group;
+        const bool one = rows <= 8 || (rows > 16 && rows <= 24);
         if (dtype == RMLK_F32) {
             if (c.d == 64) return one ? paged::launch_few<float, 64, 1>(st, c, s, a, workspace) : paged::launch_few<float, 64, 2>(st, c, s, a, workspace);
             return one ? paged::launch_few<float, 128, 1>(st, c, s, a, workspace) : paged::launch_few<float, 128, 2>(st, c, s, a, workspace);
