@@ -14,7 +14,9 @@
 // Both contractions are products of 8-bit integers (mma.sync m16n8k32, exact 32-bit sums), so the codes are operands as they lie there.  (As f16, four
 // instructions went into each pair of codes: 530 per step of 4 KB, and the SMs, not HBM, were the bound: 5.0 TB/s.)
 //   scores  S[16 rows x 8 keys] = Q K^T.  Queries are fixed-point numbers under a power of two per row: 15 bits and sign for f16, 22 for fp32 - half a
-//           step is 2^-15 or 2^-23 of the row's largest value - as two or three signed digits of 8 bits, a row of the MMA each.
+//           step is 2^-15 or 2^-23 of the row's largest value - as two or three signed digits of 8 bits, a row of the MMA each.  Where a row's values, none counted
+//           for more than 1/16 of its largest, are on average less than 1/43 of it (a few outliers: normally distributed values are so beside one of 34 standard deviations), digits
+//           would lose too much of them: the tile's scores are formed in fp32 from the queries themselves.
 //   values  O^T[16 dims x 8 rows] = V^T P^T.  Weights exp2(s - m), m the row's largest score in the step, are fixed-point numbers of 16 bits (f16 results) or 23
 //           (fp32): half a step is 2^-17 or 2^-24 of the largest weight of the step.  Unsigned digits, an MMA each; the accumulator fragment of S holds just the
 //           weights that the operand fragment wants, four tokens' bytes to a register, and a 4 x 4 transpose of bytes puts four tokens' codes side by side.
@@ -213,6 +215,40 @@ struct Share {
         }
     }
 };
+
+// A step's products of queries and codes in fp32, as lanes hold them: rows g (and g + 8) of the tile from row0 on, keys 8 j + 2 c4 and the next.
+template <int D, int NR>
+struct Scores {
+    float x[NR][4096 / D / 8][2];
+};
+template <typename T, int D, int NR>
+__device__ __noinline__ Scores<D, NR> scores_in_fp32(const T* q, int64_t stride, int group, int64_t first, int h, int row0, int rows, const uint8_t* keys) {
+    constexpr int J = 4096 / D / 8;
+    const int g = (threadIdx.x & 31) >> 2, c4 = threadIdx.x & 3;
+    Scores<D, NR> y;
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        const int row = row0 + g + 8 * r, token = row / group;
+        const T* src = q + (first + token) * stride + (static_cast<int64_t>(h) * group + row - token * group) * D;
+#pragma unroll
+        for (int j = 0; j < J; j++) y.x[r][j][0] = y.x[r][j][1] = 0.f;
+#pragma unroll 1
+        for (int u = 0; u < D / 4; u++) {  // four dims at a time
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = row < rows ? static_cast<float>(src[4 * u + i]) : 0.f;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(keys + j / 2 * (16 * D) + unit_at<D>(8 * (j & 1) + 2 * c4 + e, u >> 2) + 4 * (u & 3));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y.x[r][j][e] = fmaf(v[i], static_cast<float>(static_cast<int8_t>(w >> (8 * i))), y.x[r][j][e]);
+                }
+        }
+    }
+    return y;
+}
 
 template <typename T, int D, int NR>
 __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const Cache c, const Batch q, const Attend a, const int tiles, unsigned* counters, float* partials) {
@@ -423,6 +459,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
 #pragma unroll
             for (int s = 0; s < L::STAGES - 1; s++) issue();
         }
+        bool wide = false;  // a row of the tile has values that its digits would lose: scores are formed in fp32 instead
         // digits: [32 dims][row tile]: rows g and g + 8 of the lane's first four dims, then of the next four
         uint32_t qf[2 * PIECES][L::QT][4];
         if constexpr (L::F32 && NR == 1) {
@@ -453,6 +490,16 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             const float up = exp2_int(e), more = L::F32 ? 256.f : 1.f;
             // an infinity or a NaN makes NaN of the row
             factor[r] = most < 0x7f800000u ? a.scale * 1.44269504f / more * exp2_int(-e) : __int_as_float(0x7fc00000);
+            // (no condition around the sum: lanes of other rows take part in it)
+            const float limit = most < 0x7f800000u ? __uint_as_float(most) * (1.f / 16.f) : 0.f;
+            float capped = 0.f;
+#pragma unroll
+            for (int s = 0; s < 4 * PIECES; s++) {
+                const float4 x = four(s);
+                capped += (fminf(fabsf(x.x), limit) + fminf(fabsf(x.y), limit)) + (fminf(fabsf(x.z), limit) + fminf(fabsf(x.w), limit));
+            }
+            const float of_row = quad_sum(capped);
+            wide = wide | (of_row < 0.375f * D * limit);
 #pragma unroll
             for (int s = 0; s < 4 * PIECES; s++) {
                 const float4 x = four(s);
@@ -470,6 +517,11 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                     f[r][at + 1] = d0;
                 }
             }
+        }
+        wide = __any_sync(0xffffffffu, wide);
+        if (wide) {
+#pragma unroll
+            for (int r = 0; r < NR; r++) factor[r] = factor[r] == factor[r] ? a.scale * 1.44269504f : factor[r];
         }
         const int all_see = relative(min(before + 1 + (tile * ROWS) / a.group, keys));  // that every row of the tile sees
 
@@ -506,6 +558,18 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                     for (int e = 0; e < 2; e++) {
                         const float high = static_cast<float>(s[r][e] * 256 + s[r][2 + e]);
                         x[r][j][e] = (L::F32 ? fmaf(high, 256.f, static_cast<float>(s[L::QT - 1][2 * r + e])) : high) * t;
+                    }
+                }
+            }
+            if (wide) {
+                const Scores<D, NR> y = scores_in_fp32<T, D, NR>(static_cast<const T*>(a.q), a.qs, a.group, static_cast<int64_t>(b) * q.each, h, tile * ROWS, rows, at);
+#pragma unroll
+                for (int j = 0; j < KS / 8; j++) {
+                    const float ks = scales[stage * NC + j / 2].x;
+#pragma unroll
+                    for (int r = 0; r < NR; r++) {
+                        x[r][j][0] = y.x[r][j][0] * (factor[r] * ks);
+                        x[r][j][1] = y.x[r][j][1] * (factor[r] * ks);
                     }
                 }
             }

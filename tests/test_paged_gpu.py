@@ -388,6 +388,25 @@ def test_queries_of_any_size(cuda):
         _attend(q, cache, n, table, 0.0)
 
 
+def test_queries_with_outliers(cuda):
+    """A few values of a query are far larger than the rest, in dims that keys have no part in or the same in all: the rest decides the weights.
+
+    D fp32 roundings of 2^-24 each in a score, where the bound of `attention` counts D / 16 + 8 of 2^-23: at most 4 times that for D = 128."""
+    from rmlk_b200 import kernels as K
+    g = _gen(24)
+    for d, group, dtype in ((64, 4, torch.float32), (128, 3, torch.float16), (128, 16, torch.float32), (64, 9, torch.float16)):
+        for each in (1, 2, 300):
+            lens = [each + 500, each, 5000]
+            cache, table, n = E.make(2, 32, d, lens, cuda, g)
+            cache.k[..., 3], cache.k[..., 17] = 0, 0
+            for up in (3.0, 40.0, 1000.0, 30000.0):
+                q = torch.randn(3 * each, 2 * group, d, generator=g).to(dtype).to(cuda)
+                q[1::2, :, 3], q[:, 1::2, 17] = up, -up
+                out = K.paged_attention(q, cache, n, table, d ** -0.5)
+                want, bound = E.attention(q, cache, n, table, d ** -0.5)
+                E.close(out, want, 4 * bound)
+
+
 def test_pages_out_of_range(cuda):
     """A row that sees a token without a valid page is NaN and the status says so; the others have their values."""
     from rmlk_b200 import kernels as K
