@@ -25,7 +25,7 @@
 //
 // Measured: 3 requests over 50001 to 33334 keys, f16, 8 KV heads of 128: 55 us, 4.7 TB/s of the call and 6.3 to 7 TB/s between its ends; the rest is the start (which sequence,
 // which page, first data: 5 us) and the joining of the parts (4 us).  64 requests over 1000 to 508 keys, fp32, 8 heads of 64: 22 us, with the whole CTA waiting at the end of each
-// segment 24.  24 requests of 4 tokens over 2000 to 1042 keys, f16, 6 heads to each of 4: 30 us; 24 query rows are two tiles, each of which takes the keys once more, from L2.
+// segment 24.  24 requests of 4 tokens over 2000 to 1042 keys, f16, 6 heads to each of 4: 29 us; 24 query rows are three tiles of 8, each of which takes the keys once more, from L2.
 #pragma once
 
 #include "paged.cuh"
