@@ -643,12 +643,13 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             for (int pass = 0; pass < passes; pass++) {
                 const float ref = passes == 1 ? v_top : scales[stage * NC + pass].y;
                 if (!(ref > 0.f && ref < INFINITY)) continue;  // nothing but zeros (or NaN, seen to above)
-                const float per = MOST / ref;
+                // v / ref for 0 <= v <= ref: the reciprocal of a number near the lower end of fp32 would be infinite, of 2^64 times it is not
+                const float up = ref < 1.f ? 18446744073709551616.f : 1.f, per = 1.f / (ref * up);
                 uint32_t p[NR][NC][L::DIGITS];
 #pragma unroll
                 for (int n = 0; n < NC; n++) {
                     // (a page whose scale is not finite: its weights are 0, or the row is NaN already)
-                    const float v = scales[stage * NC + n].y, k = passes > 1 ? (n == pass ? MOST : 0.f) : v == ref ? MOST : v < INFINITY ? v * per : 0.f;
+                    const float v = scales[stage * NC + n].y, k = passes > 1 ? (n == pass ? MOST : 0.f) : v == ref ? MOST : v < INFINITY ? v * up * per * MOST : 0.f;
 #pragma unroll
                     for (int r = 0; r < NR; r++) {
                         // the lower bits of 2^23 + a number below 2^23 are that number
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                 }
                 float2 f[NR];
 #pragma unroll
-                for (int r = 0; r < NR; r++) f[r] = Share<D, NR>::of_sums(weight[r] * (ref * (1.f / MOST)), c4);
+                for (int r = 0; r < NR; r++) f[r] = Share<D, NR>::of_sums(weight[r] * (L::F32 ? ref : ref * (1.f / MOST)), c4);
                 uint32_t v[NC][4][D / 32];
 #pragma unroll
                 for (int n = 0; n < NC; n++)
@@ -705,7 +706,8 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                                 for (int t = 0; t < L::DIGITS; t++) mma_u8(o[t], tr[n][2 * k], tr[n][2 * k + 1], tr[n + 1][2 * k], tr[n + 1][2 * k + 1], p[r][n][t], p[r][n + 1][t]);
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const float value = L::F32 ? fmaf(static_cast<float>(o[L::DIGITS - 1][e] * 256 + o[1][e]), 256.f, static_cast<float>(o[0][e]))
+                                // (fp32: 1 / MOST goes to the digits; the scale of V, down to 2^-126, would keep next to no bits under it.  f16 has no such values.)
+                                const float value = L::F32 ? fmaf(static_cast<float>(o[L::DIGITS - 1][e] * 256 + o[1][e]), 256.f / MOST, static_cast<float>(o[0][e]) * (1.f / MOST))
                                                            : static_cast<float>(o[1][e] * 256 + o[0][e]);
                                 acc[2 * w + k][r][e] = fmaf(value, e & 1 ? f[r].y : f[r].x, acc[2 * w + k][r][e]);
                             }

@@ -1,0 +1,61 @@
+"""Attention over the paged 8-bit cache under scales of any size and sign, against 64 bits (tests/eight_bit.py has the derivation of the bounds)."""
+import math
+
+import pytest
+import torch
+
+import eight_bit as E
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(*seed):
+    g = torch.Generator()
+    g.manual_seed(sum((i + 1) * 7919 * s for i, s in enumerate(seed)))
+    return g
+
+
+def _make(kv, page, d, lens, dev, gen):
+    """As eight_bit.make, but page 0 is a stranger's: no sequence names it, its codes are large and its scales 1."""
+    from rmlk_b200 import kernels as K
+    cache, table, n = E.make(kv, page, d, lens, dev, gen)
+    cache = K.PagedCache(*(torch.cat([torch.full_like(t[:1], 127 if t.dim() == 4 else 1), t]) for t in cache))
+    return cache, torch.where(table < 0, table, table + 1).to(torch.int32), n
+
+
+def _scales(cache, low, high, gen):
+    return torch.exp2(torch.randint(low, high, cache.v_scales.shape, generator=gen).float()).to(cache.v_scales.device)
+
+
+def _attend(q, cache, n, table, d, starts=None):
+    from rmlk_b200 import kernels as K
+    return K.paged_attention(q, cache, n, table, d ** -0.5, starts=starts), *E.attention(q, cache, n, table, d ** -0.5, starts)
+
+
+@pytest.mark.parametrize("page,d,each", [(16, 64, 1), (64, 64, 4), (16, 128, 4), (32, 128, 1)])
+def test_values_that_are_tiny_throughout(cuda, page, d, each):
+    """Scales of V near the lower end of fp32, as paged_append makes them for values below 1e-30, all alike, near one another and far apart: as precise as any others.  The last
+    step of a sequence has places without keys, for which page 0 is read."""
+    g = _gen(page, d, each)
+    cache, table, n = _make(2, page, d, [each + 1, 40, 70, 300, 2983], cuda, g)
+    q = torch.randn(5 * each, 6, d, generator=g).to(cuda)
+    for low, high in ((-126, -125), (-126, -123), (-122, -102), (-110, -109), (-112, -109), (-104, -102)):
+        cache.v_scales.copy_(_scales(cache, low, high, g))
+        out, want, bound = _attend(q, cache, n, table, d)
+        E.close(out, want, bound)
+
+
+@pytest.mark.parametrize("page,d,each", [(16, 64, 1), (128, 64, 2), (32, 128, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_values_of_zero_are_zero(cuda, page, d, each, dtype):
+    """A cache that paged_append has filled with zeros has the scales 2^-126; whatever page 0 holds, the result is zero to the last bit."""
+    from rmlk_b200 import kernels as K
+    g = _gen(page, d, each)
+    lens = [each, 33, 100, 777]
+    cache, table, n = _make(2, page, d, lens, cuda, g)
+    k, v = torch.randn(sum(lens), 2, d, generator=g).to(dtype).to(cuda), torch.zeros(sum(lens), 2, d, dtype=dtype, device=cuda)
+    K.paged_append(cache, k, v, n, table, starts=torch.tensor([sum(lens[:b]) for b in range(5)], dtype=torch.int32, device=cuda))
+    used = table[table >= 0].long()
+    assert bool((cache.v_scales[used] == 2.0 ** -126).all())
+    out = K.paged_attention(torch.randn(4 * each, 4, d, generator=g).to(dtype).to(cuda), cache, n, table, d ** -0.5)
+    assert not bool(out.any())
