@@ -505,7 +505,7 @@ RMLK_API int rmlk_b200_matmul_i8(rmlk_stream_t stream, int out_dtype, int64_t m,
                         const float* x_scales, const void* w, int64_t ldw, const float* w_scales, void* out, int64_t ldo, int* status);
 
 /* A cache of keys and values in pages of page_size tokens: k, v: int8 codes [pages, kv_heads, page_size, head_dim]; k_scales, v_scales:
- * [pages, kv_heads] fp32, one for the block of a page and head: a value is its code times the scale.  page_size 16, 32, 64 or 128;
+ * [pages, kv_heads] fp32, one for the block of a page and head: a value is its code times the scale, which may be below zero.  page_size 16, 32, 64 or 128;
  * head_dim 64 or 128; everything on 16-byte boundaries.
  * Sequence b of a batch holds lens[b] tokens (int32, device); token t lies in slot t % page_size of page table[b * table_width + t / page_size]
  * (int32, device; table_width * page_size up to 2^30).  Entries behind the last token's page are not read.  The new tokens of a call are the LAST
@@ -541,7 +541,7 @@ RMLK_API int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rmlk_
  * p = lens[b] - new[b] + i, sees positions 0 .. p;
  *   out[row, h] = softmax_t(scale q[row, h] . k[t, h / (q_heads / kv_heads)]) v[t, ..]      (scale: any finite number)
  * q, out: [tokens, q_heads, head_dim] f32 or f16, heads dense, rows q_stride / out_stride elements apart; q_heads a multiple of
- * kv_heads, up to 64 for each; rows on 16-byte boundaries.  A row that sees nothing is 0; one that sees a block whose scale is NaN is NaN; one that sees
+ * kv_heads, up to 64 for each; rows on 16-byte boundaries.  A row that sees nothing is 0; one that sees a block whose scale is not finite is NaN; one that sees
  * a token whose page is not in [0, pages) or lies behind table_width is NaN, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG
  * (RMLK_ERR_TIMEOUT: a bounded wait expired).
  * Few rows over many keys share the keys out over the whole GPU, where every sequence has as many (starts NULL); with starts at most eight SMs walk along

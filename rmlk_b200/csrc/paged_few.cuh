@@ -573,16 +573,19 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                     }
                 }
             }
-            // scales of V: the largest, and whether the others are of its size
-            float v_top = 0.f, v_low = INFINITY;
+            // scales of V: the largest magnitude, and whether the others are of its size and sign; what is not finite
+            float v_most = 0.f, v_least = 0.f, v_low = INFINITY;
             bool broken = false;
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                const float v = scales[stage * NC + n].y;
-                broken = broken || !(v < INFINITY);
-                v_top = fmaxf(v_top, v);
-                if (v > 0.f) v_low = fminf(v_low, v);
+                const float2 kv = scales[stage * NC + n];
+                const float size = fabsf(kv.y);
+                broken = broken || !(fabsf(kv.x) < INFINITY) || !(size < INFINITY);
+                v_most = fmaxf(v_most, kv.y);
+                v_least = fminf(v_least, kv.y);
+                if (size > 0.f) v_low = fminf(v_low, size);
             }
+            const float v_top = fmaxf(v_most, -v_least);
             if (KS + step * L::UNIT > all_see) {
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
@@ -598,8 +601,10 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
 #pragma unroll
                 for (int r = 0; r < NR; r++)
 #pragma unroll
-                    for (int n = 0; n < NC; n++)
-                        if (!(scales[stage * NC + n].y < INFINITY) && 16 * n < sees[r] - step * L::UNIT) sum[r] = __int_as_float(0x7fc00000);
+                    for (int n = 0; n < NC; n++) {
+                        const float2 kv = scales[stage * NC + n];
+                        if (!(fabsf(kv.x) < INFINITY && fabsf(kv.y) < INFINITY) && 16 * n < sees[r] - step * L::UNIT) sum[r] = __int_as_float(0x7fc00000);
+                    }
             }
             float weight[NR];  // of the step's sums: exp2(largest score of the step - running maximum)
             bool more = false;
@@ -635,21 +640,21 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                 sum[r] = fmaf(part, weight[r], sum[r]);
             }
             // ---- values ----
-            // Scales of V go into the weights, relative to the step's largest.  Where they differ by more than 2^3 a page at a time is taken, under its own.
-            const bool even = v_low * 8.f >= v_top;
+            // Scales of V go into the weights, relative to the step's largest.  Where they differ by more than 2^3, or in sign, a page at a time is taken, under its own.
+            const bool even = v_low * 8.f >= v_top && !(v_most > 0.f && v_least < 0.f);
             constexpr float MOST = L::F32 ? 8388607.f : 65535.f;
             const int passes = NC == 1 || even ? 1 : NC;
 #pragma unroll 1
             for (int pass = 0; pass < passes; pass++) {
-                const float ref = passes == 1 ? v_top : scales[stage * NC + pass].y;
-                if (!(ref > 0.f && ref < INFINITY)) continue;  // nothing but zeros (or NaN, seen to above)
-                // v / ref for 0 <= v <= ref: the reciprocal of a number near the lower end of fp32 would be infinite, of 2^64 times it is not
-                const float up = ref < 1.f ? 18446744073709551616.f : 1.f, per = 1.f / (ref * up);
+                const float ref = passes == 1 ? (v_most > 0.f ? v_top : -v_top) : scales[stage * NC + pass].y, size = fabsf(ref);
+                if (!(size > 0.f && size < INFINITY)) continue;  // nothing but zeros (or NaN, seen to above)
+                // v / size for 0 <= v <= size: the reciprocal of a number near the lower end of fp32 would be infinite, of 2^64 times it is not
+                const float up = size < 1.f ? 18446744073709551616.f : 1.f, per = 1.f / (size * up);
                 uint32_t p[NR][NC][L::DIGITS];
 #pragma unroll
                 for (int n = 0; n < NC; n++) {
                     // (a page whose scale is not finite: its weights are 0, or the row is NaN already)
-                    const float v = scales[stage * NC + n].y, k = passes > 1 ? (n == pass ? MOST : 0.f) : v == ref ? MOST : v < INFINITY ? v * up * per * MOST : 0.f;
+                    const float v = fabsf(scales[stage * NC + n].y), k = passes > 1 ? (n == pass ? MOST : 0.f) : v == size ? MOST : v < INFINITY ? v * up * per * MOST : 0.f;
 #pragma unroll
                     for (int r = 0; r < NR; r++) {
                         // the lower bits of 2^23 + a number below 2^23 are that number

@@ -59,3 +59,42 @@ def test_values_of_zero_are_zero(cuda, page, d, each, dtype):
     assert bool((cache.v_scales[used] == 2.0 ** -126).all())
     out = K.paged_attention(torch.randn(4 * each, 4, d, generator=g).to(dtype).to(cuda), cache, n, table, d ** -0.5)
     assert not bool(out.any())
+
+
+@pytest.mark.parametrize("d,each,group", [(64, 1, 4), (128, 1, 7), (64, 3, 5), (128, 2, 8), (64, 70, 4), (128, 60, 4)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_scales_below_zero(cuda, d, each, group, dtype):
+    """A value is its code times the scale, whatever the sign: all below zero, some of them, of one size and of many; for one token, for a few and for prompts."""
+    g = _gen(d, each, group)
+    cache, table, n = _make(2, 16, d, [each, each + 17, 200, 1500], cuda, g)
+    q = torch.randn(4 * each, 2 * group, d, generator=g).to(dtype).to(cuda)
+    for low, high, share in ((-4, -3, 1.0), (-5, -3, 0.5), (-12, 2, 0.5), (-5, -3, 0.02)):
+        for part in (cache.v_scales, cache.k_scales):
+            part.copy_(_scales(cache, low if part is cache.v_scales else -5, high if part is cache.v_scales else -3, g))
+            part.mul_(torch.where(torch.rand(part.shape, generator=g) < share, -1.0, 1.0).to(cuda))
+        out, want, bound = _attend(q, cache, n, table, d)
+        E.close(out, want, bound)
+
+
+@pytest.mark.parametrize("d,each,group", [(64, 1, 4), (128, 2, 8), (64, 4, 6), (128, 60, 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_scales_that_are_not_finite(cuda, d, each, group, dtype):
+    """Infinities of either sign and NaN make NaN of the rows and heads that see a token of their page, and of no others."""
+    from rmlk_b200 import kernels as K
+    g = _gen(d, each, group, 5)
+    lens = [200 + each, 100 + each, 48 + each]
+    cache, table, n = _make(2, 16, d, lens, cuda, g)
+    q = torch.randn(3 * each, 2 * group, d, generator=g).to(dtype).to(cuda)
+    pages = table[0, 2], table[1, 6], table[2, 3]  # seen by all rows of their sequence; by its last ones; by the last one alone or all but the first
+    for value in (math.inf, -math.inf, math.nan):
+        for of_k in (True, False):
+            told = [t.clone() for t in cache]
+            for i, page in enumerate(pages):
+                told[2 if of_k else 3][page, i % 2] = value
+            out = K.paged_attention(q, K.PagedCache(*told), n, table, d ** -0.5)
+            for i, page in enumerate(pages):
+                told[2 if of_k else 3][page, i % 2] = math.nan
+            want, bound = E.attention(q, K.PagedCache(*told), n, table, d ** -0.5)
+            assert torch.equal(torch.isnan(out), torch.isnan(want))
+            assert bool(torch.isnan(out).any()) and not bool(torch.isnan(out).all())
+            E.close(out, want, bound)
