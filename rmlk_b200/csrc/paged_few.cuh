@@ -13,10 +13,13 @@
 // A warp's step: 4 KB of keys and of values, copied by its own lanes with cp.async: no warp waits for another.
 // Both contractions are products of 8-bit integers (mma.sync m16n8k32, exact 32-bit sums), so the codes are operands as they lie there.  (As f16, four
 // instructions went into each pair of codes: 530 per step of 4 KB, and the SMs, not HBM, were the bound: 5.0 TB/s.)
-//   scores  S[16 rows x 8 keys] = Q K^T.  Queries are fixed-point numbers under a power of two per row: 15 bits and sign for f16, 22 for fp32 - half a
-//           step is 2^-15 or 2^-23 of the row's largest value - as two or three signed digits of 8 bits, a row of the MMA each.  Where a row's values, none counted
-//           for more than 1/16 of its largest, are on average less than 1/43 of it (a few outliers: normally distributed values are so beside one of 34 standard deviations), digits
-//           would lose too much of them: the tile's scores are formed in fp32 from the queries themselves.
+//   scores  S[16 rows x 8 keys] = Q K^T.  Queries are fixed-point numbers of 22 bits and sign under a power of two per row - half a step is 2^-23 of the row's largest value -
+//           as three signed digits of 8 bits, a row of the MMA each.  Where digits would lose too much, scores are formed in fp32 from the queries themselves.
+//           f16: values above 2^-11 of the largest are held as they are.  What the others lose is summed up for each row; where it could move a score's exponent by more than
+//           2^-13 in some key of the step, all codes of which were +-128, the step goes to fp32.  (With two digits, 15 bits, keys that have no part in a query's few outliers
+//           of 16 to 33 times the rest came out up to 1.2 % off.)
+//           fp32: every value loses something, next to nothing beside its score as a rule.  Where a row's values, none counted for more than 1/16 of its largest, are on average
+//           less than 1/43 of it (a few outliers: normally distributed values are so beside one of 34 standard deviations), all of the tile's steps go to fp32.
 //   values  O^T[16 dims x 8 rows] = V^T P^T.  Weights exp2(s - m), m the row's largest score in the step, are fixed-point numbers of 16 bits (f16 results) or 23
 //           (fp32): half a step is 2^-17 or 2^-24 of the largest weight of the step.  Unsigned digits, an MMA each; the accumulator fragment of S holds just the
 //           weights that the operand fragment wants, four tokens' bytes to a register, and a 4 x 4 transpose of bytes puts four tokens' codes side by side.
@@ -54,12 +57,12 @@ struct Few {
     static constexpr int UNIT = 4 * KS;
     static constexpr int STAGES = 2;
     static constexpr int K_BYTES = KS * D, STEP = 2 * K_BYTES;
-    static constexpr int QT = F32 ? NR + 1 : NR;  // row tiles of the scores' MMAs: (high, low digit) of each group, and the third digits of both
-    static constexpr int DIGITS = F32 ? 3 : 2;
+    static constexpr int QT = NR + 1;             // row tiles of the scores' MMAs: (first, second digit) of each group, and the third digits of both
+    static constexpr int DIGITS = F32 ? 3 : 2;    // of the weights
     static constexpr int RING = 4 * STAGES * STEP;
     static constexpr int FRAGS = D / 16 * NR;    // groups of four sums per lane
     static constexpr int HAND = 32 * (FRAGS * 16 + NR * 8);  // a warp's share on its way to another: sums, maxima, weights' sums
-    static constexpr int SCALES = RING + 2 * HAND, SCAN = SCALES + 4 * STAGES * NC * 8, SMEM = SCAN + 64;
+    static constexpr int SCALES = RING + 2 * HAND, SCAN = SCALES + 4 * STAGES * NC * 8, SEGMENTS = SCAN + 64, SMEM = SEGMENTS + 4 * 2 * 64;
     static constexpr int PER_SM = NR == 2 ? 2 : 3;
 };
 constexpr int MOST_PARTS = 32;  // CTAs for a problem, on average: each costs the last one a fraction of a microsecond
@@ -344,44 +347,73 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
     };
 
     // ---- the stream of loads ----
-    Segment ask;
-    ask.b = share_b;
-    ask.seq = share_seq;
-    ask.unit = lo;
-    look(ask);
-    Segment now = ask;
+    // The segments that are asked for and worked on wait in shared memory: in registers they would push out what the steps need.  (Every lane writes the same and reads what it wrote.)
+    struct Place {
+        Segment s;
+        __device__ __forceinline__ void put(const Segment& x) volatile {
+            s.b = x.b, s.h = x.h, s.tile = x.tile, s.steps = x.steps, s.left = x.left;
+            s.seq = x.seq, s.unit = x.unit, s.units = x.units, s.taken = x.taken, s.first_key = x.first_key;
+        }
+        __device__ __forceinline__ Segment get() volatile {
+            Segment x;
+            x.b = s.b, x.h = s.h, x.tile = s.tile, x.steps = s.steps, x.left = s.left;
+            x.seq = s.seq, x.unit = s.unit, x.units = s.units, x.taken = s.taken, x.first_key = s.first_key;
+            return x;
+        }
+    };
+    static_assert(sizeof(Place) <= 64, "");
+    volatile Place* const asked = reinterpret_cast<volatile Place*>(smem + L::SEGMENTS + 128 * warp);
+    volatile Place* const at_work = reinterpret_cast<volatile Place*>(smem + L::SEGMENTS + 128 * warp + 64);
+    int ask_steps;
+    {
+        Segment first;
+        first.b = share_b;
+        first.seq = share_seq;
+        first.unit = lo;
+        look(first);
+        asked->put(first);
+        at_work->put(first);
+        ask_steps = first.steps;
+    }
     int block = -1;  // page and head as one index; -1: no key there, -2: a key without a page
     constexpr int PAGED_STEPS = 32 / NC;  // pages of so many steps are looked up at a time, one per lane
     const int block_bytes = c.page * D;
     int fill = 0, fill_stage = 0;  // next step to be asked for, its place in the ring
     auto issue = [&]() {
-        while (fill == ask.steps && ask.unit < hi) {
-            move_on(ask);
-            fill = 0;
-            if (ask.unit >= hi) ask.steps = 0;
+        if (fill == ask_steps) {
+            Segment ask = asked->get();
+            while (fill == ask.steps && ask.unit < hi) {
+                move_on(ask);
+                fill = 0;
+                if (ask.unit >= hi) ask.steps = 0;
+            }
+            asked->put(ask);
+            ask_steps = ask.steps;
         }
-        if (fill < ask.steps) {
+        if (fill < ask_steps) {
+            const int h = asked->s.h;
+            const int64_t first_key = asked->s.first_key;
             const int in_batch = fill % PAGED_STEPS;
             if (in_batch == 0) {
                 const int off = (fill + lane / NC) * L::UNIT + (lane % NC) * 16;
                 block = -1;
-                if (off < ask.left) {
-                    const int64_t at = (ask.first_key + off) >> c.page_log;
-                    const int p = at < q.width ? q.table[static_cast<int64_t>(ask.b) * q.width + at] : -1;
-                    block = p >= 0 && p < c.pages ? p * c.kv_heads + ask.h : -2;
+                if (off < asked->s.left) {
+                    const int64_t at = (first_key + off) >> c.page_log;
+                    const int p = at < q.width ? q.table[static_cast<int64_t>(asked->s.b) * q.width + at] : -1;
+                    block = p >= 0 && p < c.pages ? p * c.kv_heads + h : -2;
                     if (block == -2 && a.status) *a.status = RMLK_ERR_INVALID_ARG;
                 }
             }
             const uint32_t dst = ring + fill_stage * L::STEP;
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                const int at = __shfl_sync(0xffffffffu, block, in_batch * NC + n), from = at < 0 ? ask.h : at;  // (page 0 is read where there is none)
+                const int at = __shfl_sync(0xffffffffu, block, in_batch * NC + n), from = at < 0 ? h : at;  // (page 0 is read where there is none)
                 if (lane < 2) {  // the scales of K and V: 0 where there is no key, NaN where a key has no page
                     float* to = reinterpret_cast<float*>(scales + fill_stage * NC + n) + lane;
                     if (at >= 0) copy_async<4>(static_cast<uint32_t>(__cvta_generic_to_shared(to)), (lane ? c.vs : c.ks) + at);
                     else *to = at == -1 ? 0.f : __int_as_float(0x7fc00000);
                 }
-                const int64_t off = static_cast<int64_t>(from) * block_bytes + ((static_cast<int>(ask.first_key & 127) + fill * L::UNIT + 16 * n) & (c.page - 1)) * D;
+                const int64_t off = static_cast<int64_t>(from) * block_bytes + ((static_cast<int>(first_key & 127) + fill * L::UNIT + 16 * n) & (c.page - 1)) * D;
 #pragma unroll
                 for (int j = 0; j < D / 32; j++) {
                     const uint32_t to = dst + n * (16 * D) + unit_at<D>((512 / D) * j + lane / (D / 16), lane % (D / 16));
@@ -431,9 +463,9 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
     int stage = 0;
     bool first = true, handed = false;  // first segment of the CTA; the hand-over places have been used
 
-    while (now.unit < hi) {
-        const int b = now.b, h = now.h, tile = now.tile;
-        const int64_t keys = keys_of(b), first_key = now.first_key;
+    while (true) {
+        const int b = at_work->s.b, h = at_work->s.h, tile = at_work->s.tile, steps = at_work->s.steps;
+        const int64_t keys = keys_of(b), first_key = at_work->s.first_key;
         const int64_t before = static_cast<int64_t>(q.lens[b]) - q.each;  // keys before the first new token
 
         // ---- queries: fragments of the scores' MMAs, and what each lane's rows see.  (Asked for first, looked at when the first keys are on their way.) ----
@@ -459,10 +491,11 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
 #pragma unroll
             for (int s = 0; s < L::STAGES - 1; s++) issue();
         }
-        bool wide = false;  // a row of the tile has values that its digits would lose: scores are formed in fp32 instead
+        // what digits of the tile's queries may lose in an exponent, for keys under the scale 1: three digits, the first two of them (f16)
+        float lost = 0.f, lost_by_two = 0.f;
         // digits: [32 dims][row tile]: rows g and g + 8 of the lane's first four dims, then of the next four
         uint32_t qf[2 * PIECES][L::QT][4];
-        if constexpr (L::F32 && NR == 1) {
+        if constexpr (NR == 1) {
 #pragma unroll
             for (int s = 0; s < 2 * PIECES; s++) qf[s][NR][1] = qf[s][NR][3] = 0;  // no second group
         }
@@ -484,45 +517,49 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             }
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            // 2^e: the largest in [2^14, 2^15) - times 2^8 for three digits - but not above what signed digits hold, 127 127 (127)
+            // 2^e: the largest in [2^14, 2^15), times 2^8 for the third digit, but not above what signed digits hold, 127 127 127
             int e = scale_exponent(most < 0x7f800000u ? most : 0u);
-            if (__uint_as_float(most) * exp2_int(e) > (L::F32 ? 32639.49f : 32639.f)) e--;
-            const float up = exp2_int(e), more = L::F32 ? 256.f : 1.f;
+            if (__uint_as_float(most) * exp2_int(e) > 32639.49f) e--;
+            const float up = exp2_int(e), more = 256.f;
             // an infinity or a NaN makes NaN of the row
             factor[r] = most < 0x7f800000u ? a.scale * 1.44269504f / more * exp2_int(-e) : __int_as_float(0x7fc00000);
-            // (no condition around the sum: lanes of other rows take part in it)
-            const float limit = most < 0x7f800000u ? __uint_as_float(most) * (1.f / 16.f) : 0.f;
-            float capped = 0.f;
+            if constexpr (L::F32) {
+                // (no condition around the sum: lanes of other rows take part in it)
+                const float limit = most < 0x7f800000u ? __uint_as_float(most) * (1.f / 16.f) : 0.f;
+                float capped = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4 * PIECES; s++) {
-                const float4 x = four(s);
-                capped += (fminf(fabsf(x.x), limit) + fminf(fabsf(x.y), limit)) + (fminf(fabsf(x.z), limit) + fminf(fabsf(x.w), limit));
+                for (int s = 0; s < 4 * PIECES; s++) {
+                    const float4 x = four(s);
+                    capped += (fminf(fabsf(x.x), limit) + fminf(fabsf(x.y), limit)) + (fminf(fabsf(x.z), limit) + fminf(fabsf(x.w), limit));
+                }
+                const float of_row = quad_sum(capped);
+                if (of_row < 0.375f * D * limit) lost = INFINITY;
             }
-            const float of_row = quad_sum(capped);
-            wide = wide | (of_row < 0.375f * D * limit);
+            float rest = 0.f;  // (f16) of the lane's values, in steps; squares of the third digits
+            int thirds = 0;
 #pragma unroll
             for (int s = 0; s < 4 * PIECES; s++) {
                 const float4 x = four(s);
                 const int v[4] = {__float2int_rn(x.x * up * more), __float2int_rn(x.y * up * more), __float2int_rn(x.z * up * more), __float2int_rn(x.w * up * more)};
+                if constexpr (!L::F32)
+                    rest += (fabsf(x.x * up * more - static_cast<float>(v[0])) + fabsf(x.y * up * more - static_cast<float>(v[1]))) +
+                            (fabsf(x.z * up * more - static_cast<float>(v[2])) + fabsf(x.w * up * more - static_cast<float>(v[3])));
                 // signed digits: the byte of v + 0x80 (+ 0x8000) carries what the digits below borrow
                 const uint32_t d0 = bytes_of<0>(v[0], v[1], v[2], v[3]), d1 = bytes_of<1>(v[0] + 0x80, v[1] + 0x80, v[2] + 0x80, v[3] + 0x80);
                 uint32_t(&f)[L::QT][4] = qf[s >> 1];
                 const int at = 2 * (s & 1);
-                if constexpr (L::F32) {
-                    f[r][at] = bytes_of<2>(v[0] + 0x8080, v[1] + 0x8080, v[2] + 0x8080, v[3] + 0x8080);
-                    f[r][at + 1] = d1;
-                    f[NR][at + r] = d0;
-                } else {
-                    f[r][at] = d1;
-                    f[r][at + 1] = d0;
-                }
+                f[r][at] = bytes_of<2>(v[0] + 0x8080, v[1] + 0x8080, v[2] + 0x8080, v[3] + 0x8080);
+                f[r][at + 1] = d1;
+                f[NR][at + r] = d0;
+                if constexpr (!L::F32) thirds = __dp4a(static_cast<int>(d0), static_cast<int>(d0), thirds);
+            }
+            if constexpr (!L::F32) {  // (a row that is NaN has no part in either)
+                lost = fmaxf(lost, quad_sum(rest) * fabsf(factor[r]) * 128.f);
+                lost_by_two = fmaxf(lost_by_two, sqrtf(quad_sum(static_cast<float>(thirds))) * fabsf(factor[r]) * 128.f);
             }
         }
-        wide = __any_sync(0xffffffffu, wide);
-        if (wide) {
-#pragma unroll
-            for (int r = 0; r < NR; r++) factor[r] = factor[r] == factor[r] ? a.scale * 1.44269504f : factor[r];
-        }
+        lost = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lost)));
+        if constexpr (!L::F32) lost_by_two = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lost_by_two)));
         const int all_see = relative(min(before + 1 + (tile * ROWS) / a.group, keys));  // that every row of the tile sees
 
         Share<D, NR> own;
@@ -530,12 +567,26 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
         float(&acc)[D / 16][NR][4] = own.acc;
         float(&top)[NR] = own.top;
         float(&sum)[NR] = own.sum;
-        for (int step = 0; step < now.steps; step++, stage = stage + 1 == L::STAGES ? 0 : stage + 1) {
+        for (int step = 0; step < steps; step++, stage = stage + 1 == L::STAGES ? 0 : stage + 1) {
             __syncwarp();  // the slot that is filled next has been read, its scales too
             issue();
             asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 1) : "memory");
             __syncwarp();  // (of all lanes)
             const uint8_t* at = ring_ptr + stage * L::STEP;
+            // scales of V: the largest magnitude, and whether the others are of its size and sign; what is not finite; the largest scale of K
+            float k_top = 0.f, v_most = 0.f, v_least = 0.f, v_low = INFINITY;
+            bool broken = false;
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const float2 kv = scales[stage * NC + n];
+                const float size = fabsf(kv.y);
+                broken = broken || !(fabsf(kv.x) < INFINITY) || !(size < INFINITY);
+                k_top = fmaxf(k_top, fabsf(kv.x));
+                v_most = fmaxf(v_most, kv.y);
+                v_least = fminf(v_least, kv.y);
+                if (size > 0.f) v_low = fminf(v_low, size);
+            }
+            const float v_top = fmaxf(v_most, -v_least);
             // ---- scores ----
             float x[NR][KS / 8][2];
 #pragma unroll
@@ -545,7 +596,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
                 for (int i = 0; i < PIECES; i++) {
                     const uint4 w = *reinterpret_cast<const uint4*>(at + j / 2 * (16 * D) + unit_at<D>(8 * (j & 1) + g, 4 * i + c4));
 #pragma unroll
-                    for (int t = 0; t < L::QT; t++) {
+                    for (int t = 0; t < (L::F32 ? L::QT : NR); t++) {
                         mma_s8(s[t], qf[2 * i][t][0], qf[2 * i][t][1], qf[2 * i][t][2], qf[2 * i][t][3], w.x, w.y);
                         mma_s8(s[t], qf[2 * i + 1][t][0], qf[2 * i + 1][t][1], qf[2 * i + 1][t][2], qf[2 * i + 1][t][3], w.z, w.w);
                     }
@@ -557,35 +608,43 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const float high = static_cast<float>(s[r][e] * 256 + s[r][2 + e]);
-                        x[r][j][e] = (L::F32 ? fmaf(high, 256.f, static_cast<float>(s[L::QT - 1][2 * r + e])) : high) * t;
+                        x[r][j][e] = (L::F32 ? fmaf(high, 256.f, static_cast<float>(s[NR][2 * r + e])) : high * 256.f) * t;
                     }
                 }
             }
+            if (!L::F32 && lost_by_two * k_top > 2.44140625e-4f) {  // 2^-12: the third digits too
+#pragma unroll
+                for (int j = 0; j < KS / 8; j++) {
+                    int s[4] = {};
+#pragma unroll
+                    for (int i = 0; i < PIECES; i++) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(at + j / 2 * (16 * D) + unit_at<D>(8 * (j & 1) + g, 4 * i + c4));
+                        mma_s8(s, qf[2 * i][NR][0], qf[2 * i][NR][1], qf[2 * i][NR][2], qf[2 * i][NR][3], w.x, w.y);
+                        mma_s8(s, qf[2 * i + 1][NR][0], qf[2 * i + 1][NR][1], qf[2 * i + 1][NR][2], qf[2 * i + 1][NR][3], w.z, w.w);
+                    }
+                    const float ks = scales[stage * NC + j / 2].x;
+#pragma unroll
+                    for (int r = 0; r < NR; r++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) x[r][j][e] = fmaf(static_cast<float>(s[2 * r + e]), factor[r] * ks, x[r][j][e]);
+                }
+            }
+            const bool wide = lost * k_top > 1.220703125e-4f;  // 2^-13; (a tile that is all wide: infinite)
             if (wide) {
+                float direct[NR];
+#pragma unroll
+                for (int r = 0; r < NR; r++) direct[r] = factor[r] == factor[r] ? a.scale * 1.44269504f : factor[r];
                 const Scores<D, NR> y = scores_in_fp32<T, D, NR>(static_cast<const T*>(a.q), a.qs, a.group, static_cast<int64_t>(b) * q.each, h, tile * ROWS, rows, at);
 #pragma unroll
                 for (int j = 0; j < KS / 8; j++) {
                     const float ks = scales[stage * NC + j / 2].x;
 #pragma unroll
                     for (int r = 0; r < NR; r++) {
-                        x[r][j][0] = y.x[r][j][0] * (factor[r] * ks);
-                        x[r][j][1] = y.x[r][j][1] * (factor[r] * ks);
+                        x[r][j][0] = y.x[r][j][0] * (direct[r] * ks);
+                        x[r][j][1] = y.x[r][j][1] * (direct[r] * ks);
                     }
                 }
             }
-            // scales of V: the largest magnitude, and whether the others are of its size and sign; what is not finite
-            float v_most = 0.f, v_least = 0.f, v_low = INFINITY;
-            bool broken = false;
-#pragma unroll
-            for (int n = 0; n < NC; n++) {
-                const float2 kv = scales[stage * NC + n];
-                const float size = fabsf(kv.y);
-                broken = broken || !(fabsf(kv.x) < INFINITY) || !(size < INFINITY);
-                v_most = fmaxf(v_most, kv.y);
-                v_least = fminf(v_least, kv.y);
-                if (size > 0.f) v_low = fminf(v_low, size);
-            }
-            const float v_top = fmaxf(v_most, -v_least);
             if (KS + step * L::UNIT > all_see) {
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
@@ -722,6 +781,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             }
         }
 
+        Segment now = at_work->get();
         // ---- the four warps' shares: 2 to 0, 3 to 1, 1 to 0 ----
 #pragma unroll
         for (int r = 0; r < NR; r++) sum[r] = quad_sum(sum[r]);
@@ -746,7 +806,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             own.join_shared(s_hand + SLOT, lane, c4);
             pair_arrive<FREE_1>();
             if (now.taken == now.units) {
-                store(own, b, h, tile);
+                store(own, now.b, now.h, now.tile);
             } else {
                 own.put(partials + (static_cast<int64_t>(blockIdx.x) * 2 + (first ? 0 : 1)) * SLOT, lane);
                 __threadfence();
@@ -763,6 +823,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
         first = false;
         if (now.unit + now.taken == hi) break;
         move_on(now);
+        at_work->put(now);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (warp == 2) pair_wait<FREE_0>();  // (no arrival is left open)
@@ -813,7 +874,7 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             finish(head);
         }
         __syncthreads();
-        if (s_at[1]) finish(now);
+        if (s_at[1]) finish(at_work->get());
     }
 }
 
