@@ -65,3 +65,19 @@ def test_f16_queries_and_keys_of_any_scale(cuda, d):
             out = K.paged_attention(q, cache, n, table, d ** -0.5)
             want, bound = E.attention(q, cache, n, table, d ** -0.5)
             E.close(out, want, 4 * bound)  # (scores in fp32: D roundings of 2^-24, where the bound counts D / 16 + 8 of 2^-23)
+
+
+@pytest.mark.parametrize("d,each,group", [(64, 1, 4), (128, 2, 3), (128, 1, 16), (64, 5, 5)])
+def test_fp32_queries_of_two_sizes(cuda, d, each, group):
+    """As above: the digits of a row lie under its largest value, and keys need not have a part in that."""
+    from rmlk_b200 import kernels as K
+    g = _gen(d, each, group)
+    cache, table, n, x = _case(d, each, group, torch.float32, cuda, g)
+    cache.k[..., ::2] = 0
+    for large, small, scale in ((20.0, 1.0, 1.0), (300.0, 1.0, 1.0), (1e6, 1.0, 1.0), (1e9, 1e-6, 1e6)):
+        q = x * small
+        q[..., ::2] = x[..., ::2] * large
+        q = q.to(cuda)
+        out = K.paged_attention(q, cache, n, table, scale * d ** -0.5)
+        want, bound = E.attention(q, cache, n, table, scale * d ** -0.5)
+        E.close(out, want, 4 * bound)  # (scores in fp32: D roundings of 2^-24, where the bound counts D / 16 + 8 of 2^-23)
