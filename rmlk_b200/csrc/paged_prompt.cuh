@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 const float k = c.ks[block], v = c.vs[block];
                 plain = plain && k >= 0.f && k < INFINITY && v >= 0.f && v < INFINITY;
                 v_top = fmaxf(v_top, v);
-                if (v > 7.52316385e-37f) v_low = fminf(v_low, v);  // 2^-120: a block of zeros has the scale 2^-126
+                if (v > 1.17549435e-38f) v_low = fminf(v_low, v);  // 2^-126: the scale of a block of zeros
             }
         }
         const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(v_top)), l = __reduce_min_sync(0xffffffffu, __float_as_uint(v_low));
@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), at = lanes + t * 128, o_at = lanes + L::O_AT + t * L::O_PITCH;
         const int sees = r < rows ? sees_of(row0 + r) : 0, least = sees_of(row0 + t * 128);  // least: what every row of the tile sees
         const float q_scale = fabsf(a.scale) * 1.44269504f * (L::F32 ? s_row[r] : 1.f);
-        const float v_inv = 1.f / v_top;
+        // v / v_top: the reciprocal of a number near the lower end of fp32 would be infinite, of 2^64 times it is not
+        const float v_up = v_top < 1.f ? 18446744073709551616.f : 1.f, v_inv = 1.f / (v_top * v_up);
         float top = -INFINITY, sum = 0.f;
         bool ok = true, fresh = true;  // fresh: nothing kept yet (fp32)
         int in_run = 0;                // (fp32) blocks since the sums were last added up
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         page_of(1);
         for (int j = 0; j < own_blocks; j++) {
             // lane n has the scales of 16 keys; f_of: what a row's scores are multiplied by (not zero: hidden scores stay -inf)
-            const float ks = ks_next, vs = vs_next * v_inv;
+            const float ks = ks_next, vs = vs_next * v_up * v_inv;
             auto f_of = [&](int n) { return fmaxf(__shfl_sync(0xffffffffu, ks, n) * q_scale, 1e-38f); };
             const bool even = __all_sync(0xffffffffu, vs == 1.f);  // all scales of V are the largest
             scales_of();
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         tc_fence_after();
         // (the sums of a share go to where the operands of both tiles were)
         if constexpr (SHARED) asm volatile("bar.sync 3, %0;" ::"n"(ROWS) : "memory");
-        const float inv = SHARED ? v_top : 1.f / sum * v_top;
+        const float inv = 1.f / sum;  // (not times v_top: that could leave the normal numbers although the result does not)
         const int row = row0 + r, token = token_of(row);
         T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D;
 #pragma unroll 1
@@ -559,12 +560,12 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             if constexpr (SHARED) {
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
-                    const float4 x = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                    const float4 x = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
                     *reinterpret_cast<float4*>(sm + r * (D * 4) + ((((i + e) >> 2) ^ (r & 7)) << 4)) = own_blocks > 0 ? x : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             } else if (r < rows) {
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(!ok ? __int_as_float(0x7fc00000) : sees <= 0 ? 0.f : __uint_as_float(o[e]) * inv);
+                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(!ok ? __int_as_float(0x7fc00000) : sees <= 0 ? 0.f : __uint_as_float(o[e]) * inv * v_top);
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     if constexpr (L::F32) {
@@ -734,7 +735,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 }
             const int row = row0 + r, token = token_of(row);
             const float inv = 1.f / sum;
-            o = sees_of(row) <= 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            o = sees_of(row) <= 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv * v_top, o.y * inv * v_top, o.z * inv * v_top, o.w * inv * v_top);
             T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D + 4 * u;
             if constexpr (L::F32) *reinterpret_cast<float4*>(dst) = o;
             else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(o.x, o.y), pack_f16(o.z, o.w));

@@ -98,3 +98,33 @@ def test_scales_that_are_not_finite(cuda, d, each, group, dtype):
             assert torch.equal(torch.isnan(out), torch.isnan(want))
             assert bool(torch.isnan(out).any()) and not bool(torch.isnan(out).all())
             E.close(out, want, bound)
+
+
+@pytest.mark.parametrize("new,total", [([40, 33], [1000, 700]), ([130] * 40, [130 + 9 * i for i in range(40)])])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompts_over_values_of_any_size(cuda, new, total, d):
+    """Scales of V at both ends of fp32, alike and not, alone and with the keys shared by a cluster.  Nothing but the result itself has to fit: the sum of the weights times the values
+    is a thousand times larger, the largest scale over the weights' sum as much smaller."""
+    g = _gen(d, len(new))
+    cache, table, n = _make(2, 32, d, total, cuda, g)
+    starts = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device=cuda)
+    q = torch.randn(sum(new), 8, d, generator=g).to(cuda)
+    for low, high in ((-126, -125), (-126, -119), (-115, -109), (100, 101), (106, 110)):
+        cache.v_scales.copy_(_scales(cache, low, high, g))
+        out, want, bound = _attend(q, cache, n, table, d, starts)
+        E.close(out, want, bound)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_that_see_only_tiny_values(cuda, d):
+    """The first rows of a prompt see a page of tiny values, the others one of ordinary values as well: the first keep theirs."""
+    g = _gen(d, 3)
+    cache, table, n = _make(1, 16, d, [40], cuda, g)
+    q = torch.randn(40, 4, d, generator=g).to(cuda)
+    for tiny in (2.0 ** -123, 2.0 ** -125):
+        cache.v_scales.fill_(0.125)
+        cache.v_scales[table[0, 0]] = tiny
+        out, _, _ = _attend(q, cache, n, table, d, torch.tensor([0, 40], dtype=torch.int32, device=cuda))
+        for i in (0, 5, 15, 16, 39):
+            want, bound = E.attention(q[i: i + 1], cache, torch.tensor([i + 1]), table, d ** -0.5)
+            E.close(out[i: i + 1], want, bound)
