@@ -16,7 +16,10 @@
 // 16 prompts of up to 512 tokens, fp32, 32 heads of 64: 90 us.  A CTA has 4 blocks on average, so starting (queries turned into f16 pairs) and storing are half of it; with the pages
 // looked at before the queries, not beside them, 95 us.
 // The output sums stay in TMEM.  They are brought under a new maximum only when a row's has grown by more than 2^8 (weights are up to 2^14 then), which after the first
-// blocks hardly happens.  For fp32 results they are added to fp32 sums every four blocks: the accumulator truncates, and 256 keys are what its error allows.
+// blocks hardly happens.  The accumulator truncates, up to 2^-23 of a sum with every 16 keys (values of one sign over 200000 keys came out 1.4e-3 too small), so they are added to
+// fp32 sums every 256 keys for fp32 results, every 4096 for f16.  Those are in TMEM too, where two f16 tiles of 128 values leave no room: up to 16384 keys of a CTA they do without,
+// 1.0e-4 of a sum; over more, scores have one place instead of two, and the sums of one half of the values go to the other, those of the other half to shared memory.  4 prompts of 1024
+// tokens, 32 heads of 128: over 16000 keys 1.39 ms, over 20000 2.16, where sums that are cut off took 1.71.
 // Scales of K go into the scores' factor, scales of V into the weights, relative to the largest that the rows see.  Where scales of V span more than 2^10, or
 // something is not finite or has no page, the rows are taken one by one in fp32 (row_in_fp32): slow, and right for everything.
 #pragma once
@@ -62,14 +65,16 @@ struct Prompt {
     static constexpr int MAKERS = 128, THREADS = ROWS + MAKERS + 64;
     static constexpr int NBUF = 3;                         // blocks of keys, and of values, in shared memory
     static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = Q_HALF * HALVES, KV_HALF = KT * 128, KV_TILE = KV_HALF * HALVES;
-    static constexpr uint32_t Q = 0, K = TILES * PARTS * Q_TILE, V = K + NBUF * KV_TILE, ROW_SCALE = V + NBUF * KV_TILE, RED = ROW_SCALE + ROWS * 8, BARS = RED + 128,
-                              TOTAL = BARS + 256 + 1024;
+    static constexpr bool FULL = !F32 && D == 128;         // no room in TMEM for fp32 sums beside those of the MMAs
+    static constexpr uint32_t Q = 0, K = TILES * PARTS * Q_TILE, V = K + NBUF * KV_TILE, BEHIND = V + NBUF * KV_TILE, HALF_KEPT = BEHIND,
+                              ROW_SCALE = FULL ? ROWS * D * 4 : BEHIND, RED = BEHIND + (FULL ? ROWS * 64 * 4 : ROWS * 8), BARS = RED + 128, TOTAL = BARS + 256 + 1024;
     // TMEM columns: for each tile two places for scores (64 columns) and the weights made of them (two keys to a column; fp32: the second numbers behind the first), sums and (fp32)
     // kept sums
     static constexpr uint32_t O_AT = 256, O_PITCH = 128, KEPT = D;
-    static constexpr int FLUSH = 4;  // (fp32) blocks per accumulation
+    static constexpr int FLUSH = F32 ? 4 : 64, MOST = 256;  // blocks per accumulation; (FULL) of a CTA that does without
     static_assert(TOTAL <= 227 * 1024, "shared memory budget exceeded");
-    static_assert(ROWS * D * 4 <= ROW_SCALE, "a CTA's sums take the place of its operands");
+    static_assert(ROWS * D * 4 <= ROW_SCALE && ROW_SCALE + ROWS * 8 <= RED, "a CTA's sums take the place of its operands");
+    static_assert(!FULL || ROW_SCALE + ROWS * 8 <= BEHIND, "");
 };
 
 // One query row by one warp, a key after the other, in fp32: any scales, NaN for what is not finite and for a key without a page.
@@ -166,6 +171,58 @@ __device__ __forceinline__ uint4 eight_f16(uint32_t w0, uint32_t w1) {
     return make_uint4(two(w0, 0x4140), two(w0, 0x4342), two(w1, 0x4140), two(w1, 0x4342));
 }
 
+// The sums of a row that lie beside those of the MMAs: in TMEM, of FULL tiles the upper half of them in shared memory
+template <typename T, int D>
+struct KeptSums {
+    using L = Prompt<T, D>;
+    uint32_t o_at, at;
+    uint8_t* half;
+    int r;
+
+    __device__ __forceinline__ float4* unit(int i) const { return reinterpret_cast<float4*>(half + ((((i - 64) >> 2) ^ (r & 7)) << 4)); }
+    __device__ __forceinline__ void get(int i, uint32_t (&m)[32]) const {
+        if (L::FULL && i >= 64) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                const float4 x = *unit(i + e);
+                m[e] = __float_as_uint(x.x);
+                m[e + 1] = __float_as_uint(x.y);
+                m[e + 2] = __float_as_uint(x.z);
+                m[e + 3] = __float_as_uint(x.w);
+            }
+        } else {
+            tmem_ld_x32(at + i, m);
+        }
+    }
+    __device__ __forceinline__ void put(int i, const uint32_t (&m)[32]) const {
+        if (L::FULL && i >= 64) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) *unit(i + e) = make_float4(__uint_as_float(m[e]), __uint_as_float(m[e + 1]), __uint_as_float(m[e + 2]), __uint_as_float(m[e + 3]));
+        } else {
+            tmem_st_x32(at + i, m);
+        }
+    }
+    // the MMAs' sums go to these, all times `corr`
+    __device__ __forceinline__ void add(float corr, bool fresh) const {
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+            uint32_t o[32], m[32];
+            tmem_ld_x32(o_at + i, o);
+            get(i, m);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+                m[e] = __float_as_uint((__uint_as_float(o[e]) + (fresh ? 0.f : __uint_as_float(m[e]))) * corr);
+                o[e] = 0;
+            }
+            put(i, m);
+            tmem_st_x32(o_at + i, o);
+        }
+    }
+};
+template <typename K>
+__device__ __noinline__ void add_seldom(K kept, float corr, bool fresh) { kept.add(corr, fresh); }
+
 // SHARED: a cluster of `cluster` CTAs shares the keys of each tile pair
 template <typename T, int D, bool SHARED>
 __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const Cache c, const Batch q, const Attend a, const int cluster) {
@@ -256,6 +313,10 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     const int all_blocks = (seen + KT - 1) / KT, each_blocks = (all_blocks + splits - 1) / splits, block0 = min(share * each_blocks, all_blocks), key0 = block0 * KT;
     const int blocks = min(each_blocks, all_blocks - block0);
     const int blocks0 = rows > 128 ? min(max((sees_of(row0 + 127) + KT - 1) / KT - block0, 0), blocks) : blocks, blocks1 = rows > 128 ? blocks : 0;
+    const bool lean = L::FULL && blocks > L::MOST;  // one place for scores
+    // block j's scores: which place, how many came there before
+    auto place_of = [&](int j) { return lean ? 0 : j & 1; };
+    auto turn_of = [&](int j) { return lean ? j : j >> 1; };
     const bool negative = a.scale < 0.f;  // scores' factors are not below zero: the sign goes to the queries
     int* status = a.status;
     constexpr int OTHERS = L::MAKERS + 64, FIRST = ROWS / 32;  // threads and first warp that are not the softmax's
@@ -382,8 +443,9 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
     }
     const uint32_t tmem = maker ? 0u : *tmem_slot;
 
-    if (warp < FIRST) {
-        // ---------------- softmax ----------------
+    // (once for each number of places for scores: a choice within the loop took 4 % where most prompts have two)
+    auto softmax = [&](auto one_place) {
+        constexpr bool ONE = decltype(one_place)::value;
         const int t = warp >> 2, r = tid, own_blocks = t == 0 ? blocks0 : blocks1;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), at = lanes + t * 128, o_at = lanes + L::O_AT + t * L::O_PITCH;
         const int sees = r < rows ? sees_of(row0 + r) : 0, least = sees_of(row0 + t * 128);  // least: what every row of the tile sees
@@ -391,8 +453,11 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         // v / v_top: the reciprocal of a number near the lower end of fp32 would be infinite, of 2^64 times it is not
         const float v_up = v_top < 1.f ? 18446744073709551616.f : 1.f, v_inv = 1.f / (v_top * v_up);
         float top = -INFINITY, sum = 0.f;
-        bool ok = true, fresh = true;  // fresh: nothing kept yet (fp32)
-        int in_run = 0;                // (fp32) blocks since the sums were last added up
+        bool ok = true, fresh = true;  // fresh: nothing kept yet
+        int in_run = 0;                // blocks since the sums were last added up
+        constexpr bool KEEPS = !L::FULL || ONE;
+        using Kept = KeptSums<T, D>;
+        const Kept kept = {o_at, L::FULL ? at + KT : o_at + L::KEPT, L::FULL ? sm + L::HALF_KEPT + r * 256 : nullptr, r};
         // scales of 16 keys each: lanes look up pages two blocks ahead, scales one
         int page_next = 0;
         float ks_next = 0.f, vs_next = 0.f;
@@ -422,10 +487,10 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
             page_of(j + 2);
             const bool hidden = key0 + (j + 1) * KT > least;
             const int see = sees - key0 - j * KT;
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, j & 1), (j >> 1) & 1, abort_flag, status));
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, ONE ? 0 : j & 1), (ONE ? j : j >> 1) & 1, abort_flag, status));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t s_at = at + (j & 1) * KT;
+            const uint32_t s_at = at + (ONE ? 0 : j & 1) * KT;
             float x[KT];
             tmem_ld_x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(x));
             tmem_ld_x32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
@@ -501,27 +566,13 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 if (!ok) break;
                 tc_fence_after();
             }
-            // ---- the sums under the new maximum; (fp32) added to those that are kept ----
-            if constexpr (L::F32) {
-                if (j > 0 && (any || ++in_run == L::FLUSH)) {
-#pragma unroll 1
-                    for (int i = 0; i < D; i += 32) {
-                        uint32_t o[32], m[32];
-                        tmem_ld_x32(o_at + i, o);
-                        tmem_ld_x32(o_at + L::KEPT + i, m);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            m[e] = __float_as_uint((__uint_as_float(o[e]) + (fresh ? 0.f : __uint_as_float(m[e]))) * corr);
-                            o[e] = 0;
-                        }
-                        tmem_st_x32(o_at + L::KEPT + i, m);
-                        tmem_st_x32(o_at + i, o);
-                    }
-                    fresh = false;
-                    in_run = 0;
-                }
-            } else if (any) {
+            // ---- the sums under the new maximum; now and then added to those that are kept ----
+            if (KEEPS && j > 0 && ((any && (L::F32 || !fresh)) || ++in_run >= L::FLUSH)) {
+                if constexpr (L::F32) kept.add(corr, fresh);
+                else add_seldom(kept, corr, fresh);
+                fresh = false;
+                in_run = 0;
+            } else if (!L::F32 && any) {
 #pragma unroll 1
                 for (int i = 0; i < D; i += 32) {
                     uint32_t o[32];
@@ -548,12 +599,12 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         for (int i = 0; i < D; i += 32) {
             uint32_t o[32];  // (of a tile without keys: nothing that is looked at)
             tmem_ld_x32(o_at + i, o);
-            if constexpr (L::F32) {
+            if (KEEPS && !fresh) {
                 uint32_t m[32];
-                tmem_ld_x32(o_at + L::KEPT + i, m);
+                kept.get(i, m);
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) + (fresh ? 0.f : __uint_as_float(m[e])));
+                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(m[e]));
             } else {
                 tmem_wait_ld();
             }
@@ -581,6 +632,15 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         }
         if constexpr (SHARED) reinterpret_cast<float2*>(sm + L::ROW_SCALE)[r] = make_float2(top, ok ? sum : __int_as_float(0x7fc00000));
         tc_fence_before();
+    };
+    if (warp < FIRST) {
+        // ---------------- softmax ----------------
+        if constexpr (L::FULL) {
+            if (lean) softmax(std::true_type{});
+            else softmax(std::false_type{});
+        } else {
+            softmax(std::false_type{});
+        }
     } else if (maker) {
         // ---------------- codes to f16 tiles: 16-byte pieces of a key, a thread always the same piece, of keys own_key + i STEP ----------------
         constexpr int PIECES = D / 16, STEP = L::MAKERS / PIECES, N = KT / STEP;
@@ -649,12 +709,12 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
 #pragma unroll 1
             for (int j = 0; j < blocks && ok; j++) {
                 ok = mbar_wait(k_full(i), phase, abort_flag, status);
-                const uint32_t kd = k_desc + i * (L::KV_TILE >> 4), d = tmem + (j & 1) * KT;
+                const uint32_t kd = k_desc + i * (L::KV_TILE >> 4), d = tmem + place_of(j) * KT;
 #pragma unroll
                 for (int t = 0; t < TILES; t++) {
                     if (!ok || j >= (t == 0 ? blocks0 : blocks1)) continue;
-                    // the weights of block j - 2, which lie there, have been read
-                    ok = mbar_wait(s_free(t, j & 1), ((j >> 1) & 1) ^ 1, abort_flag, status);
+                    // the weights of the block before, which lie there, have been read
+                    ok = mbar_wait(s_free(t, place_of(j)), (turn_of(j) & 1) ^ 1, abort_flag, status);
                     if (!ok) continue;
                     tc_fence_after();
 #pragma unroll
@@ -665,7 +725,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                             for (int kk = 0; kk < 4; kk++)
                                 mma_ss(d + t * 128, q_desc + (((t * PARTS + part) * L::Q_TILE + half * L::Q_HALF) >> 4) + kk * 2, kd + ((half * L::KV_HALF) >> 4) + kk * 2, qk,
                                        part < PARTS - 1 || half > 0 || kk > 0);
-                    umma::commit<1>(s_full(t, j & 1));
+                    umma::commit<1>(s_full(t, place_of(j)));
                 }
                 if (ok) umma::commit<1>(k_free(i));
                 if (++i == NBUF) {
@@ -695,9 +755,9 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 for (int part = PARTS - 1; part >= 0; part--)
 #pragma unroll
                     for (int kk = 0; kk < 4; kk++)
-                        mma_ts(tmem + L::O_AT + t * L::O_PITCH, tmem + t * 128 + (j & 1) * KT + part * 32 + kk * 8, vd + kk * 128, pv, part < PARTS - 1 || kk > 0 ? 1u : j > 0);
+                        mma_ts(tmem + L::O_AT + t * L::O_PITCH, tmem + t * 128 + place_of(j) * KT + part * 32 + kk * 8, vd + kk * 128, pv, part < PARTS - 1 || kk > 0 ? 1u : j > 0);
                 umma::commit<1>(o_done(t));
-                umma::commit<1>(s_free(t, j & 1));
+                umma::commit<1>(s_free(t, place_of(j)));
             }
             if (ok) umma::commit<1>(v_free(i));
             if (++i == NBUF) {

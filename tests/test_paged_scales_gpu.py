@@ -128,3 +128,54 @@ def test_rows_that_see_only_tiny_values(cuda, d):
         for i in (0, 5, 15, 16, 39):
             want, bound = E.attention(q[i: i + 1], cache, torch.tensor([i + 1]), table, d ** -0.5)
             E.close(out[i: i + 1], want, bound)
+
+
+@pytest.mark.parametrize("d,batch,each,total", [(64, 80, 4, 120000), (128, 80, 4, 120000), (128, 80, 2, 120000), (128, 2, 4, 400000), (64, 2, 4, 400000), (128, 80, 4, 16000), (128, 3, 4, 100)])
+def test_sums_over_long_prompts_are_not_cut_off(cuda, d, batch, each, total):
+    """Values of one sign under many keys: what each MMA cuts off its sum is always of the same sign and would add up.  Results are off by roundings to nearest of either sign
+    (weights, results: each at most 2^-11), which in the mean over many results nearly vanish, and by what is cut off: at most 2^-23 for each 16 of 16384 keys, 2^-13.  The mean of
+    N results that are off by at most 2^-10 is off by 2^-10 / sqrt(N) with 6 standard deviations' room: 6 x 2^-10 / sqrt(3) / sqrt(N)."""
+    from rmlk_b200 import kernels as K
+    g = _gen(d, batch, each)
+    page, group = 128, 64
+    cache, _, _ = E.make(1, page, d, [4 * page], cuda, g)
+    cache.v.copy_(cache.v.abs().clamp_min(20))
+    table = torch.randint(0, 4, (batch, -(-total // page)), generator=g).to(torch.int32).to(cuda)  # (pages may be named more than once)
+    n = torch.full((batch,), total, dtype=torch.int32, device=cuda)
+    n[-1] -= 5000 if total > 5000 else 0
+    q = torch.randn(batch * each, group, d, generator=g).to(torch.float16).to(cuda)
+    starts = torch.arange(0, batch * each + 1, each, dtype=torch.int32, device=cuda)
+    out = K.paged_attention(q, cache, n, table, d ** -0.5, starts=starts)
+    for b in (0, batch - 1):
+        rows = slice(b * each, (b + 1) * each)
+        want, _ = E.attention(q[rows], cache, n[b: b + 1], table[b: b + 1], d ** -0.5)
+        off = (out[rows].double() - want) / want
+        assert float(off.abs().max()) < 2 * 2.0 ** -11 + 2.0 ** -13
+        assert abs(float(off.mean())) < 2.0 ** -13 + 6 * 2.0 ** -10 / math.sqrt(3 * off.numel())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_tiles_one_after_the_other(cuda, d):
+    """Two f16 tiles over more keys than they take at once, alone and with the keys shared by a cluster: ragged ends, tiles that see different numbers of keys, first rows that see none."""
+    from rmlk_b200 import kernels as K
+    g = _gen(31, d)
+    page, group = 64, 4
+    for new, total in (([300, 64, 40], [17000, 33333, 60]), ([65] * 60, [16385 + 37 * i for i in range(60)]), ([20000], [19990]), ([64], [140001])):
+        cache, _, _ = E.make(1, page, d, [9 * page], cuda, g)
+        table = torch.randint(0, 9, (len(new), -(-max(total) // page)), generator=g).to(torch.int32).to(cuda)
+        n = torch.tensor(total, dtype=torch.int32, device=cuda)
+        starts = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device=cuda)
+        q = torch.randn(sum(new), group, d, generator=g).to(torch.float16).to(cuda)
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        out = K.paged_attention(q, cache, n, table, d ** -0.5, starts=starts, status=status)
+        assert int(status) == 0
+        for b in sorted({0, len(new) // 2, len(new) - 1}):
+            rows = slice(int(starts[b]), int(starts[b + 1]))
+            if new[b] > 1000:  # some of its rows, as the last ones of shorter sequences
+                for i in (0, 11, 5000, 16500, 19999):
+                    seen = total[b] - new[b] + i + 1
+                    want, bound = E.attention(q[rows][i: i + 1], cache, torch.tensor([seen], device=cuda), table[b: b + 1], d ** -0.5)
+                    E.close(out[rows][i: i + 1], want, bound)
+            else:
+                want, bound = E.attention(q[rows], cache, n[b: b + 1], table[b: b + 1], d ** -0.5)
+                E.close(out[rows], want, bound)
