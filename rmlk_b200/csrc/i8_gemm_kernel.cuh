@@ -73,6 +73,12 @@ __device__ __forceinline__ float scaled(int sum, float a, float b) {
     return t >= 1.17549435e-38f && t < INFINITY ? v * t : v * a * b;
 }
 
+// Copies that are on their way to stage s: waited for before the CTA may leave, also when it has given up.
+__device__ __forceinline__ void wait_for_copies(uint32_t full, uint32_t parity) {
+    for (uint32_t i = 0; i < tc::SPIN_LIMIT; i++)
+        if (tc::mbar_try_wait(full, parity)) return;
+}
+
 struct Tile {
     int n_tile, m_tile;
 };
@@ -150,14 +156,15 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
         if (lane == 0) {
             const uint32_t pair_bar = CG == 2 ? mapa_shared(bars, 0) : bars;  // the pair's full barriers live in its first CTA
             dep_wait();
-            int s = 0, done = 0;
+            int s = 0, asked = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int w = first; w < tiles && ok; w += stride) {
                 const Tile t = tile_at(w, p);
                 for (int kb = 0; kb < nk && ok; kb++) {
-                    if (done++ >= ST) ok = mbar_wait(empty(s), phase ^ 1, abort_flag, p.status);
+                    if (asked >= ST) ok = mbar_wait(empty(s), phase ^ 1, abort_flag, p.status);
                     if (!ok) break;
+                    asked++;
                     if (in_pair == 0) mbar_expect_tx(full(s), CG * L::STAGE);
                     const uint32_t dst = base + s * L::STAGE, bar = pair_bar + 8u * s;
                     load_2d<CG>(dst, &tmW, (kb0 + kb) * KB, (t.n_tile * CG + static_cast<int>(in_pair)) * BN, bar);
@@ -168,10 +175,13 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
                     }
                 }
             }
+            if (in_pair == 0)  // (the pair's bytes all arrive here; its CTAs leave together)
+                for (int i = max(asked - ST, 0); i < asked; i++) wait_for_copies(full(i % ST), (i / ST) & 1);
         }
     } else if (warp == 1) {
         // ---------------- MMAs: one thread of the pair's first CTA ----------------
         if (lane == 0 && in_pair == 0) {
+            dep_wait();  // (a bounded wait that starts before the kernel before this one has ended would count that one's time)
             constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((MT >> 3) << 17) | ((CG * BN >> 4) << 24);  // s8 x s8 -> s32, both k-major
             const uint64_t w_desc0 = smem_desc_k128(base), x_desc0 = smem_desc_k128(base + L::W_BYTES);
             int s = 0, buf = 0;
@@ -215,7 +225,8 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (int w = first; w < tiles && ok; w += stride) {
+        int w = first;
+        for (; w < tiles; w += stride) {
             const Tile t = tile_at(w, p);
             const int64_t n = (static_cast<int64_t>(t.n_tile) * CG + in_pair) * BN + sub * 32 + lane;
             const int64_t m_base = static_cast<int64_t>(t.m_tile) * MT + part * HM;
@@ -254,9 +265,18 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
                 acc_phase ^= 1;
             }
         }
-        if (SPLIT && !ok) {
+        if constexpr (!SPLIT) {  // given up: what has not been written is NaN
+            for (; w < tiles; w += stride) {
+                const Tile t = tile_at(w, p);
+                const int64_t n = (static_cast<int64_t>(t.n_tile) * CG + in_pair) * BN + sub * 32 + lane, m_base = static_cast<int64_t>(t.m_tile) * MT + part * HM;
+                for (int j = 0; j < HM && m_base + j < p.M; j++)
+                    if (n < p.N) static_cast<Out*>(p.out)[(m_base + j) * p.ldo + n] = static_cast<Out>(__int_as_float(0x7fc00000));
+            }
+        } else if (!ok) {  // the cluster's sums are not all there: all of it gives up
 #pragma unroll
             for (int j = 0; j < HM; j++) sums[j] = 0;
+            const uint32_t flag = smem_u32(base_ptr + L::BAR_OFFSET + 8 * L::N_BARS + 8);
+            for (int r = 0; r < splits; r++) asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(mapa_shared(flag, r)), "r"(1) : "memory");
         }
         if constexpr (SPLIT) {
             // CTA r of the cluster adds up tokens r, r + splits, ...: their sums go to its shared memory
@@ -273,7 +293,8 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
     if constexpr (SPLIT) {
         __syncwarp();
         cluster_sync_all();
-        if (warp >= 2 && !*abort_flag && n < p.N) {
+        if (warp >= 2 && n < p.N) {
+            const bool given_up = *abort_flag;
             const int* s = reinterpret_cast<const int*>(base_ptr + L::SUMS) + channel;
             int sum[MOST] = {};
 #pragma unroll 1
@@ -285,7 +306,7 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
             Out* o = static_cast<Out*>(p.out) + n;
 #pragma unroll
             for (int i = 0; i < MOST; i++) {
-                if (at0 + i * ROWS < here) o[(m0 + ((at0 + i * ROWS) << log_splits)) * p.ldo] = static_cast<Out>(scaled(sum[i], sx[i], sw));
+                if (at0 + i * ROWS < here) o[(m0 + ((at0 + i * ROWS) << log_splits)) * p.ldo] = static_cast<Out>(given_up ? __int_as_float(0x7fc00000) : scaled(sum[i], sx[i], sw));
             }
         }
     }
