@@ -12,7 +12,10 @@ constexpr int BK = 32;    // fp32 elements per k-block: one 128-byte row
 constexpr int BN = 128;   // weight columns per CTA = MMA M = TMEM lanes
 // weight-TMA warp, MMA warp, G x 4 converter / epilogue warps, activation-TMA warp
 constexpr int threads_for(int groups) { return 64 + 128 * groups + 32; }
-constexpr uint32_t SPIN_LIMIT = 1u << 20;
+// Attempts of a bounded wait, of 80 ns each as a rule: 5 s.  A product's MMA thread may begin to wait while the kernel before it in the stream still runs (its launch overlaps that one's
+// end), so the limit has to be longer than kernels run; 2^20 attempts, 82 ms, were not.  (Waiting for that kernel's end first costs a decode step 0.5 %: the instructions behind the
+// wait come late.)
+constexpr uint32_t SPIN_LIMIT = 1u << 26;
 constexpr uint32_t TF32_MASK = 0xffffe000u;  // sign, exponent and the 10 mantissa bits a tf32 MMA operand keeps
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
