@@ -523,7 +523,7 @@ typedef struct rmlk_paged_cache {
 /* Puts the keys and values of new tokens into the cache, the keys rotated on the way, and rotates their queries.
  *   k, v: [tokens, kv_heads, head_dim] (f32 or f16), q: [tokens, q_heads, head_dim] or NULL; heads dense, rows *_stride elements apart.
  *   rotation, as rmlk_b200_rope has it: r = x cos[p] + (-x[D/2:], x[:D/2]) sin[p] with rows p = the token's position of the tables cos, sin
- *   [table_rows, head_dim] f32.  Keys: products and sum exact, one rounding to fp32.  Queries, written to q_out: in fp32, the sine's product rounded
+ *   [table_rows, head_dim] f32.  Keys: products exact, their sum rounded to fp64 and that to fp32.  Queries, written to q_out: in fp32, the sine's product rounded
  *   and the cosine's fused with the sum, then rounded to their type.  NULL: keys as they are (and no q).
  * Scale of a block: a power of two, 2^e >= 2^-126, the least with max |value| <= 127 2^e over the new tokens; where the block holds earlier tokens
  * (slots before the first new one) at least its present scale, and where it grows their codes are divided by the ratio, rounded to nearest even.

@@ -1,6 +1,6 @@
 // New keys and values into a paged cache of 8-bit codes, the keys rotated on the way; the queries rotated beside them.
 //
-//   r = x cos[p] + (-x[D/2:], x[:D/2]) sin[p]       (keys: exact, one rounding to fp32; queries: in fp32)
+//   r = x cos[p] + (-x[D/2:], x[:D/2]) sin[p]       (keys: in fp64, then rounded to fp32; queries: in fp32)
 //   2^e: the least power of two with max |r| <= 127 2^e over the new tokens of a block (page, head), at least the block's present scale
 //   code = rne(r 2^-e)
 //
@@ -88,8 +88,9 @@ __device__ __forceinline__ void put_four(__half* p, float4 x) {
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// Keys: four dims of the lower half of a head and the four that go with them, in fp64.  Products of fp32 values are exact there, and the sum is rounded once, so that a key's
-// codes do not depend on how the rotation is computed.  (The conversions cost more than the arithmetic, 8 cycles per warp each: with the queries rotated so too they were the
+// Keys: four dims of the lower half of a head and the four that go with them, in fp64.  Products of fp32 values are exact there; their sum is rounded to fp64 and that to fp32,
+// so that a key's codes do not depend on how the rotation is computed.  (Two roundings: where the sum lies next to the middle of two fp32 numbers, closer than fp64 tells, the result
+// may be the other of them.)  (The conversions cost more than the arithmetic, 8 cycles per warp each: with the queries rotated so too they were the
 // bound, 55 us for 5600 tokens of 32 + 8 heads of 128.)
 struct Rotation {
     double cl[4], sl[4], ch[4], sh[4];
