@@ -544,6 +544,9 @@ RMLK_API int rmlk_b200_paged_append(rmlk_stream_t stream, int dtype, const rmlk_
  * kv_heads, up to 64 for each; rows on 16-byte boundaries.  A row that sees nothing is 0; one that sees a block whose scale is not finite is NaN; one that sees
  * a token whose page is not in [0, pages) or lies behind table_width is NaN, and *status (device word, may be NULL) becomes RMLK_ERR_INVALID_ARG
  * (RMLK_ERR_TIMEOUT: a bounded wait expired).
+ * Sums, maxima and scores are fp32.  The weights exp(s - maximum) that multiply the values keep, for f32, 22 bits; for f16, 16 bits beside the largest among 32 or 64 keys where a
+ * sequence has few rows, 11 bits (they are f16 numbers) where it has many.
+ * Where the scales of V that many rows see span more than 2^10, or one of K or V is below zero or not finite, those rows are taken one by one: right, and hundreds of times slower.
  * Few rows over many keys share the keys out over the whole GPU, where every sequence has as many (starts NULL); with starts at most eight SMs walk along
  * one sequence and head.  So single tokens beside whole prompts are best given to a call of their own.
  * `workspace`: rmlk_b200_paged_attention_workspace_bytes() bytes (0: none is needed) on a 16-byte boundary, zero-filled before its first use; its

@@ -92,10 +92,12 @@ using namespace rmlk;
 // rows, which walks over all their keys.  With P = batch x kv_heads, few_kernel takes the time of P ceil(rows / 16) tiles spread evenly over the GPU, prompt_kernel that of
 // its CTAs, as many at a time as there are SMs.  A CTA with all keys takes as long as `cost` tiles of few_kernel on an SM.  Measured with 8 KV heads over 8000 keys, us (few,
 // prompt), B x rows of a KV head:
-//   f16 128: 1 x 64 26, 28;  1 x 256 63, 40;  1 x 512 111, 61;  8 x 64 112, 156;  8 x 128 210, 159;  8 x 256 404, 186;  64 x 32 407, 604;  64 x 64 793, 603
-//   f32 128: 1 x 64 30, 37;  1 x 256 77, 64;  8 x 64 139, 200;  8 x 128 260, 203;  8 x 256 508, 203;  64 x 32 505, 755;  64 x 64 992, 760
-//   f16 64:  1 x 64 19, 25;  1 x 256 41, 34;  8 x 128 128, 136;  8 x 256 246, 174;  64 x 64 478, 511;  64 x 128 944, 512
-//   f32 64:  1 x 64 21, 32;  1 x 256 48, 42;  8 x 128 150, 187;  8 x 256 287, 246;  64 x 64 564, 764;  64 x 128 1115, 772
+//   f16 128: 1 x 64 29, 30;  1 x 256 69, 41;  1 x 512 120, 61;  8 x 64 121, 100;  8 x 128 227, 103;  8 x 256 436, 113;  64 x 32 437, 610;  64 x 64 854, 611
+//   f32 128: 1 x 64 32, 36;  1 x 256 82, 64;  8 x 64 147, 113;  8 x 128 278, 118;  8 x 256 538, 204;  64 x 32 537, 752;  64 x 64 1051, 757
+//   f16 64:  1 x 64 21, 25;  1 x 256 45, 34;  8 x 64 74, 76;  8 x 128 137, 77;  8 x 256 263, 98;  64 x 64 511, 500;  64 x 128 1006, 503
+//   f32 64:  1 x 64 23, 34;  1 x 256 50, 42;  8 x 64 85, 125;  8 x 128 158, 130;  8 x 256 302, 136;  64 x 64 589, 719;  64 x 128 1165, 723
+// The rule picks the faster one of each but for f16 64, 64 x 64 (2 %).  It knows the table's width, not the lengths: over 600 keys, for which few_kernel's start and joins count most,
+// its choice of few_kernel is up to 1.6 times as slow as the other (f16 64: 64 x 64 95, 60; 8 x 64 20, 14; f16 128: 64 x 32 98, 71), under a table of 8000 or 131072 keys alike.
 // The new tokens of ragged sequences lie at places that only the device knows: they go to prompt_kernel.
 static bool takes_few(bool f32, int64_t tokens, int64_t batch, int64_t kv_heads, int64_t group, int64_t head_dim, int64_t most_keys, bool ragged) {
     if (ragged || batch < 1) return false;
@@ -135,8 +137,9 @@ extern "C" int rmlk_b200_paged_attention(rmlk_stream_t stream, int dtype, const 
     if (takes_few(dtype == RMLK_F32, tokens, batch, c.kv_heads, a.group, c.d, s.width << c.page_log, starts != nullptr)) {
         if (!workspace || workspace_bytes < paged::few_workspace(c.d) || !aligned_to(workspace, 16))
             return fail(RMLK_ERR_INVALID_ARG, "paged_attention: the workspace is missing, too small or misaligned (rmlk_b200_paged_attention_workspace_bytes)");
-        // tiles of 8 or 16 rows; one of 16 takes 1.4 times as long.  24 x 4 tokens, 6 heads of 128 to each of 4, 1500 keys, f16: three of 8 27 us, two of 16 29; 16 rows: 22, 18; 40 rows
-        // (2 requests, 8 KV heads, 20000 keys): 61, 60
+        // Tiles of 8 or 16 rows; one of 16 takes 1.6 times as long over long contexts, where the keys come from HBM, 1.9 times over short ones.  In tiles of 8, of 16, us: 24 rows (24
+        // requests, 4 KV heads, 1500 keys) f16 64 20.5, 25.3, f16 128 28.3, 35.2, f32 64 22.4, 26.3, f32 128 33.0, 40.6; over 8000 keys 56, 60; 87, 95; 64, 68; 109, 115.  16 rows (32 requests,
+        // 8 heads, 2000 keys): 31.7, 31.3; 49.8, 47.1; 35.8, 34.1; 60.4, 56.0.  40 rows (2 requests, 8 heads, 20000 keys): 41, 43; 64, 66; 47, 47; 78, 78.
         const int rows = s.each * a.group;
         const bool one = rows <= 8 || (rows > 16 && rows <= 24);
         if (dtype == RMLK_F32) {

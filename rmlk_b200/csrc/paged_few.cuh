@@ -27,9 +27,10 @@
 // A step's sums, joined from the digits, times exp2(m - running maximum) and the page's scale are added to fp32 sums.  The order of a contraction is free, so 16
 // consecutive bytes of a key are a lane's operands of two MMAs.
 //
-// Measured: 3 requests over 50001 to 33334 keys, f16, 8 KV heads of 128: 55 us, 4.7 TB/s of the call and 6.3 to 7 TB/s between its ends; the rest is the start (which sequence,
-// which page, first data: 5 us) and the joining of the parts (4 us).  64 requests over 1000 to 508 keys, fp32, 8 heads of 64: 22 us, with the whole CTA waiting at the end of each
-// segment 24.  24 requests of 4 tokens over 2000 to 1042 keys, f16, 6 heads to each of 4: 29 us; 24 query rows are three tiles of 8, each of which takes the keys once more, from L2.
+// Measured: 3 requests over 50001 to 33334 keys, f16, 8 KV heads of 128: 53.5 us, 4.8 TB/s of the call and more between its ends; the rest is the start (which sequence, which page,
+// first data: 5 us) and the joining of the parts (4 us).  64 requests over 1000 to 508 keys, fp32, 8 heads of 64: 23.3 us; with the whole CTA waiting at the end of each segment it
+// took 2 us more.  24 requests of 4 tokens over 2000 to 1042 keys, f16, 6 heads to each of 4: 29.9 us; 24 query rows are three tiles of 8, each of which takes the keys once more,
+// from L2.  64 requests over 8000 keys, f16, 8 heads of 128: 174 us; where all steps form their scores in fp32, 1235.
 #pragma once
 
 #include "paged.cuh"

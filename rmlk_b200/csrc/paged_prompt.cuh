@@ -2,7 +2,8 @@
 //
 // A CTA keeps two tiles (fp32 with 128 values: one) of 128 query rows of one KV head - the rows of the query heads that share it lie behind one another - and walks over the
 // keys that they see in blocks of 64.  Both contractions run on tcgen05.mma kind::f16: codes are exact in f16, f16 queries too; fp32 queries and, for fp32 results, weights are two
-// f16 numbers each (the second the rounding error of the first), whose products go to the same accumulator.
+// f16 numbers each (the second the rounding error of the first), whose products go to the same accumulator.  For f16 results a weight is one f16 number, off by at most 2^-11 of itself,
+// while the weights' sum is that of the fp32 ones: the result is off by some 2e-4 before it is rounded, as much as that rounding does; second numbers would add half as many MMAs again.
 //   warps 0-3, 4-7   softmax of a tile, one thread to a row: scores out of TMEM, weights back into TMEM in their place, where the values' MMAs take them as their first operand
 //   warps 8-11       codes of K and V from the pages into f16 tiles, three of each: the codes are turned once for both tiles
 //   warps 12, 13     one thread of each issues the MMAs of the scores, up to two blocks ahead of the softmax, and those of the values
@@ -10,7 +11,7 @@
 // over distributed shared memory.
 // What was tried, f16, 4 prompts of up to 1024 tokens, 32 heads of 128, behind up to 5000 keys: one thread for all MMAs and the weights through shared memory 445 us (the thread needs some 70
 // cycles per MMA: it was the bound); two CTAs of one tile per SM, blocks of 128 keys with the scores behind the values 433 us (half of a CTA's time is MMAs, during which its softmax
-// waits), blocks of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); as it is 330 us, 0.70 PFLOP/s.
+// waits), blocks of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); as it is 339 us, 0.69 PFLOP/s.
 // What bounds it there: instructions (49 % of all issue slots: a score is scaled, compared, exponentiated and packed, a code turned) beside the tensor pipe (36 % of its cycles), which
 // wait for one another at the ends of a block.
 // 16 prompts of up to 512 tokens, fp32, 32 heads of 64: 90 us.  A CTA has 4 blocks on average, so starting (queries turned into f16 pairs) and storing are half of it; with the pages
@@ -20,8 +21,9 @@
 // fp32 sums every 256 keys for fp32 results, every 4096 for f16.  Those are in TMEM too, where two f16 tiles of 128 values leave no room: up to 16384 keys of a CTA they do without,
 // 1.0e-4 of a sum; over more, scores have one place instead of two, and the sums of one half of the values go to the other, those of the other half to shared memory.  4 prompts of 1024
 // tokens, 32 heads of 128: over 16000 keys 1.39 ms, over 20000 2.16, where sums that are cut off took 1.71.
-// Scales of K go into the scores' factor, scales of V into the weights, relative to the largest that the rows see.  Where scales of V span more than 2^10, or
-// something is not finite or has no page, the rows are taken one by one in fp32 (row_in_fp32): slow, and right for everything.
+// Scales of K go into the scores' factor, scales of V into the weights, relative to the largest that the rows see.  Where scales of V span more than 2^10, some
+// are below zero, or something is not finite or has no page, the rows are taken one by one in fp32 (row_in_fp32): right for everything, and
+// hundreds of times slower (0.36 us per key and row of 64 values, a row to each of the CTA's warps).
 #pragma once
 
 #include "paged.cuh"
@@ -592,9 +594,9 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         tc_fence_after();
         // (the sums of a share go to where the operands of both tiles were)
         if constexpr (SHARED) asm volatile("bar.sync 3, %0;" ::"n"(ROWS) : "memory");
-        const float inv = 1.f / sum;  // (not times v_top: that could leave the normal numbers although the result does not)
+        [[maybe_unused]] const float inv = 1.f / sum;  // (not times v_top: that could leave the normal numbers although the result does not)
         const int row = row0 + r, token = token_of(row);
-        T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D;
+        [[maybe_unused]] T* dst = static_cast<T*>(a.out) + (first + token) * a.os + (static_cast<int64_t>(h) * a.group + row - token * a.group) * D;
 #pragma unroll 1
         for (int i = 0; i < D; i += 32) {
             uint32_t o[32];  // (of a tile without keys: nothing that is looked at)
