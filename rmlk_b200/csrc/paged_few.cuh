@@ -18,8 +18,8 @@
 //           f16: values above 2^-11 of the largest are held as they are.  What the others lose is summed up for each row; where it could move a score's exponent by more than
 //           2^-13 in some key of the step, all codes of which were +-128, the step goes to fp32.  (With two digits, 15 bits, keys that have no part in a query's few outliers
 //           of 16 to 33 times the rest came out up to 1.2 % off.)
-//           fp32: every value loses something, next to nothing beside its score as a rule.  A step goes to fp32 where the root of the sum of squares of what is lost, times codes of
-//           128, could move an exponent by more than 2^-16: scores of some tens for ordinary rows.  (A rule on a row's values alone, whether a few are far larger than the rest,
+//           fp32: every value loses something, next to nothing beside its score as a rule.  A step goes to fp32 where that, 1 / sqrt(12) of a step each and a root of their sum of
+//           squares, times codes of 128, could move an exponent by more than 2^-16: scores of some tens for ordinary rows.  (A rule on a row's values alone, whether a few are far larger than the rest,
 //           let rows pass half of whose values were 300 times the others; with keys that had no part in those the result was 12 % off.)
 //   values  O^T[16 dims x 8 rows] = V^T P^T.  Weights exp2(s - m), m the row's largest score in the step, are fixed-point numbers of 16 bits (f16 results) or 23
 //           (fp32): half a step is 2^-17 or 2^-24 of the largest weight of the step.  Unsigned digits, an MMA each; the accumulator fragment of S holds just the
@@ -525,17 +525,15 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             const float up = exp2_int(e), more = 256.f;
             // an infinity or a NaN makes NaN of the row
             factor[r] = most < 0x7f800000u ? a.scale * 1.44269504f / more * exp2_int(-e) : __int_as_float(0x7fc00000);
-            // what three digits leave of the lane's values, in steps: f16 its size, fp32 its square; f16 also squares of the third digits
-            float rest = 0.f;
+            float rest = 0.f;  // (f16) what three digits leave of the lane's values, in steps; squares of the third digits
             int thirds = 0;
 #pragma unroll
             for (int s = 0; s < 4 * PIECES; s++) {
                 const float4 x = four(s);
                 const int v[4] = {__float2int_rn(x.x * up * more), __float2int_rn(x.y * up * more), __float2int_rn(x.z * up * more), __float2int_rn(x.w * up * more)};
-                const float4 left = make_float4(x.x * up * more - static_cast<float>(v[0]), x.y * up * more - static_cast<float>(v[1]), x.z * up * more - static_cast<float>(v[2]),
-                                                x.w * up * more - static_cast<float>(v[3]));
-                if constexpr (L::F32) rest += (left.x * left.x + left.y * left.y) + (left.z * left.z + left.w * left.w);
-                else rest += (fabsf(left.x) + fabsf(left.y)) + (fabsf(left.z) + fabsf(left.w));
+                if constexpr (!L::F32)
+                    rest += (fabsf(x.x * up * more - static_cast<float>(v[0])) + fabsf(x.y * up * more - static_cast<float>(v[1]))) +
+                            (fabsf(x.z * up * more - static_cast<float>(v[2])) + fabsf(x.w * up * more - static_cast<float>(v[3])));
                 // signed digits: the byte of v + 0x80 (+ 0x8000) carries what the digits below borrow
                 const uint32_t d0 = bytes_of<0>(v[0], v[1], v[2], v[3]), d1 = bytes_of<1>(v[0] + 0x80, v[1] + 0x80, v[2] + 0x80, v[3] + 0x80);
                 uint32_t(&f)[L::QT][4] = qf[s >> 1];
@@ -547,7 +545,8 @@ __global__ void __launch_bounds__(128, Few<T, D, NR>::PER_SM) few_kernel(const C
             }
             // (a row that is NaN has no part in these)
             if constexpr (L::F32) {
-                lost = fmaxf(lost, sqrtf(quad_sum(rest)) * fabsf(factor[r]) * (128.f * 8.f));  // (the limit is 2^-16 for it)
+                // a step / sqrt(12) for each value; the limit is 2^-16 for it
+                if (most > 0) lost = fmaxf(lost, fabsf(factor[r]) * ((D == 64 ? 2.3094011f : 3.2659863f) * 128.f * 8.f));
             } else {
                 lost = fmaxf(lost, quad_sum(rest) * fabsf(factor[r]) * 128.f);
                 lost_by_two = fmaxf(lost_by_two, sqrtf(quad_sum(static_cast<float>(thirds))) * fabsf(factor[r]) * 128.f);
