@@ -23,7 +23,8 @@
 // tokens, 32 heads of 128: over 16000 keys 1.39 ms, over 20000 2.16, where sums that are cut off took 1.71.
 // Scales of K go into the scores' factor, scales of V into the weights, relative to the largest that the rows see.  Where scales of V span more than 2^10, some
 // are below zero, or something is not finite or has no page, the rows are taken one by one in fp32 (row_in_fp32): right for everything, and
-// hundreds of times slower (0.36 us per key and row of 64 values, a row to each of the CTA's warps).
+// hundreds of times slower (0.36 us per key and row of 64 values, a row to each of the CTA's warps).  So are, at the end and by themselves, fp32 rows whose values differ in size by so
+// much that two f16 numbers lose what the scores need (rows_again).
 #pragma once
 
 #include "paged.cuh"
@@ -119,6 +120,27 @@ __device__ __noinline__ void row_in_fp32(const Cache& c, const Batch& q, const A
     T* o = static_cast<T*>(a.out) + row * a.os + static_cast<int64_t>(h) * D;
 #pragma unroll
     for (int i = 0; i < N; i++) o[lane + 32 * i] = static_cast<T>(sees <= 0 ? 0.f : acc[i] / sum);
+}
+
+// (fp32) What the second f16 number of a query's values leaves, up to half of f16's least step, may move an exponent by more than 2^-16: 1 / sqrt(12) of a step each and a root of
+// their sum of squares, times codes of 128 under the largest scale of K.  Only where scores would be millions, if the row's values were of one size.
+template <int D>
+__device__ __forceinline__ bool pairs_lose(float step, float k_top, float scale) {
+    return 5.9604645e-8f * (D == 64 ? 2.3094011f : 3.2659863f) * 128.f * step * (fabsf(scale) * 1.44269504f * k_top) > 1.52587890625e-5f;
+}
+// Those of the rows first_row, first_row + every, ... that pairs hold too little of, again.
+template <typename T, int D>
+__device__ __noinline__ void rows_again(const Cache& c, const Batch& q, const Attend& a, int b, int64_t first, int h, int row0, int rows, int first_row, int every, int before, int keys, float k_top) {
+    const int lane = threadIdx.x & 31;
+    for (int r = first_row; r < rows; r += every) {
+        const int row = row0 + r, token = row / a.group, head = h * a.group + row - token * a.group;
+        const T* src = static_cast<const T*>(a.q) + (first + token) * a.qs + static_cast<int64_t>(head) * D;
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) most = max(most, finite_abs_bits(static_cast<float>(src[lane + 32 * i])));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (most > 0 && pairs_lose<D>(exp2_int(-scale_exponent(most)), k_top, a.scale)) row_in_fp32<T, D>(c, q, a, b, first + token, head, min(before + token + 1, keys));
+    }
 }
 
 // two fp32 operations by one instruction
@@ -325,7 +347,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
 
     // ---- while the softmax's warps bring the queries, the others look at the pages: all there, scales finite and not below zero, those of V of one size? ----
     if (warp >= FIRST) {
-        float v_top = 0.f, v_low = INFINITY;
+        float v_top = 0.f, v_low = INFINITY, k_top = 0.f;
         bool plain = true;
         const int pages = (seen + c.page - 1) >> c.page_log;
         for (int i = tid - ROWS; i < pages; i += OTHERS) {
@@ -336,12 +358,17 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 const int64_t block = static_cast<int64_t>(p) * c.kv_heads + h;
                 const float k = c.ks[block], v = c.vs[block];
                 plain = plain && k >= 0.f && k < INFINITY && v >= 0.f && v < INFINITY;
+                k_top = fmaxf(k_top, k);
                 v_top = fmaxf(v_top, v);
                 if (v > 1.17549435e-38f) v_low = fminf(v_low, v);  // 2^-126: the scale of a block of zeros
             }
         }
         const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(v_top)), l = __reduce_min_sync(0xffffffffu, __float_as_uint(v_low));
         plain = __all_sync(0xffffffffu, plain);
+        if constexpr (L::F32) {
+            const uint32_t k = __reduce_max_sync(0xffffffffu, __float_as_uint(k_top));
+            if (lane == 0) s_red[2 * (OTHERS / 32) + warp - FIRST] = k;
+        }
         if (lane == 0) {
             s_red[2 * (warp - FIRST)] = t;
             s_red[2 * (warp - FIRST) + 1] = plain ? l : 0u;  // (0: no lower end, never of one size)
@@ -366,6 +393,7 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
                 mbar_init(o_done(t), 1);
             }
             *abort_flag = 0;
+            s_red[31] = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         asm volatile("bar.sync 2, %0;" ::"n"(OTHERS) : "memory");
@@ -454,6 +482,18 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         const float q_scale = fabsf(a.scale) * 1.44269504f * (L::F32 ? s_row[r] : 1.f);
         // v / v_top: the reciprocal of a number near the lower end of fp32 would be infinite, of 2^64 times it is not
         const float v_up = v_top < 1.f ? 18446744073709551616.f : 1.f, v_inv = 1.f / (v_top * v_up);
+        if constexpr (L::F32) {
+            float k_top = 0.f;
+            for (int w = 0; w < OTHERS / 32; w++) k_top = fmaxf(k_top, __uint_as_float(s_red[2 * (OTHERS / 32) + w]));
+            if (pairs_lose<D>(s_row[r], k_top, a.scale)) {
+                // what is needed to form such rows again, at the end (kept in registers until then it cost 3 %; every row writes the same)
+                const uint32_t note[9] = {static_cast<uint32_t>(b), static_cast<uint32_t>(h), static_cast<uint32_t>(row0), static_cast<uint32_t>(rows), static_cast<uint32_t>(before),
+                                          static_cast<uint32_t>(keys), static_cast<uint32_t>(first), static_cast<uint32_t>(first >> 32), __float_as_uint(k_top)};
+#pragma unroll
+                for (int i = 0; i < 9; i++) s_red[22 + i] = note[i];
+                s_red[31] = 1;
+            }
+        }
         float top = -INFINITY, sum = 0.f;
         bool ok = true, fresh = true;  // fresh: nothing kept yet
         int in_run = 0;                // blocks since the sums were last added up
@@ -810,6 +850,13 @@ __global__ void __launch_bounds__(Prompt<T, D>::THREADS, 1) prompt_kernel(const 
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
+    // (behind the barrier: every row has its first result; where a cluster shares the keys, from this CTA)
+    if constexpr (L::F32)
+        if (s_red[31]) {
+            const int by = SHARED ? cluster : 1, own = SHARED ? static_cast<int>(blockIdx.x) % by : 0;
+            rows_again<T, D>(c, q, a, s_red[22], static_cast<int64_t>(s_red[29]) << 32 | s_red[28], s_red[23], s_red[24], s_red[25], own + by * (threadIdx.x >> 5), by * (L::THREADS / 32), s_red[26],
+                             s_red[27], __uint_as_float(s_red[30]));
+        }
 }
 
 }  // namespace paged

@@ -81,3 +81,20 @@ def test_fp32_queries_of_two_sizes(cuda, d, each, group):
         out = K.paged_attention(q, cache, n, table, scale * d ** -0.5)
         want, bound = E.attention(q, cache, n, table, scale * d ** -0.5)
         E.close(out, want, 4 * bound)  # (scores in fp32: D roundings of 2^-24, where the bound counts D / 16 + 8 of 2^-23)
+
+
+@pytest.mark.parametrize("d,group,new,total", [(64, 4, [70, 40], [500, 900]), (128, 2, [100, 130], [100, 2000]), (64, 3, [130] * 30, [130 + 11 * i for i in range(30)]), (128, 4, [65] * 30, [200] * 30)])
+def test_fp32_queries_of_two_sizes_in_prompts(cuda, d, group, new, total):
+    """The same for whole prompts, alone and with the keys shared by a cluster, with rows of one size beside them."""
+    from rmlk_b200 import kernels as K
+    g = _gen(d, group, len(new))
+    cache, table, n = E.make(2, 32, d, total, cuda, g)
+    cache.k[..., ::2] = 0
+    starts = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device=cuda)
+    x = torch.randn(sum(new), 2 * group, d, generator=g)
+    for large, small, scale in ((1e4, 1.0, 1.0), (1e7, 1.0, 1.0), (1e9, 1.0, 1.0), (1e9, 1e-6, 1e6), (1e30, 1.0, 1.0)):
+        q = x * small
+        q[::3, :, ::2] = x[::3, :, ::2] * large
+        out = K.paged_attention(q.to(cuda), cache, n, table, scale * d ** -0.5, starts=starts)
+        want, bound = E.attention(q.to(cuda), cache, n, table, scale * d ** -0.5, starts)
+        E.close(out, want, 4 * bound)  # (scores in fp32: D roundings of 2^-24, where the bound counts D / 16 + 8 of 2^-23)
