@@ -8,7 +8,7 @@
 // tcgen05.mma kind::i8 behind TMA, laid out as the f16 product is (umma_gemm.cu): a CTA owns 128 channels - the MMA's M, one TMEM lane each - and a tile of MT
 // tokens, the MMA's N; a pair of CTAs (cta_group::2) shares 256 channels.  Both operands have k along their rows, 128 bytes to a swizzled row.
 // What bounds it: for many tokens the tensor pipe; for few the weights' bytes, which is why a product with fewer tiles than SMs is shared along k by a cluster.
-// Measured, m x k x n: 4096 x 4096 x 14336 in f16 180 us, 2.67 POP/s; 64 x 2048 x 16384 in f32 11.4 us, 3.3 TB/s (a wave of 128 CTAs, 16 blocks of k each: the first bytes and
+// Measured, m x k x n: 4096 x 4096 x 14336 in f16 181 to 186 us, 2.6 POP/s; 64 x 2048 x 16384 in f32 11.5 us, 3.3 TB/s (a wave of 128 CTAs, 16 blocks of k each: the first bytes and
 // the last sums are half of it); 1 x 2048 x 2048 3.7 us.
 #include "umma_gemm.h"
 

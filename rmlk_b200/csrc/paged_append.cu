@@ -8,8 +8,9 @@
 // that after any number of steps a code is off by less than one step of the final scale (1/2 + 1/4 + ...); ratios of any size would add half a step
 // each time.  It costs up to one bit of the eight (a scale of max / 127 is up to twice as fine).
 //
-// What bounds it: HBM, q, k, v and the tables' rows read and q and the codes written once.  5600 tokens of 32 + 8 + 8 heads of 128, f16: 35 us, 3.8 TB/s; the values wait in
-// registers for their block's maximum (64 of them with a few spilled, 38 us with the 80 that it would take), and the keys' conversions to fp64 and back take their time.
+// What bounds it: the floor is HBM's, q, k, v and the tables' rows read and q and the codes written once.  5600 tokens of 32 + 8 + 8 heads of 128, f16: 36 us, 3.7 TB/s, with instructions in
+// 62 % of all issue slots and 45 % of the warps there could be.  Keys and values wait in registers for their block's maximum (64 of them with a few spilled, 38 us with the 80 that it would
+// take), and the keys' conversions to fp64 and back take their time; queries, most of the bytes, wait for nothing but share the instance and its registers.
 #include <algorithm>
 
 #include "paged.cuh"
