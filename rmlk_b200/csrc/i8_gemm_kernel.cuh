@@ -70,7 +70,7 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_
 // result does not.
 __device__ __forceinline__ float scaled(int sum, float a, float b) {
     const float v = static_cast<float>(sum), t = a * b;
-    return t >= 1.17549435e-38f && t < INFINITY ? v * t : v * a * b;
+    return fabsf(t) >= 1.17549435e-38f && fabsf(t) < INFINITY ? v * t : v * a * b;
 }
 
 // Copies that are on their way to stage s: waited for before the CTA may leave, also when it has given up.
