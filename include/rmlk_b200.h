@@ -526,7 +526,7 @@ typedef struct rmlk_paged_cache {
  *   [table_rows, head_dim] f32.  Keys: products exact, their sum rounded to fp64 and that to fp32.  Queries, written to q_out: in fp32, the sine's product rounded
  *   and the cosine's fused with the sum, then rounded to their type.  NULL: keys as they are (and no q).
  * Scale of a block: a power of two, 2^e >= 2^-126, the least with max |value| <= 127 2^e over the new tokens; where the block holds earlier tokens
- * (slots before the first new one) at least its present scale, and where it grows their codes are divided by the ratio, rounded to nearest even.
+ * (slots before the first new one) at least its present scale, below zero if that is, and where it grows their codes are divided by the ratio, rounded to nearest even.
  * Codes are value / 2^e rounded to nearest even.  A block that receives an infinity or a NaN gets the scale NaN - what attends to it is NaN -
  * until it is begun anew in its first slot.  Positions below 0 (lens[b] less than the new tokens) are passed over.
  * A token whose page is not in [0, pages), which lies behind table_width pages or table_rows positions is not stored, its query is not

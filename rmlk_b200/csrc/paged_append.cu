@@ -257,9 +257,10 @@ __global__ void __launch_bounds__(256, ITERS <= 2 ? 4 : 2) append_kernel(const C
         __syncwarp();  // every lane has read the old scale
     }
     float s = least_scale(m);
-    if (!(s > old)) s = s != s ? s : old;  // (a NaN of either stays)
+    if (!(s > fabsf(old))) s = s != s ? s : fabsf(old);  // (a NaN of either stays)
+    if (old < 0.f) s = -s;                               // (the codes that are there keep their sign)
     if (me == 0) *scale = s;
-    if (slot0 > 0 && s > old) {  // the codes that are there, under the larger scale
+    if (slot0 > 0 && fabsf(s) > fabsf(old)) {  // the codes that are there, under the larger scale
         const float ratio = old / s;
         for (int i = me; i < slot0 * D / 4; i += GROUP) {
             const uint32_t w = reinterpret_cast<uint32_t*>(dst)[i];
