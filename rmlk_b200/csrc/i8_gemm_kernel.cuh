@@ -73,12 +73,6 @@ __device__ __forceinline__ float scaled(int sum, float a, float b) {
     return fabsf(t) >= 1.17549435e-38f && fabsf(t) < INFINITY ? v * t : v * a * b;
 }
 
-// Copies that are on their way to stage s: waited for before the CTA may leave, also when it has given up.
-__device__ __forceinline__ void wait_for_copies(uint32_t full, uint32_t parity) {
-    for (uint32_t i = 0; i < tc::SPIN_LIMIT; i++)
-        if (tc::mbar_try_wait(full, parity)) return;
-}
-
 struct Tile {
     int n_tile, m_tile;
 };
@@ -176,7 +170,7 @@ __global__ void __launch_bounds__(Layout<CG, MT, ST, SPLIT>::THREADS, 1) gemm_ke
                 }
             }
             if (in_pair == 0)  // (the pair's bytes all arrive here; its CTAs leave together)
-                for (int i = max(asked - ST, 0); i < asked; i++) wait_for_copies(full(i % ST), (i / ST) & 1);
+                for (int i = max(asked - ST, 0); i < asked; i++) tc::wait_for_copies(full(i % ST), (i / ST) & 1);
         }
     } else if (warp == 1) {
         // ---------------- MMAs: one thread of the pair's first CTA ----------------

@@ -51,6 +51,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// Copies on their way to a stage: waited for before the CTA may leave, also when it has given up.
+__device__ __forceinline__ void wait_for_copies(uint32_t full, uint32_t parity) {
+    for (uint32_t i = 0; i < SPIN_LIMIT; i++)
+        if (mbar_try_wait(full, parity)) return;
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)

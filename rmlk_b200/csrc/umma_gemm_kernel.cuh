@@ -266,6 +266,9 @@ __global__ void __launch_bounds__(Layout<CG, SPLIT, MT, ST>::REGS_FOR, 1) gemm_k
                     }
                 }
             }
+            // A CTA that has given up waits for its copies all the same.  (A pair's all arrive in its first CTA, and its CTAs leave together.)
+            if (rank == 0 && *abort_flag)
+                for (int i = max(done - ST, 0); i < done; i++) tc::wait_for_copies(full(i % ST), (i / ST) & 1);
         }
     } else if (warp == 1) {
         // ---------------- MMAs: one thread of the pair's first CTA ----------------
