@@ -11,7 +11,7 @@
 // over distributed shared memory.
 // What was tried, f16, 4 prompts of up to 1024 tokens, 32 heads of 128, behind up to 5000 keys: one thread for all MMAs and the weights through shared memory 445 us (the thread needs some 70
 // cycles per MMA: it was the bound); two CTAs of one tile per SM, blocks of 128 keys with the scores behind the values 433 us (half of a CTA's time is MMAs, during which its softmax
-// waits), blocks of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); as it is 339 us, 0.69 PFLOP/s.
+// waits), blocks of 64 with the scores ahead 442 us (the codes are turned twice: half of all instructions); as it is 336 us, 0.70 PFLOP/s.
 // What bounds it there: instructions (49 % of all issue slots: a score is scaled, compared, exponentiated and packed, a code turned) beside the tensor pipe (36 % of its cycles), which
 // wait for one another at the ends of a block.
 // 16 prompts of up to 512 tokens, fp32, 32 heads of 64: 90 us.  A CTA has 4 blocks on average, so starting (queries turned into f16 pairs) and storing are half of it; with the pages
